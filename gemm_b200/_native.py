@@ -124,6 +124,19 @@ def stream() -> int:
     return _raw_stream(_device())
 
 
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` (a CUDA device with an index) is the current one."""
+    if _device is None:
+        _bind_torch()
+    if device.index == _device():
+        return _same_device
+    import torch
+    return torch.cuda.device(device)
+
+
 _status_ptrs = {}
 
 

@@ -1,0 +1,480 @@
+// One token per row of logits from a given uniform number, with the row's own temperature T, top-k, top-p and min-p.
+//
+//   w_i = 2^((x_i - max x) log2(e) / T).  In the order (x descending, id ascending): the first top_k ids; of these the ids that have less than top_p of the
+//   mass in front of them; of these the ids with w_i >= min_p.  The draw is the first id, in id order, at which the mass so far exceeds u times the kept mass.
+//
+// All three filters cut that order at one place, so what is kept is {key > tau} and the first m ids with key = tau.  No sort: tau comes from a histogram over
+// 1/16-wide steps below the maximum and a radix search over the keys of the step that holds the cut.
+//
+// Masses are whole numbers: w_i is rounded to a multiple of 2^-44 (the rounding moves a border of the draw by 2^-45 of the largest weight; 2^18 of them stay
+// below 2^63).  Sums are then exact in any order: the atomics of the histograms, the split over blocks and the order of the warps change nothing, and the
+// draw agrees with one in 64-bit floats except where u falls within some 1e-12 of a border (32-bit sums over a vocabulary: a row in a thousand).
+// 2^t: table of 2^(j/32) and a polynomial of degree 5 for the rest (P. T. P. Tang, "Table-driven implementation of the exponential function", 1989), in 64-bit floats.
+//
+// A cluster of up to eight blocks holds a row in its shared memory (bulk copies), so that HBM is read once whatever the number of passes; block totals and
+// histograms are exchanged through distributed shared memory, and every block reduces them for itself: one cluster barrier per step.
+#include "sm100.cuh"
+#include "host_common.h"
+#include <float.h>
+#include <algorithm>
+
+namespace gb {
+
+constexpr int kDrThreads = 512, kDrWarps = 16;
+constexpr int kDrBins = 512;               // steps of 1/16 below the maximum; the last one takes all that lies further down
+constexpr int kDrList = 256;               // candidates a warp lists
+constexpr int kDrMass = 44;                // fraction bits of a weight
+
+struct DrawArgs {
+  const void* logits;
+  long ld;
+  int rows, vocab, ctas, per;              // blocks per row, ids per block
+  const float* u;
+  const float* temperature; const int* top_k; const float* top_p; const float* min_p;      // per row; null: the value for all rows
+  float temperature_all; int top_k_all; float top_p_all, min_p_all;
+  int* out; float* logprob;                // logprob: null = not wanted
+  KernelStatus* status;
+};
+
+struct DrawShared {
+  unsigned count[2][kDrBins];              // histogram, by step parity
+  unsigned lo[2][kDrBins], hi[2][kDrBins]; // its masses in two words
+  double table[32];
+  unsigned long long warp_mass[kDrWarps];
+  int warp_ties[kDrWarps];
+  unsigned long long scan[kDrWarps];
+  unsigned long long found_before;
+  int found_at;
+  float red[kDrWarps];
+  float max_x;                             // this block's, read by the others
+  int first_max;
+  unsigned long long total[2];             // this block's kept mass, read by the others
+  int ties;
+  int list_n[kDrWarps];
+  uint64_t bar;
+  int abort_flag;
+  unsigned short list[kDrWarps][kDrList];
+};
+
+__device__ __forceinline__ uint32_t dr_mapa(uint32_t addr, int cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ uint32_t dr_peer32(const void* p, int cta) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long dr_peer64(const void* p, int cta) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void dr_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Order-preserving integer of a logit: larger logit, larger key.
+template <typename T> struct DrawKey;
+template <> struct DrawKey<float> {
+  static __device__ __forceinline__ float value(float v) { return v == v ? v : -INFINITY; }              // NaN is never drawn
+  static __device__ __forceinline__ unsigned of(float v) { const unsigned u = __float_as_uint(v + 0.0f); return (u & 0x80000000u) ? ~u : (u | 0x80000000u); }
+};
+template <> struct DrawKey<__nv_bfloat16> {
+  static __device__ __forceinline__ float value(__nv_bfloat16 b) { const float v = __bfloat162float(b); return v == v ? v : -INFINITY; }
+  static __device__ __forceinline__ unsigned of(float v) { return DrawKey<float>::of(v) >> 16; }         // (the value is a bf16: nothing is lost, and the order stays)
+};
+
+// 2^t in units of 2^-44, for t <= 0; t = -46 and below (and NaN): 0.
+__device__ __forceinline__ unsigned long long dr_weight(double t, const double* table) {
+  if (!(t > -46.0)) return 0;
+  constexpr double kRound = 6755399441055744.0;                   // 1.5 * 2^52: the sum's low bits are the rounded number
+  const double m = fma(t, 32.0, kRound);
+  const int k = __double2loint(m);
+  const double r = t - (m - kRound) * 0.03125;                    // |r| <= 1/64
+  // 2^r = sum (r ln 2)^n / n!
+  constexpr double c1 = 0.69314718055994531, c2 = 0.24022650695910072, c3 = 0.05550410866482158, c4 = 0.009618129107628477, c5 = 0.0013333558146428443;
+  double p = fma(r, c5, c4);
+  p = fma(r, p, c3); p = fma(r, p, c2); p = fma(r, p, c1); p = fma(r, p, 1.0);
+  p *= table[k & 31];
+  p = __hiloint2double(__double2hiint(p) + ((k >> 5) + kDrMass) * 1048576, __double2loint(p));     // times 2^(k >> 5), in units
+  return (unsigned long long)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;    // 2^52: rounded to a whole number
+}
+
+// Exclusive position of `target` in the running sum of the 512 threads' values: the thread with before < target <= before + v stores itself.
+__device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long target, DrawShared& s) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned long long incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
+  if (lane == 31) s.scan[warp] = incl;
+  if (threadIdx.x == 0) { s.found_at = -1; s.found_before = 0; }
+  __syncthreads();
+  unsigned long long front = 0;
+  for (int w = 0; w < warp; ++w) front += s.scan[w];
+  incl += front;
+  if (v != 0 && incl - v < target && target <= incl) { s.found_at = threadIdx.x; s.found_before = incl - v; }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDrThreads, 2)
+draw_kernel(const DrawArgs a) {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ DrawShared s;
+  using Key = DrawKey<T>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = a.ctas;
+  const int row = blockIdx.x / C, rank = blockIdx.x - row * C;     // (the cluster is C blocks along x: rank is the block's place in it)
+  if (tid == 0) { mbar_init(&s.bar, 1); s.abort_flag = 0; fence_barrier_init(); }
+  if (tid < 32) s.table[tid] = exp2((double)tid * 0.03125);
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- the block's ids [i0, i0 + n) into shared memory, at the same offset from a 16-byte boundary as they have in global memory
+  const int i0 = min(a.vocab, rank * a.per), n = min(a.vocab, i0 + a.per) - i0;
+  const T* g = (const T*)a.logits + (size_t)row * a.ld + i0;
+  const int skew = (int)((uintptr_t)g & 15) / (int)sizeof(T);
+  T* x = (T*)dyn + skew;
+  constexpr int kVec = 16 / sizeof(T);
+  const int head = min(n, (kVec - skew) % kVec), body = (n - head) / kVec * kVec;
+  if (tid == 0 && body > 0) {
+    mbar_expect_tx(&s.bar, (uint32_t)(body * sizeof(T)));
+    bulk_load(x + head, g + head, (uint32_t)(body * sizeof(T)), &s.bar);
+  }
+  if (tid < head) x[tid] = g[tid];
+  if (tid < n - head - body) x[head + body + tid] = g[head + body + tid];
+  const float temp = a.temperature != nullptr ? a.temperature[row] : a.temperature_all;
+  const int top_k = a.top_k != nullptr ? a.top_k[row] : a.top_k_all;
+  const float top_p = a.top_p != nullptr ? a.top_p[row] : a.top_p_all;
+  const float min_p = a.min_p != nullptr ? a.min_p[row] : a.min_p_all;
+  const float u = a.u != nullptr ? a.u[row] : 0.f;
+  if (body > 0) mbar_wait(&s.bar, 0, (volatile int*)&s.abort_flag, a.status, 700, row);
+  __syncthreads();
+
+  // ---- maximum
+  float mx = -INFINITY;
+  for (int i = tid; i < n; i += kDrThreads) mx = fmaxf(mx, Key::value(x[i]));
+  mx = warp_max(mx);
+  if (lane == 0) s.red[warp] = mx;
+  if (tid == 0) s.first_max = 0x7fffffff;
+  __syncthreads();
+  mx = warp_max(s.red[lane & (kDrWarps - 1)]);
+  const bool greedy = !(temp > 0.f);
+  if (greedy) {
+    int at = 0x7fffffff;
+    for (int i = tid; i < n; i += kDrThreads) if (Key::value(x[i]) == mx) { at = i0 + i; break; }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0 && at != 0x7fffffff) atomicMin(&s.first_max, at);
+  }
+  if (tid == 0) s.max_x = mx;
+  __syncthreads();
+  dr_cluster_sync();
+  for (int c = 0; c < C; ++c) mx = fmaxf(mx, __uint_as_float(dr_peer32(&s.max_x, c)));
+  if (greedy || mx == -INFINITY) {
+    // the lowest id of the maximum; a row without any logit to draw from answers 0, as the arg-max does
+    if (rank == 0 && tid == 0) {
+      int at = 0x7fffffff;
+      if (mx > -INFINITY)
+        for (int c = 0; c < C; ++c) if (__uint_as_float(dr_peer32(&s.max_x, c)) == mx) at = min(at, (int)dr_peer32(&s.first_max, c));
+      a.out[row] = at == 0x7fffffff ? 0 : at;
+      if (a.logprob != nullptr) a.logprob[row] = mx > -INFINITY ? 0.f : -INFINITY;
+    }
+    dr_cluster_sync();                                             // nobody leaves while another one reads its shared memory
+    return;
+  }
+
+  const double scale = 1.4426950408889634 / (double)temp, dmx = (double)mx;
+  auto weight = [&](float v) -> unsigned long long { return v == mx ? 1ull << kDrMass : dr_weight(((double)v - dmx) * scale, s.table); };
+  auto bin_of = [&](float v) -> int { return min(kDrBins - 1, (int)fminf((mx - v) * 16.0f, 1e6f)); };       // monotone in v (mx = inf: all in the last bin)
+  // a warp owns a run of the block's ids
+  const int run = (n + kDrWarps - 1) / kDrWarps, r0 = min(n, warp * run), rn = min(n, r0 + run) - r0;
+  bool listed = false;
+  int list_n = 0;
+  // f(value, in range) for the warp's ids, or for the listed ones; all lanes take part in every turn
+  auto each = [&](auto f) {
+    const int m = listed ? list_n : rn;
+    for (int b = 0; b < m; b += 32) {
+      const int i = b + lane;
+      const bool in = i < m;
+      const int at = in ? (listed ? (int)s.list[warp][i] : i) : 0;
+      const float v = in ? Key::value(x[r0 + at]) : -INFINITY;
+      f(v, in && v > -INFINITY);
+    }
+  };
+  int step = 0;                                                    // parity of the histogram in use
+  auto clear = [&](bool mass) {
+    for (int i = tid; i < kDrBins; i += kDrThreads) { s.count[step & 1][i] = 0; if (mass) { s.lo[step & 1][i] = 0; s.hi[step & 1][i] = 0; } }
+    __syncthreads();
+  };
+  auto put = [&](int b, bool in) {                                 // one more in bin b
+    const int b0 = __shfl_sync(0xffffffffu, b, 0);
+    if (__all_sync(0xffffffffu, in && b == b0)) { if (lane == 0) atomicAdd(&s.count[step & 1][b], 32u); }      // rows of equal logits: not 32 adds to one word
+    else if (in) atomicAdd(&s.count[step & 1][b], 1u);
+  };
+  auto put_mass = [&](int b, unsigned long long w) {
+    const unsigned l = (unsigned)w, old = atomicAdd(&s.lo[step & 1][b], l);
+    const unsigned h = (unsigned)(w >> 32) + (old + l < old ? 1u : 0u);
+    if (h != 0) atomicAdd(&s.hi[step & 1][b], h);
+  };
+  auto gather = [&](int b, bool mass) -> unsigned long long {      // the bin over all blocks
+    unsigned long long v = 0;
+    for (int c = 0; c < C; ++c)
+      v += mass ? ((unsigned long long)dr_peer32(&s.hi[step & 1][b], c) << 32) + dr_peer32(&s.lo[step & 1][b], c) : dr_peer32(&s.count[step & 1][b], c);
+    return v;
+  };
+  const unsigned key_none = Key::of(-INFINITY);
+  unsigned tau = key_none;                                         // kept: key > tau, and the first `ties` ids of key tau
+  unsigned long long ties = 0;
+  // The cut in front of which `target` (ids, or mass) lies: sets tau; returns what lies above it.  extra: mass that the ids of key `extra_key` count, which the
+  // passes leave out (the ties at the top-k cut: only some of them are kept).
+  auto cut = [&](bool mass, unsigned long long target, unsigned extra_key, unsigned long long extra, int extra_bin) -> unsigned long long {
+    // the histogram of bins is complete in all blocks
+    unsigned long long v = gather(tid, mass);
+    if (mass && tid == extra_bin) v += extra;
+    dr_find(v, target, s);
+    const int bin = s.found_at;
+    unsigned long long before = s.found_before;
+    __syncthreads();
+    if (!listed) {                                                 // from here on only ids up to this bin matter: the warp lists them, in order
+      int cnt = 0;
+      for (int b = 0; b < rn; b += 32) {
+        const int i = b + lane;
+        const float e = i < rn ? Key::value(x[r0 + i]) : -INFINITY;
+        const bool in = e > -INFINITY && bin_of(e) <= bin;
+        const unsigned m = __ballot_sync(0xffffffffu, in);
+        const int at = cnt + __popc(m & ((1u << lane) - 1));
+        if (in && at < kDrList) s.list[warp][at] = (unsigned short)i;
+        cnt += __popc(m);
+      }
+      __syncwarp();
+      if (cnt <= kDrList) { listed = true; list_n = cnt; }
+    }
+    // keys of the bin lie in [k0, k1]
+    const float eps = fmaf(fabsf(mx), 2.5e-7f, 1e-5f);
+    const unsigned k1 = bin == 0 ? Key::of(mx) : Key::of(mx - bin * 0.0625f + eps);
+    const unsigned k0 = bin == kDrBins - 1 ? Key::of(-FLT_MAX) : Key::of(mx - (bin + 1) * 0.0625f - eps);
+    const unsigned range = k1 > k0 ? k1 - k0 : 0;
+    unsigned prefix = 0;
+    for (int bits = 32 - __clz(range); bits > 0;) {
+      const int shift = max(0, bits - 8);
+      ++step;
+      clear(mass);
+      each([&](float e, bool in) {
+        const unsigned off = min(Key::of(e) - k0, range);
+        in = in && bin_of(e) == bin && (bits >= 32 ? 0u : off >> bits) == prefix;
+        if (!mass) put((off >> shift) & 255, in);
+        else if (in && Key::of(e) > tau) { const unsigned long long w = weight(e); if (w) put_mass((off >> shift) & 255, w); }
+      });
+      __syncthreads();
+      dr_cluster_sync();
+      unsigned long long d = 0;
+      const int digit = 255 - tid;                                 // from the largest key down
+      if (tid < 256) {
+        d = gather(digit, mass);
+        if (mass && extra != 0 && bin == extra_bin) {
+          const unsigned off = min(extra_key - k0, range);
+          if ((bits >= 32 ? 0u : off >> bits) == prefix && (int)((off >> shift) & 255) == digit) d += extra;
+        }
+      }
+      dr_find(d, target - before, s);
+      prefix = prefix << (bits - shift) | (unsigned)(255 - s.found_at);
+      before += s.found_before;
+      bits = shift;
+      __syncthreads();
+    }
+    tau = k0 + prefix;
+    return before;
+  };
+
+  // ---- top-k
+  unsigned long long tie_mass = 0;                                 // of the ids kept at tau
+  int tau_bin = -1;
+  auto value_of = [&](unsigned key) -> float {                     // the logit of a key
+    if (sizeof(T) == 2) key = (key << 16) | ((key & 0x8000u) ? 0u : 0xffffu);
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+  };
+  if (top_k > 0 && top_k < a.vocab) {
+    clear(false);
+    each([&](float e, bool in) { put(in ? bin_of(e) : 0, in); });
+    __syncthreads();
+    dr_cluster_sync();
+    unsigned long long mine = gather(tid, false);                  // all there are
+    unsigned long long all = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) s.warp_mass[warp] = all;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < kDrWarps; ++w) all += s.warp_mass[w];
+    __syncthreads();
+    if (all > (unsigned long long)top_k) {
+      const unsigned long long above = cut(false, (unsigned long long)top_k, 0, 0, -1);
+      ties = (unsigned long long)top_k - above;
+      const float vt = value_of(tau);
+      tie_mass = ties * weight(vt);
+      tau_bin = bin_of(vt);
+    }
+    ++step;
+  }
+  // ---- top-p of what is left
+  if (top_p < 1.f) {
+    clear(true);
+    each([&](float e, bool in) { if (in && Key::of(e) > tau) { const unsigned long long w = weight(e); if (w) put_mass(bin_of(e), w); } });
+    __syncthreads();
+    dr_cluster_sync();
+    unsigned long long all = gather(tid, true);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) s.warp_mass[warp] = all;
+    __syncthreads();
+    all = tie_mass;
+    for (int w = 0; w < kDrWarps; ++w) all += s.warp_mass[w];
+    __syncthreads();
+    const double goal = ceil((double)top_p * (double)all);
+    const unsigned long long target = goal >= (double)all ? all : goal < 1.0 ? 1ull : (unsigned long long)goal;
+    const unsigned old_tau = tau;
+    const unsigned long long old_ties = ties;
+    const unsigned long long above = cut(true, target, old_tau, tie_mass, tau_bin);
+    const unsigned long long wt = weight(value_of(tau));
+    ties = wt > 0 ? (target - above + wt - 1) / wt : 0;
+    if (tau == old_tau) ties = min(ties, old_ties);
+    ++step;
+  }
+  // ---- the draw, in id order: blocks, warps, sixteenths of a warp's ids, ids
+  const unsigned long long min_w = min_p > 0.f ? (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << kDrMass)) : 0ull;
+  unsigned long long wt = ties > 0 ? weight(value_of(tau)) : 0;
+  if (wt < min_w) wt = 0;
+  auto kept = [&](float e, bool in, bool& tie) -> unsigned long long {
+    const unsigned k = Key::of(e);
+    tie = in && k == tau;
+    if (!in || k <= tau) return 0;
+    const unsigned long long w = weight(e);
+    return w >= min_w ? w : 0;
+  };
+  unsigned long long mass = 0;
+  int n_tie = 0;
+  each([&](float e, bool in) { bool tie; mass += kept(e, in, tie); n_tie += tie; });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  n_tie = __reduce_add_sync(0xffffffffu, n_tie);
+  if (lane == 0) { s.warp_mass[warp] = mass; s.warp_ties[warp] = n_tie; s.list_n[warp] = listed ? list_n : -1; }
+  __syncthreads();
+  if (tid == 0) {
+    unsigned long long m = 0; int t = 0;
+    for (int w = 0; w < kDrWarps; ++w) { m += s.warp_mass[w]; t += s.warp_ties[w]; }
+    s.total[0] = m; s.ties = t;
+  }
+  __syncthreads();
+  dr_cluster_sync();
+  unsigned long long gt = 0, all = 0;                              // above tau: in front of this block; in all
+  unsigned long long nt = 0, all_ties = 0;
+  for (int c = 0; c < C; ++c) {
+    const unsigned long long m = dr_peer64(&s.total[0], c);
+    const unsigned t = dr_peer32(&s.ties, c);
+    if (c < rank) { gt += m; nt += t; }
+    all += m; all_ties += t;
+  }
+  all += min(all_ties, ties) * wt;
+  const double spot = (double)u * (double)all;
+  unsigned long long r = spot > 0.0 ? (spot >= (double)all ? all - 1 : (unsigned long long)spot) : 0ull;        // (u below 0 or NaN: 0; 1 and above: the last id)
+  if (r >= all) r = all - 1;
+  // mass in front of a place with m above tau and t ties in front of it
+  auto front = [&](unsigned long long m, unsigned long long t) { return m + min(t, ties) * wt; };
+  const bool here = front(gt, nt) <= r && r < front(gt + s.total[0], nt + (unsigned)s.ties);
+  if (here) {                                                      // the same for all threads of the block, and true in one block
+    int w = 0;
+    for (; w < kDrWarps - 1; ++w) {
+      if (r < front(gt + s.warp_mass[w], nt + (unsigned)s.warp_ties[w])) break;
+      gt += s.warp_mass[w]; nt += (unsigned)s.warp_ties[w];
+    }
+    const int wn = s.list_n[w], w0 = min(n, w * run), m = wn >= 0 ? wn : min(n, w0 + run) - w0;
+    const int piece = (m + kDrWarps * 32 - 1) / (kDrWarps * 32) * 32;
+    auto at_of = [&](int i) { return w0 + (wn >= 0 ? (int)s.list[w][i] : i); };
+    __syncthreads();                                               // warp_mass and warp_ties are used again
+    mass = 0; n_tie = 0;
+    for (int i = warp * piece + lane; i < min(m, (warp + 1) * piece); i += 32) {
+      const float e = Key::value(x[at_of(i)]);
+      bool tie;
+      mass += kept(e, e > -INFINITY, tie);
+      n_tie += tie;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    n_tie = __reduce_add_sync(0xffffffffu, n_tie);
+    if (lane == 0) { s.warp_mass[warp] = mass; s.warp_ties[warp] = n_tie; }
+    __syncthreads();
+    int p = 0;
+    for (; p < kDrWarps - 1; ++p) {
+      if (r < front(gt + s.warp_mass[p], nt + (unsigned)s.warp_ties[p])) break;
+      gt += s.warp_mass[p]; nt += (unsigned)s.warp_ties[p];
+    }
+    if (warp == 0) {
+      bool done = false;
+      const int end = min(m, (p + 1) * piece);
+      for (int b = p * piece; b < end && !done; b += 32) {
+        const int i = b + lane;
+        const float e = i < end ? Key::value(x[at_of(i)]) : -INFINITY;
+        bool tie;
+        unsigned long long incl = kept(e, e > -INFINITY, tie);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
+        const unsigned tm = __ballot_sync(0xffffffffu, tie);
+        const unsigned hit = __ballot_sync(0xffffffffu, r < front(gt + incl, nt + __popc(tm & (0xffffffffu >> (31 - lane)))));
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            a.out[row] = i0 + at_of(i);
+            if (a.logprob != nullptr)
+              a.logprob[row] = (float)((e == mx ? 0.0 : ((double)e - dmx) * scale) * 0.69314718055994531 - log((double)all * (1.0 / (double)(1ull << kDrMass))));
+          }
+          done = true;
+        }
+        gt += __shfl_sync(0xffffffffu, incl, 31);
+        nt += __popc(tm);
+      }
+    }
+  }
+  dr_cluster_sync();                                               // nobody leaves while another one reads its shared memory
+}
+
+template <typename T>
+static int draw_launch(DrawArgs a, cudaStream_t stream) {
+  // Blocks per row: enough that a block's share of the row fits shared memory beside a second block's.
+  int c = 1;
+  while (c < 8 && ((long)a.vocab > (long)c * 4096 || (long)((a.vocab + c - 1) / c) * (long)sizeof(T) > 90000)) c *= 2;
+  a.ctas = c;
+  a.per = ((a.vocab + c - 1) / c + 15) / 16 * 16;
+  const size_t smem = (size_t)a.per * sizeof(T) + 32;
+  if (smem > 200 * 1024) return fail("draw: the vocabulary does not fit the shared memory of eight blocks%s");
+  static size_t attr[64];
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  if (smem > attr[dev & 63]) {
+    GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attr[dev & 63] = smem;
+  }
+  launch_k_cluster(draw_kernel<T>, (unsigned)(a.rows * c), kDrThreads, smem, stream, (unsigned)c, a);
+  GB_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace gb
+
+using namespace gb;
+
+// dtype: 0 = f32, 1 = bf16.  temperature / top_k / top_p / min_p: one value per row (device), or null and the value for all rows.
+GB_API int gb_draw(const void* logits, long ld, int dtype, int rows, int vocab, const float* u, const float* temperature, float temperature_all,
+                   const int* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all, int* out, float* logprob,
+                   void* status, cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (vocab < 1 || ld < vocab || rows > (1 << 27)) return fail("draw: bad sizes%s");
+  DrawArgs a;
+  memset(&a, 0, sizeof(a));
+  a.logits = logits; a.ld = ld; a.rows = rows; a.vocab = vocab; a.u = u; a.temperature = temperature; a.temperature_all = temperature_all;
+  a.top_k = top_k; a.top_k_all = top_k_all; a.top_p = top_p; a.top_p_all = top_p_all; a.min_p = min_p; a.min_p_all = min_p_all; a.out = out;
+  a.logprob = logprob; a.status = (KernelStatus*)status;
+  return dtype == 0 ? draw_launch<float>(a, stream) : draw_launch<__nv_bfloat16>(a, stream);
+}

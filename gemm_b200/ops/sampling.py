@@ -85,3 +85,70 @@ def sample_ref(logits, temperature, top_k, top_p, seed, step):
         idx, p = candidate_set_ref(logits[r], temperature, top_k, top_p)
         out.append(int(idx[torch.multinomial(p, 1, generator=g)]))
     return torch.tensor(out, dtype=torch.int32)
+
+
+def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None, want_logprob: bool = False):
+    """One token per row of ``logits [B, V]`` (f32 or bf16; rows may lie further apart than V) from given numbers ``uniform [B]`` (f32 in [0, 1)): int32 ``[B]``, with
+    ``want_logprob`` also the f32 logarithm of the probability it was drawn with.  ``temperature``, ``top_k`` (0: no limit), ``top_p``, ``min_p``: a number, or a
+    tensor ``[B]`` with a value for each row (f32; ``top_k`` int32).
+
+    In the order (logit descending, id ascending): the first ``top_k`` ids; of these the ids that have less than ``top_p`` of the probability in front of them (at
+    least one); of these the ids with at least ``min_p`` times the largest probability.  The draw is the first id, in id order, at which the kept probability so
+    far exceeds ``uniform`` of it all.  ``temperature <= 0``: the lowest id of the largest logit.  NaN counts as -inf; a row without any logit above -inf answers
+    id 0 with logarithm -inf.  Probabilities below 2^-45 of the largest count as zero."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] < 1:
+        raise ValueError("logits: a tensor [B, V] in f32 or bf16 is needed")
+    b, v = logits.shape
+    dev = logits.device
+    if v > 1 and logits.stride(1) != 1 or (b > 1 and logits.stride(0) < v):
+        raise ValueError("logits: a row's values lie one after the other, and rows do not overlap")
+    if uniform.dtype != torch.float32 or uniform.shape != (b,) or uniform.device != dev or not uniform.is_contiguous():
+        raise ValueError(f"uniform: a contiguous f32 tensor [{b}] beside the logits is needed")
+    given = []
+    for name, x, dt, none in (("temperature", temperature, torch.float32, 1.0), ("top_k", top_k, torch.int32, 0), ("top_p", top_p, torch.float32, 1.0),
+                              ("min_p", min_p, torch.float32, 0.0)):
+        if torch.is_tensor(x):
+            if x.dtype != dt or x.shape != (b,) or x.device != dev or not x.is_contiguous():
+                raise ValueError(f"{name}: a contiguous {dt} tensor [{b}] beside the logits is needed")
+            given.append((x, none))
+        else:
+            given.append((None, none if x is None else x))
+    if not logits.is_cuda:
+        token, logprob = draw_ref(logits, uniform, *(x if x is not None else y for x, y in given))
+        return (token, logprob) if want_logprob else token
+    (t, t0), (k, k0), (p, p0), (m, m0) = given
+    with _native.on_device(dev):
+        out = torch.empty(b, dtype=torch.int32, device=dev)
+        logprob = torch.empty(b, dtype=torch.float32, device=dev) if want_logprob else None
+        rc = _native.cuda().gb_draw(_p(logits), _l(logits.stride(0) if b > 1 else v), _i(0 if logits.dtype == torch.float32 else 1), _i(b), _i(v), _p(uniform), _p(t),
+                                    _f(t0), _p(k), _i(k0), _p(p), _f(p0), _p(m), _f(m0), _p(out), _p(logprob), _c(_native.status_ptr()), _c(_native.stream()))
+        _native.check(rc, "gb_draw", n=1 if b else 0)
+    return (out, logprob) if want_logprob else out
+
+
+def draw_ref(logits, uniform, temperature, top_k, top_p, min_p):
+    """``draw`` in 64-bit floats: (tokens, logarithms)."""
+    b, v = logits.shape
+    col = lambda x: torch.as_tensor(x, device=logits.device).float().double().expand(b)[:, None]       # noqa: E731
+    t, k, p, m, u = (col(x) for x in (temperature, top_k, top_p, min_p, uniform))
+    x = torch.where(logits.isnan(), float("-inf"), logits.double())
+    val, ids = torch.sort(x, dim=-1, descending=True, stable=True)
+    rank = torch.arange(v, device=logits.device)
+    k = torch.where(~(t > 0), 1.0, torch.where(k > 0, k, float(v)))
+    d = torch.where(val == val[:, :1], 0.0, val - val[:, :1])
+    w = torch.where((rank < k) & (val > float("-inf")), torch.exp(d / torch.where(t > 0, t, 1.0)), 0.0)
+    w = torch.where(w > 2.0 ** -45, w, 0.0)
+    cum = w.cumsum(-1)
+    front = torch.cat([torch.zeros_like(cum[:, :1]), cum[:, :-1]], 1)
+    keep = (front < p * cum[:, -1:]) | ~(p < 1) | (rank == 0)
+    keep &= ~(w < m.clamp_max(1.0))
+    w = torch.zeros_like(w).scatter_(1, ids, w * keep)
+    cdf = w.cumsum(-1)
+    u = torch.where(u > 0, u, 0.0)
+    pick = (cdf <= u * cdf[:, -1:]).sum(-1, keepdim=True)
+    last = v - 1 - (w.flip(1) > 0).to(torch.int8).argmax(-1, keepdim=True)         # u = 1 and above: the last id that can be drawn
+    pick = torch.minimum(pick, last)
+    none = cdf[:, -1:] == 0
+    pick = torch.where(none, 0, pick)
+    lp = torch.where(none, float("-inf"), (w.gather(1, pick) / cdf[:, -1:]).log())
+    return pick[:, 0].to(torch.int32), lp[:, 0].float()

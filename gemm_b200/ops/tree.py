@@ -1,0 +1,173 @@
+"""Trees of drafted tokens over a paged KV cache: the attention of their nodes (csrc/kernels/tree_attn.cu, tree_any.cu) and, once the target model's tokens are
+drawn, the acceptance of a path and the move of its K / V rows (csrc/kernels/tree_commit.cu).
+
+A sequence with ``ctx`` committed tokens brings a tree of ``n`` nodes: node 0 is its last certain token, every other node a draft that continues its
+parent, which has a lower index.  Node i is cached at place ``ctx + i`` of the sequence (``kv_len = ctx + n``) and has the position ``ctx + depth``
+(``ops.paging.batch_tables`` makes these tables and the masks).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from .. import _native
+from .paging import MAX_NODES, check_int32
+
+_c, _i, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+
+
+def _p(t):
+    return _c(t.data_ptr()) if t is not None else _c(0)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor,
+                   page_size: int, mask: torch.Tensor, max_nodes: int, window: int = 0, positions: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention output ``[T, Hq, dv]`` of the nodes ``q [T, Hq, dk]`` (multiplied by scale * log2(e); rows may lie further apart than Hq * dk) over
+    ``k_cache [slots, Hkv, dk]`` / ``v_cache [slots, Hkv, dv]``.  Sequence s has the nodes ``cu_q[s] .. cu_q[s + 1]`` (at most ``max_nodes`` <= 256), cached at
+    its last places.  A node sees the places in front of the tree (``window`` > 0: those less than ``window`` in front of its ``positions`` entry) and the
+    nodes whose bits are set in its row of ``mask`` (int64 ``[T, words]``, its own bit among them as a rule).  A node that sees nothing gets zeros; rows behind
+    the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not finite."""
+    t, hq, dk = q.shape
+    slots, hkv, dv = v_cache.shape
+    dev = q.device
+    b = kv_len.numel()
+    if q.stride(2) != 1 or q.stride(1) != dk or (t > 1 and q.stride(0) < hq * dk):
+        raise ValueError("q: the heads of a token lie one after the other")
+    if k_cache.shape != (slots, hkv, dk) or not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.dtype != v_cache.dtype or k_cache.dtype != q.dtype:
+        raise ValueError("contiguous caches of the same slots, heads and type as the queries are needed")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"tree_attention takes bf16 or f32, not {q.dtype}")
+    if hkv < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads do not share {hkv} KV heads evenly")
+    check_int32(dev, cu_q=cu_q, kv_len=kv_len, block_table=block_table)
+    if cu_q.numel() != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b or page_size < 1:
+        raise ValueError("cu_q, kv_len and block_table name different numbers of sequences")
+    if k_cache.device != dev or v_cache.device != dev or mask.device != dev or mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != t or not mask.is_contiguous():
+        raise ValueError("mask: a contiguous int64 tensor [T, words] beside the queries is needed")
+    if not 1 <= max_nodes <= MAX_NODES or mask.shape[1] * 64 < max_nodes or mask.shape[1] > MAX_NODES // 64:
+        raise ValueError(f"trees of 1 to {MAX_NODES} nodes with a mask bit each, not {max_nodes} in {mask.shape[1]} words")
+    if window < 0 or (window > 0 and positions is None):
+        raise ValueError("a window needs the nodes' positions")
+    if positions is not None:
+        check_int32(dev, positions=positions)
+        if positions.numel() != t:
+            raise ValueError("positions: one for each node")
+    if out is None:
+        out = torch.empty(t, hq, dv, dtype=q.dtype, device=dev)
+    elif out.shape != (t, hq, dv) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out: a contiguous tensor [{t}, {hq}, {dv}] of the queries' type is needed")
+    if dev.type != "cuda":
+        return tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window, positions, out)
+    if t == 0 or b == 0:
+        return out
+    with _native.on_device(dev):
+        rc = _native.cuda().gb_tree_any(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _i(int(q.dtype == torch.float32)), _p(cu_q), _p(kv_len),
+                                        _p(block_table), _i(block_table.shape[1]), _i(page_size), _p(mask), _i(mask.shape[1]), _p(positions), _i(b), _l(slots),
+                                        _i(t), _i(hq), _i(hkv), _i(dk), _i(dv), _i(window), _c(_native.stream()))
+        _native.check(rc, "gb_tree_any")
+    return out
+
+
+def tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window=0, positions=None, out=None) -> torch.Tensor:
+    """``tree_attention`` in plain f32 (f64 for f64 tensors)."""
+    t, hq, _ = q.shape
+    g = hq // k_cache.shape[1]
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    if out is None:
+        out = torch.zeros(t, hq, v_cache.shape[2], dtype=q.dtype, device=q.device)
+    cu = cu_q.tolist()
+    for s in range(len(cu) - 1):
+        a, z, length = cu[s], cu[s + 1], int(kv_len[s])
+        if z <= a:
+            continue
+        ctx = max(0, length - (z - a))
+        place = torch.arange(min(length, block_table.shape[1] * page_size), device=q.device)
+        slot = block_table[s].long()[place // page_size] * page_size + place % page_size
+        off = place - ctx
+        bits = mask[a:z][:, (off >> 6).clamp(0, mask.shape[1] - 1)] >> (off & 63) & 1
+        see = (off < 0) | ((bits == 1) & (off < 64 * mask.shape[1]))
+        if window > 0:
+            see &= (off >= 0) | (place > positions[a:z, None].long() - window)
+        k = k_cache[slot].to(wide).repeat_interleave(g, dim=1)
+        v = v_cache[slot].to(wide).repeat_interleave(g, dim=1)
+        sc = (torch.einsum("qhd,khd->hqk", q[a:z].to(wide), k) * math.log(2.0)).masked_fill(~see, float("-inf"))
+        p = torch.softmax(sc, dim=-1).masked_fill(~see, 0.0)              # (a row that sees nothing is all NaN in front of the fill)
+        fine = torch.isfinite(v)
+        o = torch.einsum("hqk,khd->qhd", p, torch.where(fine, v, 0.0))
+        for key in (~fine).flatten(1).any(1).nonzero()[:, 0].tolist():     # values that are not finite reach the rows that see them, and no others
+            o += torch.where(see[:, key, None, None] & ~fine[key], v[key], 0.0)
+        out[a:z] = o.to(out.dtype)
+    return out
+
+
+class Accepted(NamedTuple):
+    count: torch.Tensor                     # int32 [B] nodes on the accepted path, the root among them (0: a sequence without nodes)
+    path: torch.Tensor                      # int32 [B, max_nodes] their indices, then -1
+    next_token: torch.Tensor                # int32 [B] the token drawn at the path's last node (-1: no nodes)
+    kv_len: torch.Tensor                    # int32 [B] committed length: ctx + count
+
+
+def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                block_table: torch.Tensor, page_size: int, max_nodes: int) -> Accepted:
+    """Accepts, from the root of every tree, the first child whose token (``tokens``) is the one drawn at its parent (``sampled``), as long as there is one, and
+    moves the accepted nodes' rows of all ``caches`` (``[slots, ...]`` contiguous, any type, e.g. every layer's K and V) from the places ``ctx + node`` to
+    ``ctx, ctx + 1, ...``, in place.  ``tokens`` / ``parents`` / ``sampled``: int32 ``[T]``; the lengths and tables are those of the verifying pass (``kv_len``
+    includes the tree).  No caches: the walk alone."""
+    dev, t, b = tokens.device, tokens.numel(), kv_len.numel()
+    check_int32(dev, tokens=tokens, parents=parents, sampled=sampled, cu_q=cu_q, kv_len=kv_len, block_table=block_table)
+    if parents.numel() != t or sampled.numel() != t:
+        raise ValueError("tokens, parents and sampled name different numbers of nodes")
+    if cu_q.numel() != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b or page_size < 1 or b > 65535:
+        raise ValueError("cu_q, kv_len and block_table name different numbers of sequences")
+    if not 1 <= max_nodes <= MAX_NODES:
+        raise ValueError(f"trees of 1 to {MAX_NODES} nodes, not {max_nodes}")
+    slots = caches[0].shape[0] if len(caches) else 0
+    for c in caches:
+        if not c.is_contiguous() or c.device != dev or c.shape[0] != slots:
+            raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
+    if dev.type != "cuda":
+        return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)
+    with _native.on_device(dev):
+        i32 = dict(dtype=torch.int32, device=dev)
+        got = Accepted(torch.empty(b, **i32), torch.empty(b, max_nodes, **i32), torch.empty(b, **i32), torch.empty(b, **i32))
+        live = [c for c in caches if c.numel()]
+        n = len(live)
+        ptrs = (ctypes.c_void_p * max(1, n))(*[c.data_ptr() for c in live])
+        rows = (ctypes.c_int * max(1, n))(*[c.numel() // slots * c.element_size() for c in live])
+        rc = _native.cuda().gb_tree_commit(ptrs, rows, _i(n), _l(slots), _p(tokens), _p(parents), _p(sampled), _p(cu_q), _p(kv_len), _p(block_table),
+                                           _i(block_table.shape[1]), _i(page_size), _i(b), _i(t), _i(max_nodes), _p(got.count), _p(got.path),
+                                           _p(got.next_token), _p(got.kv_len), _c(_native.stream()))
+        _native.check(rc, "gb_tree_commit", n=max(1, (n + 223) // 224) if b else 0)
+    return got
+
+
+def tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes) -> Accepted:
+    """``tree_commit`` in plain Python."""
+    cu, tok, par, drawn = cu_q.tolist(), tokens.tolist(), parents.tolist(), sampled.tolist()
+    count, paths, nxt, new = [], [], [], []
+    for s in range(len(cu) - 1):
+        a, n = cu[s], min(max(cu[s + 1] - cu[s], 0), max_nodes)
+        ctx = int(kv_len[s]) - max(cu[s + 1] - cu[s], 0)
+        path = [0] if n else []
+        while path:
+            kid = next((i for i in range(path[-1] + 1, n) if par[a + i] == path[-1] and tok[a + i] == drawn[a + path[-1]]), None)
+            if kid is None:
+                break
+            path.append(kid)
+        for j, node in enumerate(path):
+            src, dst = ((ctx + x) for x in (node, j))
+            if node != j and dst >= 0 and src // page_size < block_table.shape[1]:
+                src, dst = (int(block_table[s, x // page_size]) * page_size + x % page_size for x in (src, dst))
+                for c in caches:
+                    if c.numel() and 0 <= src < c.shape[0] and 0 <= dst < c.shape[0]:
+                        c[dst] = c[src]
+        count.append(len(path))
+        paths.append(path + [-1] * (max_nodes - len(path)))
+        nxt.append(drawn[a + path[-1]] if path else -1)
+        new.append(ctx + len(path))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=tokens.device)          # noqa: E731
+    return Accepted(i32(count), i32(paths).reshape(len(count), max_nodes), i32(nxt), i32(new))
