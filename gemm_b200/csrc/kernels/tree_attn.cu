@@ -1,0 +1,654 @@
+// Attention of drafted tree nodes over a paged KV cache on tcgen05 (bf16, heads of 64 or 128 columns).
+//
+// What a node sees, and the formula: tree_any.cu.  A row is a (node, query head of the group) pair, a tile is 128 rows of one KV head: floor(128 / G) nodes.
+// The context is long and the rows are few, so the kernel is built to stream K and V: one block per SM, its shared memory a ring of 32 KB tiles (K and V of
+// 128 places in turn) that TMA keeps full across work items, and two softmax groups of 128 threads, one thread per row.
+//   one tile in the item:   the groups take alternate KV blocks, each with its own maximum, sum and output accumulator, joined at the end;
+//   two tiles in the item:  each group has its tile, and both use the same K and V (wide trees: half the loads, which would bound the products).
+// TMEM: S / P (128 columns, P overwrites S in place) and O (128 columns) per group: all of it.
+//
+// Work: KV blocks of all (sequence, KV head, tile pair) items in one line, cut into equal pieces, one per SM: a long context is shared by many SMs, short ones
+// fill one, whatever the mix.  The cut goes by lengths that only the device knows (a captured launch may be replayed with other ones), so every block works out
+// its piece from the lengths.  A piece that holds an item's part leaves the part's output (f32, normalised) and base-2 logarithm of its sum in a workspace; a second
+// launch joins the parts in the order of their blocks.
+//
+// P is rounded to bf16 for the second product (the tensor cores' operand type; sums stay f32): at most 2^-9 of each weight.
+#include "sm100.cuh"
+#include "host_common.h"
+#include <algorithm>
+
+namespace gb {
+
+constexpr int kTaThreads = 352;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads
+constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, the rest is the ring
+constexpr int kTaSmem = 1024 + kTaTiles * 32768 + 2048;
+
+struct TreeAttnArgs {
+  const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
+  int n_seqs, max_pages, page_size, words, window, hq, hkv, total_tokens;
+  int pair;                          // tiles per item: 1 or 2
+  int whole;                         // items are not cut (short contexts): no parts
+  __nv_bfloat16* out;                // [T, hq, DV]
+  float* part_o; float* part_lse;    // [2 * grid][pair * 128][DV], [2 * grid][pair * 128]
+  int4* part_of;                     // [grid]: the item that begins in a piece and goes on behind it {sequence, item of it, parts, first part's slot}; parts = 0: none
+  const __nv_bfloat16* v_cache; long num_slots;
+  KernelStatus* status;
+};
+
+// Shape of a sequence's work.
+struct TaSeq {
+  int begin, nodes, len, ctx, first, blocks, units, tiles, items;
+  __device__ __forceinline__ void load(const TreeAttnArgs& a, int s) {
+    const int G = a.hq / a.hkv, tpt = 128 / G;
+    begin = min(max(a.cu_q[s], 0), a.total_tokens);
+    nodes = max(min(a.cu_q[s + 1], a.total_tokens) - begin, 0);
+    const int kv = a.kv_len[s];
+    len = max(0, (int)min((long long)kv, (long long)a.max_pages * a.page_size));
+    ctx = max(0, kv - nodes);
+    first = a.window > 0 ? max(0, ctx - a.window + 1) / 128 : 0;
+    blocks = max(0, (len + 127) / 128 - first);
+    units = a.whole ? 1 : max(1, blocks);
+    tiles = (nodes + tpt - 1) / tpt;
+    items = (tiles + a.pair - 1) / a.pair * a.hkv;
+  }
+};
+
+// The pieces: [c * total / active, (c + 1) * total / active) of the line of units.
+struct TaPiece {
+  long long total, pos, left;
+  int active, seq, item, unit;
+};
+
+// The part of an item that a block works on.
+struct TaSeg {
+  TaSeq q;
+  int seq, item, kvh, tile, n_tiles;      // first tile, 1 or 2 of them
+  int lo, n;                              // KV blocks [lo, lo + n) of the sequence
+  bool full, head;                        // all of the item's blocks; its first ones
+  int nth;                                // number of the segment in its piece
+  long long pos;                          // its first unit's place in the line
+};
+
+struct TaWalk {
+  TaPiece p;
+  TaSeq q;
+  int at, nth;
+  __device__ __forceinline__ bool next(const TreeAttnArgs& a, TaSeg& s) {
+    if (p.left <= 0) return false;
+    if (at != p.seq) { q.load(a, p.seq); at = p.seq; }
+    const int take = (int)min((long long)(q.units - p.unit), p.left);
+    const int pairs = q.items / a.hkv;
+    s.q = q; s.seq = p.seq; s.item = p.item;
+    s.kvh = p.item / pairs; s.tile = (p.item - s.kvh * pairs) * a.pair; s.n_tiles = min(a.pair, q.tiles - s.tile);
+    s.lo = q.first + (a.whole ? 0 : p.unit); s.n = a.whole ? q.blocks : min(take, q.blocks - p.unit);
+    s.full = take == q.units; s.head = p.unit == 0; s.nth = nth++; s.pos = p.pos;
+    p.left -= take; p.pos += take; p.unit += take;
+    if (p.unit == q.units) {
+      p.unit = 0;
+      if (++p.item == q.items) {
+        p.item = 0;
+        if (p.left > 0) do { ++p.seq; q.load(a, p.seq); at = p.seq; } while (q.items == 0 && p.seq + 1 < a.n_seqs);
+      }
+    }
+    return true;
+  }
+};
+
+// What the softmax groups keep of the walk, in shared memory: thread 0 finds the next segment while the present one is worked on (their registers hold a row of scores).
+struct TaGroups {
+  TaWalk walk;
+  TaSeg seg[2];
+  int more[2];
+};
+
+__device__ __forceinline__ bool bar256_and(bool pred) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, 2, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(r) : "r"((uint32_t)pred) : "memory");
+  return r != 0;
+}
+
+// Bits [at, at + 32) of a node's mask row (at may be negative: zeros in front).
+__device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int words, int at) {
+  if (at <= -32 || at >= words * 64) return 0;
+  if (at < 0) return (uint32_t)row[0] << -at;
+  const int w = at >> 6, sh = at & 63;
+  unsigned long long v = row[w] >> sh;
+  if (sh > 32 && w + 1 < words) v |= row[w + 1] << (64 - sh);
+  return (uint32_t)v;
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+
+template <int DK, int DV>
+__global__ void __launch_bounds__(kTaThreads, 1)
+tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV);
+  uint8_t* sQ = smem;                                             // pair x [128 rows] (64-column halves of 128 B, swizzled)
+  uint8_t* ring = smem + a.pair * kQ;
+  const int slots = min(10, (int)((kTaTiles * 32768 - a.pair * kQ) / kSlot));
+  uint64_t* bars = (uint64_t*)(smem + kTaTiles * 32768);
+  uint64_t* q_full = bars; uint64_t* q_empty = bars + 1;
+  uint64_t* s_full = bars + 2; uint64_t* p_ready = bars + 4; uint64_t* o_full = bars + 6;      // [2] each, by group
+  uint64_t* t_full = bars + 8; uint64_t* t_empty = bars + 18;                                  // [10] each
+  uint32_t* tmem_slot = (uint32_t*)(bars + 28);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  int* s_odd = (int*)(tmem_slot + 2);                             // [8] tree nodes of the segment whose value rows are not finite, as bits
+  float* s_x = (float*)(bars + 36);                               // [2][128]: what the groups tell each other about a row
+  long long* s_scan = (long long*)s_x;                            // prologue only
+  TaPiece* s_piece = (TaPiece*)(s_x + 256);
+  TaGroups* s_groups = (TaGroups*)(s_x + 256);                    // behind the prologue
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1); mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 128); mbar_init(&o_full[i], 1); }
+    for (int i = 0; i < 10; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 1); }
+    *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) s_odd[i] = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+  }
+  if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  pdl_wait();
+  // ---- the block's piece of the line
+  {
+    const int per = (a.n_seqs + kTaThreads - 1) / kTaThreads;
+    const int i0 = min(a.n_seqs, (int)threadIdx.x * per), i1 = min(a.n_seqs, i0 + per);
+    long long mine = 0;
+    TaSeq q;
+    for (int i = i0; i < i1; ++i) { q.load(a, i); mine += (long long)q.items * q.units; }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
+    if (lane == 31) s_scan[warp] = incl;
+    if (threadIdx.x == 0) { s_piece->left = 0; s_piece->total = 0; }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long total = 0, front = 0;
+    for (int w = 0; w < kTaThreads / 32; ++w) { if (w == warp) front = total; total += s_scan[w]; }
+    const long long excl = front + incl - mine;
+    // at least two units a piece: a part costs more to write and join than a block to work on
+    const int active = (int)min((long long)gridDim.x, a.whole ? total : (total + 1) / 2);
+    if ((int)blockIdx.x < active) {
+      const long long lo = blockIdx.x * total / active, hi = (blockIdx.x + 1ll) * total / active;
+      if (excl <= lo && lo < excl + mine) {
+        long long at = excl;
+        int i = i0;
+        for (;; ++i) { q.load(a, i); const long long c = (long long)q.items * q.units; if (lo < at + c) break; at += c; }
+        s_piece->total = total; s_piece->pos = lo; s_piece->left = hi - lo; s_piece->active = active; s_piece->seq = i;
+        s_piece->item = (int)((lo - at) / q.units); s_piece->unit = (int)((lo - at) % q.units);
+      }
+    }
+    __syncthreads();
+  }
+  TaWalk walk;
+  walk.p = *s_piece;
+  walk.at = -1; walk.nth = 0;
+  __syncthreads();                                                // s_x is the groups' from here on
+  const uint32_t tmem_base = *tmem_slot;
+  const int G = a.hq / a.hkv, tpt = 128 / G;
+  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0);
+
+  if (warp == 8) {
+    TaSeg s;
+    // ---------------------------------------------------------------- K and V: the lanes fetch and issue a page each
+    const int ppb = 128 / a.page_size;
+    const uint32_t page_bytes = (uint32_t)a.page_size * 128;
+    int slot = 0; uint32_t ph = 0;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      if (s.n <= 0) continue;
+      const int* bt = a.block_table + (size_t)s.seq * a.max_pages;
+      const int last_page = (s.q.len + a.page_size - 1) / a.page_size - 1;
+      int page = lane < ppb ? bt[min(s.lo * ppb + lane, last_page)] : 0;
+      for (int j = 0; j < s.n && ok; ++j) {
+        const int now = page;
+        if (j + 1 < s.n && lane < ppb) page = bt[min((s.lo + j + 1) * ppb + lane, last_page)];      // (pages behind the end: the last one again; nothing of them counts)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = ok && mbar_wait(&t_empty[slot], ph ^ 1, abort_flag, a.status, 800, j);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int D = kv ? DV : DK;
+          const CUtensorMap* tm = kv ? &tmV : &tmK;
+          if (lane == 0) mbar_expect_tx(&t_full[slot], 256u * D);
+          __syncwarp();
+          if (lane < ppb) {
+            uint8_t* dst = ring + slot * kSlot + lane * page_bytes;
+            tma_load_3d(dst, tm, &t_full[slot], 0, s.kvh, now * a.page_size);
+            if (D > 64) tma_load_3d(dst + 16384, tm, &t_full[slot], 64, s.kvh, now * a.page_size);
+          }
+          if (++slot == slots) { slot = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 10) {
+    if (lane == 0) {
+      TaSeg s;
+      uint32_t ph = 0;
+      while (walk.next(a, s)) {
+        if (s.n <= 0) continue;
+        if (!mbar_wait(q_empty, ph ^ 1, abort_flag, a.status, 810, s.seq)) break;
+        mbar_expect_tx(q_full, (uint32_t)(2 * DK * G * tpt) * s.n_tiles);
+        for (int t = 0; t < s.n_tiles; ++t) {
+          const int tok = s.q.begin + (s.tile + t) * tpt;
+          tma_load_3d(sQ + t * kQ, &tmQ, q_full, 0, s.kvh * G, tok);
+          if constexpr (DK > 64) tma_load_3d(sQ + t * kQ + 16384, &tmQ, q_full, 64, s.kvh * G, tok);
+        }
+        ph ^= 1;
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      TaSeg s;
+      constexpr uint32_t idesc_s = make_idesc(128, 128, 1, 1, 0, 0);
+      constexpr uint32_t idesc_o = make_idesc(128, DV, 1, 1, 0, 1);            // B (= V) is MN-major
+      const uint32_t q_addr = smem_u32(sQ), r_addr = smem_u32(ring);
+      uint32_t q_ph = 0, p_ph = 0;                                             // p_ph: a bit per group
+      int k_slot = 0, v_slot = 1;                                              // ring places of the next K and V tile: every other one
+      uint32_t k_ph = 0, v_ph = 0;
+      auto step_on = [&](int& slot, uint32_t& ph) { slot += 2; if (slot >= slots) { slot -= slots; ph ^= 1; } };
+      bool ok = true;
+      while (ok && walk.next(a, s)) {
+        if (s.n <= 0) continue;
+        const bool two = s.n_tiles == 2;
+        const int steps = two ? 2 * s.n : s.n;
+        if (!mbar_wait(q_full, q_ph, abort_flag, a.status, 820, s.seq)) break;
+        q_ph ^= 1;
+        // step i: group i & 1; KV block i, or i / 2 where the groups share the blocks
+        auto issue_s = [&](int i) -> bool {
+          const int p = i & 1;
+          if (!mbar_wait(&t_full[k_slot], k_ph, abort_flag, a.status, 821, i)) return false;
+          tc_fence_after();
+          const uint64_t qd = make_sdesc_sw128(q_addr + (two && p ? kQ : 0)), kd = make_sdesc_sw128(r_addr + k_slot * kSlot);
+#pragma unroll
+          for (int ks = 0; ks < DK / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
+            mma_f16_ss(tmem_base + p * 256, sdesc_at(qd, off), sdesc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[p]);
+          if (!two || p) { tc_commit(&t_empty[k_slot]); step_on(k_slot, k_ph); }
+          if (i == steps - 1) tc_commit(q_empty);
+          return true;
+        };
+        ok = issue_s(0);
+        if (ok && steps > 1) ok = issue_s(1);
+        for (int i = 0; i < steps && ok; ++i) {
+          const int p = i & 1;
+          if (!mbar_wait(&p_ready[p], (p_ph >> p) & 1, abort_flag, a.status, 822, i)) { ok = false; break; }
+          p_ph ^= 1u << p;
+          if (!mbar_wait(&t_full[v_slot], v_ph, abort_flag, a.status, 823, i)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t vd = make_sdesc_sw128_mn(r_addr + v_slot * kSlot, 16384);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)                                       // (the group's first block of the segment: O starts from zero)
+            mma_f16_ts(tmem_base + p * 256 + 128, tmem_base + p * 256 + ks * 8, sdesc_at(vd, ks * 2048), idesc_o, (i >= 2 || ks > 0) ? 1u : 0u);
+          if (!two || p) { tc_commit(&t_empty[v_slot]); step_on(v_slot, v_ph); }
+          if (i + 2 >= steps) tc_commit(&o_full[p]);                           // the group's last block
+          // The pipe runs this thread's MMAs in order: S of step i + 2 overwrites P of step i only after it has been read, and its arrival tells that O
+          // holds all of the group's earlier products.
+          if (i + 2 < steps) ok = issue_s(i + 2);
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax: one row per thread
+    const int g = warp >> 2;                                                   // group
+    const int r = threadIdx.x & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem_base + g * 256 + lane_off;
+    const int t_local = r / G, h_local = r - t_local * G;
+    uint32_t s_ph = 0, o_ph0 = 0, o_ph1 = 0;
+    uint32_t t0 = 0;                                                           // ring tiles in front of the segment
+    constexpr float kTau = 8.0f;       // O and the sum are rescaled only where a row's maximum has grown by more than 2^kTau
+    bool ok = true;
+    if (threadIdx.x == 0) { s_groups->walk = walk; s_groups->more[0] = s_groups->walk.next(a, s_groups->seg[0]); }
+    bar256_and(true);
+    for (int turn = 0; s_groups->more[turn]; turn ^= 1) {
+      const TaSeg& s = s_groups->seg[turn];
+      if (threadIdx.x == 0) s_groups->more[turn ^ 1] = s_groups->walk.next(a, s_groups->seg[turn ^ 1]);
+      const bool two = s.n_tiles == 2;
+      const int node = (s.tile + (two ? g : 0)) * tpt + t_local;               // of the sequence
+      const bool live = t_local < tpt && node < s.q.nodes;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      const int tok = s.q.begin + min(node, s.q.nodes - 1);
+      const unsigned long long* mrow = a.mask + (size_t)tok * a.words;
+      const int ctx = s.q.ctx, len = s.q.len;
+      const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first place of the context that the row sees
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int b = two ? 0 : g; b < s.n && ok; b += two ? 1 : 2) {
+        const int kv0 = (s.lo + b) * 128;
+        const bool tail = kv0 + 128 > min(ctx, len);                           // tree nodes, or places behind the end
+        ok = mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b);
+        if (!ok) break;
+        s_ph ^= 1;
+        if (tail && (!two || g == 0)) {
+          // Values of places that some row does not see must be finite: a weight of 0 times them is added.  Thread r looks at place r of the block; what is not
+          // finite is taken out, noted, and put back at the end for the rows that see it.  (Behind the wait for S, which tells that the products in front are done:
+          // in front of it the place's tile before this one may still be on its way, and its barrier two phases from the one waited for.)
+          const uint32_t t = t0 + 2 * b + 1;
+          ok = mbar_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b);
+          if (ok && kv0 + r >= min(ctx, len)) {
+            uint8_t* row = ring + (t % slots) * kSlot + r * 128;
+            bool odd = false;
+#pragma unroll 2
+            for (int c = 0; c < DV / 8; ++c) {
+              uint4* w = reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
+              uint4 v = *w;
+              uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+              bool put = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t keep = kv0 + r < len ? 0xffffffffu : 0u;
+                if ((x[k] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
+                if ((x[k] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
+                put |= keep != 0xffffffffu;
+                x[k] &= keep;
+              }
+              if (put) *w = v;
+              odd |= put;
+            }
+            const int x = kv0 + r - ctx;
+            if (odd && kv0 + r < len && x >= 0 && x < 256) atomicOr(&s_odd[x >> 5], 1 << (x & 31));
+          }
+          fence_proxy_async_smem();
+        }
+        if (!ok) break;
+        tc_fence_after();
+        __syncwarp();
+        if (warp_live) {
+          const bool edge = tail || kv0 < lo;
+          auto see_of = [&](int c) -> uint32_t {
+            const int k0 = kv0 + c * 32;
+            uint32_t see = low_bits(ctx - k0) & ~low_bits(lo - k0);
+            if (tail) see = (see | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
+            return see;
+          };
+          uint32_t see[4];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            float sv[64];
+            tmem_ld_x32(s_t + c * 32, reinterpret_cast<uint32_t*>(sv));
+            tmem_ld_x32(s_t + c * 32 + 32, reinterpret_cast<uint32_t*>(sv) + 32);
+            if (edge) { see[c] = see_of(c); see[c + 1] = see_of(c + 1); }
+            tc_wait_ld();
+            if (edge) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) if (!((see[c + (i >> 5)] >> (i & 31)) & 1)) sv[i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          float alpha = 1.0f;
+          const bool grow = top > m + kTau || (m == -INFINITY && top > -INFINITY);
+          if (grow) { alpha = fast_exp2(m - top); m = top; }
+          if (!first && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int c = 0; c < DV / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_x32(s_t + 128 + c * 32, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_x32(s_t + 128 + c * 32, o);
+            }
+          }
+          first = false;
+          const float ref = m == -INFINITY ? 0.f : m;
+          float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            float sv[64];
+            tmem_ld_x32(s_t + c * 32, reinterpret_cast<uint32_t*>(sv));
+            tmem_ld_x32(s_t + c * 32 + 32, reinterpret_cast<uint32_t*>(sv) + 32);
+            tc_wait_ld();
+            if (edge) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) if (!((see[c + (i >> 5)] >> (i & 31)) & 1)) sv[i] = -INFINITY;
+            }
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float p0 = fast_exp2(sv[2 * i] - ref), p1 = fast_exp2(sv[2 * i + 1] - ref);
+              rs[i & 1] += p0; rs[2 + (i & 1)] += p1;
+              pk[i] = pack_bf16x2(p0, p1);
+            }
+            tmem_st_x32(s_t + c * 16, pk);
+          }
+          l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+          tc_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&p_ready[g]);
+      }
+      t0 += 2 * s.n;
+      // ---- the segment's rows.  Both groups hold a share of every row (split: each writes half of the columns), or each has its own (one tile and one block: group 0)
+      const bool split = !two && s.n > 1;
+      const bool has = two || split || g == 0;                                 // this group writes something
+      float w0 = 0.f, w1 = 0.f, lse;                                           // factors of the accumulators (not split: w0 that of this group's)
+      s_x[g * 128 + r] = m;
+      ok = bar256_and(ok);                                                     // all 256 threads leave together
+      if (!ok) break;
+      if (split) {
+        const float mo = s_x[(g ^ 1) * 128 + r];
+        bar256_and(true);
+        s_x[g * 128 + r] = l;
+        bar256_and(true);
+        const float lo_ = s_x[(g ^ 1) * 128 + r], top = fmaxf(m, mo), ref = top == -INFINITY ? 0.f : top;
+        const float am = exp2f(m - ref), ao = exp2f(mo - ref);                 // -inf: 0
+        const float sum = g == 0 ? am * l + ao * lo_ : ao * lo_ + am * l;      // (in the same order in both groups)
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        w0 = (g == 0 ? am : ao) * inv;
+        w1 = (g == 0 ? ao : am) * inv;
+        lse = sum == 0.f ? -INFINITY : ref + log2f(sum);
+      } else {
+        w0 = l == 0.f ? 0.f : 1.0f / l;
+        lse = l == 0.f ? -INFINITY : m + log2f(l);
+      }
+      uint32_t any_odd = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) any_odd |= (uint32_t)s_odd[i];
+      const int own = two ? g : 0;                                             // the accumulator that w0 goes with
+      if (s.n > 0 && has) {
+        ok = mbar_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, s.seq);
+        if (split) ok = ok && mbar_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, s.seq);
+      }
+      if (s.n > 0) o_ph0 ^= 1;
+      if (two ? s.n > 0 : s.n > 1) o_ph1 ^= 1;
+      tc_fence_after();
+      __syncwarp();
+      if (ok && has && warp_live) {
+        const int head = s.kvh * G + h_local;
+        const long prow = ((long)(2 * blockIdx.x + (s.nth == 0 ? 0 : 1)) * a.pair + (two ? g : 0)) * 128 + r;      // of the parts
+        constexpr int kC = DV / 32;
+        const int c0 = split && g == 1 ? kC / 2 : 0, c1 = split && g == 0 ? kC / 2 : kC;
+        for (int c = c0; c < c1; ++c) {
+          float o[32];
+          __syncwarp();
+          if (s.n > 0) {
+            uint32_t o0[32], o1[32];
+            tmem_ld_x32(tmem_base + lane_off + own * 256 + 128 + c * 32, o0);
+            if (split) tmem_ld_x32(tmem_base + lane_off + 256 + 128 + c * 32, o1);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = split ? fmaf(__uint_as_float(o0[i]), w0, __uint_as_float(o1[i]) * w1) : __uint_as_float(o0[i]) * w0;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (live) {
+            if (any_odd) {
+              for (int x = 0; x < min(256, a.words * 64); ++x) {
+                if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
+                const int at = ctx + x;
+                const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
+                if (slot < 0 || slot >= a.num_slots) continue;
+                const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
+              }
+            }
+            if (s.full) {
+              uint4* dst = reinterpret_cast<uint4*>(a.out + ((size_t)tok * a.hq + head) * DV + c * 32);
+#pragma unroll
+              for (int v = 0; v < 4; ++v)
+                dst[v] = make_uint4(pack_bf16x2(o[v * 8], o[v * 8 + 1]), pack_bf16x2(o[v * 8 + 2], o[v * 8 + 3]), pack_bf16x2(o[v * 8 + 4], o[v * 8 + 5]),
+                                    pack_bf16x2(o[v * 8 + 6], o[v * 8 + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(a.part_o + prow * DV + c * 32);
+#pragma unroll
+              for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+            }
+          }
+        }
+        if (live && !s.full && c0 == 0) a.part_lse[prow] = lse;
+      }
+      if (threadIdx.x == 0 && !s.full && s.head) {
+        const long long last = s.pos + s.q.units - 1;                          // the item's last unit, and the piece it lies in
+        const int owner = (int)(((last + 1) * s_groups->walk.p.active - 1) / s_groups->walk.p.total);
+        a.part_of[blockIdx.x] = make_int4(s.seq, s.item, owner - (int)blockIdx.x + 1, 2 * (int)blockIdx.x + (s.nth == 0 ? 0 : 1));
+      }
+      if (any_odd) {
+        bar256_and(true);
+        if (threadIdx.x < 8) s_odd[threadIdx.x] = 0;
+      }
+      tc_fence_before();
+      ok = bar256_and(ok);                                                     // both accumulators and s_x are free again
+      if (!ok) break;
+    }
+  }
+  pdl_trigger();                       // a long kernel: its dependents are released at its end
+  if (*abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
+}
+
+// Joins the parts of the items that were cut: out = sum_i 2^(lse_i - max) O_i / sum_i 2^(lse_i - max), in the order of the parts.  One warp per row.
+template <int DV>
+__global__ void __launch_bounds__(256)
+tree_join_kernel(const TreeAttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int4 of = a.part_of[blockIdx.x];
+  if (of.z <= 0) return;
+  TaSeq q;
+  q.load(a, of.x);
+  const int G = a.hq / a.hkv, tpt = 128 / G, pairs = q.items / a.hkv;
+  const int kvh = of.y / pairs, tile = (of.y - kvh * pairs) * a.pair;
+  const int lane = threadIdx.x & 31;
+  const int per_block = a.pair * 128 / (int)gridDim.y;
+  for (int k = threadIdx.x >> 5; k < per_block; k += 8) {
+    const int row = blockIdx.y * per_block + k;                                // of the item
+    const int r = row & 127, t_local = r / G, node = (tile + (row >> 7)) * tpt + t_local;
+    if (t_local >= tpt || node >= q.nodes) continue;
+    auto at = [&](int i) { return (long)(i == 0 ? of.w : 2 * ((int)blockIdx.x + i)) * (a.pair * 128) + row; };
+    float top = -INFINITY;
+    for (int i = lane; i < of.z; i += 32) top = fmaxf(top, a.part_lse[at(i)]);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    constexpr int kV = DV / 32;
+    float acc[kV], den = 0.f;
+#pragma unroll
+    for (int v = 0; v < kV; ++v) acc[v] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < of.z; ++i) {
+      const float lse = a.part_lse[at(i)];
+      const float w = exp2f(lse - ref);
+      const float* o = a.part_o + at(i) * DV + lane * kV;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) acc[v] += lse == -INFINITY ? 0.f : w * o[v];
+      den += w;
+    }
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((size_t)(q.begin + node) * a.hq + kvh * G + (r - t_local * G)) * DV + lane * kV);
+#pragma unroll
+    for (int v = 0; v < kV / 2; ++v) dst[v] = pack_bf16x2(acc[2 * v] * inv, acc[2 * v + 1] * inv);
+  }
+}
+
+template <int DK, int DV>
+static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const void* v_cache, TreeAttnArgs a, int grid, cudaStream_t stream) {
+  const int G = a.hq / a.hkv, tpt = 128 / G;
+  CUtensorMap tmQ, tmK, tmV;
+  {
+    uint64_t dims[3] = {DK, (uint64_t)a.hq, (uint64_t)a.total_tokens};
+    uint64_t strides[2] = {DK * 2, (uint64_t)q_ts * 2};
+    uint32_t box[3] = {64, (uint32_t)G, (uint32_t)tpt};
+    if (make_tmap(&tmQ, q, TM_BF16, 3, dims, strides, box, TM_SW_128)) return -1;
+  }
+  {
+    uint64_t dk[3] = {DK, (uint64_t)a.hkv, (uint64_t)a.num_slots}, dv[3] = {DV, (uint64_t)a.hkv, (uint64_t)a.num_slots};
+    uint64_t sk[2] = {DK * 2, (uint64_t)a.hkv * DK * 2}, sv[2] = {DV * 2, (uint64_t)a.hkv * DV * 2};
+    uint32_t box[3] = {64, 1, (uint32_t)a.page_size};
+    if (make_tmap(&tmK, k_cache, TM_BF16, 3, dk, sk, box, TM_SW_128)) return -1;
+    if (make_tmap(&tmV, v_cache, TM_BF16, 3, dv, sv, box, TM_SW_128)) return -1;
+  }
+  static bool attr[64];
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  if (!attr[dev & 63]) {
+    GB_CUDA_OK(cudaFuncSetAttribute(tree_attn_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTaSmem));
+    attr[dev & 63] = true;
+  }
+  launch_k(tree_attn_kernel<DK, DV>, grid, kTaThreads, kTaSmem, stream, tmQ, tmK, tmV, a);
+  GB_CUDA_OK(cudaGetLastError());
+  if (!a.whole) {
+    launch_k(tree_join_kernel<DV>, dim3(grid, 4 * a.pair), 256, 0, stream, a);
+    GB_CUDA_OK(cudaGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace gb
+
+using namespace gb;
+
+// Blocks of the launch, and whether the items stay whole: bounds by what the host knows (at most max_pages pages and max_nodes nodes a sequence).
+static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int* pair, int* whole) {
+  const int tpt = 128 / (hq / hkv), tiles = (max_nodes + tpt - 1) / tpt;
+  *pair = tiles > 1 ? 2 : 1;
+  const long blocks = std::max(1l, ((long)max_pages * page_size + 127) / 128), items = (long)n_seqs * hkv * ((tiles + *pair - 1) / *pair);
+  *whole = blocks <= 2;
+  return (int)std::max(1l, std::min((long)sm_count(), *whole ? items : (items * blocks + 1) / 2));
+}
+
+// Floats of the workspace that gb_tree_attn wants.
+GB_API int gb_tree_attn_workspace(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int dv) {
+  int pair, whole;
+  const long grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &pair, &whole);
+  return whole ? 4 : (int)(grid * 4 + 2 * grid * pair * 128 * (dv + 1));          // (at most 148 * 2 * 2 * 128 rows)
+}
+
+GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const void* v_cache, void* out, float* workspace, const int* cu_q, const int* kv_len,
+                        const int* block_table, int max_pages, int page_size, const void* mask, int words, const int* positions, int n_seqs, long num_slots,
+                        int tokens, int max_nodes, int hq, int hkv, int dk, int dv, int window, void* status, cudaStream_t stream) {
+  if (tokens <= 0 || n_seqs <= 0) return 0;
+  if ((dk != 64 && dk != 128) || (dv != 64 && dv != 128)) return fail("tree_attn: heads of 64 or 128 columns%s");
+  if (hq < 1 || hkv < 1 || hq % hkv || hq / hkv > 128) return fail("tree_attn: bad head counts%s");
+  if (page_size < 8 || page_size > 128 || 128 % page_size) return fail("tree_attn: page_size must be 8..128 and divide 128%s");
+  if (max_nodes < 1 || words < 1 || max_pages < 0 || window < 0 || num_slots < 1) return fail("tree_attn: bad sizes%s");
+  if (window > 0 && positions == nullptr) return fail("tree_attn: a window needs the nodes' positions%s");
+  TreeAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &a.pair, &a.whole);
+  a.cu_q = cu_q; a.kv_len = kv_len; a.block_table = block_table; a.mask = (const unsigned long long*)mask; a.positions = positions; a.n_seqs = n_seqs;
+  a.max_pages = max_pages; a.page_size = page_size; a.words = words; a.window = window; a.hq = hq; a.hkv = hkv; a.total_tokens = tokens;
+  a.num_slots = num_slots; a.out = (__nv_bfloat16*)out; a.v_cache = (const __nv_bfloat16*)v_cache; a.status = (KernelStatus*)status;
+  if (!a.whole) {
+    a.part_of = (int4*)workspace;
+    a.part_o = workspace + grid * 4;
+    a.part_lse = a.part_o + 2l * grid * a.pair * 128 * dv;
+  }
+  if (dk == 64) return dv == 64 ? tree_attn_launch<64, 64>(q, q_ts, k_cache, v_cache, a, grid, stream) : tree_attn_launch<64, 128>(q, q_ts, k_cache, v_cache, a, grid, stream);
+  return dv == 64 ? tree_attn_launch<128, 64>(q, q_ts, k_cache, v_cache, a, grid, stream) : tree_attn_launch<128, 128>(q, q_ts, k_cache, v_cache, a, grid, stream);
+}

@@ -23,6 +23,9 @@ def _p(t):
     return _c(t.data_ptr()) if t is not None else _c(0)
 
 
+_TILE, _PAGES = (64, 128), (8, 16, 32, 64, 128)
+
+
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor,
                    page_size: int, mask: torch.Tensor, max_nodes: int, window: int = 0, positions: Optional[torch.Tensor] = None,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -64,8 +67,20 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         return tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window, positions, out)
     if t == 0 or b == 0:
         return out
+    lib = _native.cuda()
+    # the tcgen05 kernel's forms: its tiles hold 64 or 128 columns, 128 rows and whole pages, and TMA wants 16-byte boundaries
+    if q.dtype == torch.bfloat16 and dk in _TILE and dv in _TILE and page_size in _PAGES and hq // hkv <= 128 and q.stride(0) % 8 == 0 \
+            and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        with _native.on_device(dev):
+            cols = block_table.shape[1]
+            work = torch.empty(lib.gb_tree_attn_workspace(_i(b), _i(cols), _i(page_size), _i(max_nodes), _i(hq), _i(hkv), _i(dv)), dtype=torch.float32, device=dev)
+            rc = lib.gb_tree_attn(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _p(work), _p(cu_q), _p(kv_len), _p(block_table), _i(cols),
+                                  _i(page_size), _p(mask), _i(mask.shape[1]), _p(positions), _i(b), _l(slots), _i(t), _i(max_nodes), _i(hq), _i(hkv), _i(dk), _i(dv),
+                                  _i(window), _c(_native.status_ptr()), _c(_native.stream()))
+            _native.check(rc, "gb_tree_attn", n=1 if work.numel() <= 4 else 2)
+        return out
     with _native.on_device(dev):
-        rc = _native.cuda().gb_tree_any(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _i(int(q.dtype == torch.float32)), _p(cu_q), _p(kv_len),
+        rc = lib.gb_tree_any(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _i(int(q.dtype == torch.float32)), _p(cu_q), _p(kv_len),
                                         _p(block_table), _i(block_table.shape[1]), _i(page_size), _p(mask), _i(mask.shape[1]), _p(positions), _i(b), _l(slots),
                                         _i(t), _i(hq), _i(hkv), _i(dk), _i(dv), _i(window), _c(_native.stream()))
         _native.check(rc, "gb_tree_any")

@@ -272,6 +272,23 @@ def test_attention_kernel_masked_places(hq, hkv, n, d):
 
 
 @gpu
+@pytest.mark.parametrize("nodes,hkv,ctx", [(8, 4, 4000), (40, 2, 1500)])
+def test_attention_kernel_long_pieces(nodes, hkv, ctx):
+    """Many items to a block, with last blocks in all states of filling: every run gives the same, right answer."""
+    r = random.Random(nodes)
+    n, c = ([r.randint(1, top) for _ in range(48)] for top in (nodes, ctx))
+    s = attention_inputs(n, c, 4 * hkv, hkv, 128, 128, 128, seed=1)
+    dev = on_gpu(s)
+    cold = torch.empty(64 << 20, device="cuda")
+    got = []
+    for i in range(6):
+        cold.fill_(i)                                                       # the cache comes from HBM again
+        got.append(tree.tree_attention(**dev))
+    close(got[0], s)
+    assert all(torch.equal(g, got[0]) for g in got)
+
+
+@gpu
 def test_attention_kernel_rows_and_strides():
     """Query rows cut out of a wider projection; rows behind the last sequence keep what they hold; an empty batch."""
     s = attention_inputs([4, 9], [200, 33], 8, 2, 128, 128, 16)
