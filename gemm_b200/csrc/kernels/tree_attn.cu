@@ -2,15 +2,17 @@
 //
 // What a node sees, and the formula: tree_any.cu.  A row is a (node, query head of the group) pair, a tile is 128 rows of one KV head: floor(128 / G) nodes.
 // The context is long and the rows are few, so the kernel is built to stream K and V: one block per SM, its shared memory a ring of 32 KB tiles (K and V of
-// 128 places in turn) that TMA keeps full across work items, and two softmax groups of 128 threads, one thread per row.
+// 128 places in turn) that TMA keeps full across work items, and two softmax groups of 128 threads, one thread per TMEM lane.
 //   one tile in the item:   the groups take alternate KV blocks, each with its own maximum, sum and output accumulator, joined at the end;
 //   two tiles in the item:  each group has its tile, and both use the same K and V (wide trees: half the loads, which would bound the products).
+// A tile of 64 rows or fewer is folded: its rows lie two or four times in the 128 lanes, and each copy's thread takes that share of a block's places (zeros stand in P
+// for the others), with a maximum and a sum of its own.  The products cost the same, and the chain S -> weights -> P is half or a quarter as long.
 // TMEM: S / P (128 columns, P overwrites S in place) and O (128 columns) per group: all of it.
 //
 // Work: KV blocks of all (sequence, KV head, tile pair) items in one line, cut into equal pieces, one per SM: a long context is shared by many SMs, short ones
 // fill one, whatever the mix.  The cut goes by lengths that only the device knows (a captured launch may be replayed with other ones), so every block works out
-// its piece from the lengths.  A piece that holds an item's part leaves the part's output (f32, normalised) and base-2 logarithm of its sum in a workspace; a second
-// launch joins the parts in the order of their blocks.
+// its piece from the lengths, and one warp hands its segments to the others.  A piece that holds an item's part leaves the part's output (f32, normalised) and base-2
+// logarithm of its sum in a workspace; a second launch joins the parts in the order of their blocks.
 //
 // P is rounded to bf16 for the second product (the tensor cores' operand type; sums stay f32): at most 2^-9 of each weight.
 #include "sm100.cuh"
@@ -19,14 +21,16 @@
 
 namespace gb {
 
-constexpr int kTaThreads = 352;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads
-constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, the rest is the ring
+constexpr int kTaThreads = 384;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads; 11: segments
+constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, with folded rows one to join them in, the rest is the ring
+constexpr int kTaSegs = 4;          // segments handed out ahead
 constexpr int kTaSmem = 1024 + kTaTiles * 32768 + 2048;
 
 struct TreeAttnArgs {
   const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
   int n_seqs, max_pages, page_size, words, window, hq, hkv, total_tokens;
   int pair;                          // tiles per item: 1 or 2
+  int fold;                          // copies of the rows in a tile: 1, 2 or 4 (pair = 1, and at most 128 / fold rows in any sequence)
   int whole;                         // items are not cut (short contexts): no parts
   __nv_bfloat16* out;                // [T, hq, DV]
   float* part_o; float* part_lse;    // [2 * grid][pair * 128][DV], [2 * grid][pair * 128]
@@ -39,7 +43,7 @@ struct TreeAttnArgs {
 struct TaSeq {
   int begin, nodes, len, ctx, first, blocks, units, tiles, items;
   __device__ __forceinline__ void load(const TreeAttnArgs& a, int s) {
-    const int G = a.hq / a.hkv, tpt = 128 / G;
+    const int G = a.hq / a.hkv, tpt = 128 / a.fold / G;
     begin = min(max(a.cu_q[s], 0), a.total_tokens);
     nodes = max(min(a.cu_q[s + 1], a.total_tokens) - begin, 0);
     const int kv = a.kv_len[s];
@@ -64,9 +68,9 @@ struct TaSeg {
   TaSeq q;
   int seq, item, kvh, tile, n_tiles;      // first tile, 1 or 2 of them
   int lo, n;                              // KV blocks [lo, lo + n) of the sequence
-  bool full, head;                        // all of the item's blocks; its first ones
-  int nth;                                // number of the segment in its piece
-  long long pos;                          // its first unit's place in the line
+  bool full;                              // all of the item's blocks
+  int slot;                               // of its part in the workspace
+  int parts;                              // the item begins here and is cut: into so many parts
 };
 
 struct TaWalk {
@@ -81,7 +85,13 @@ struct TaWalk {
     s.q = q; s.seq = p.seq; s.item = p.item;
     s.kvh = p.item / pairs; s.tile = (p.item - s.kvh * pairs) * a.pair; s.n_tiles = min(a.pair, q.tiles - s.tile);
     s.lo = q.first + (a.whole ? 0 : p.unit); s.n = a.whole ? q.blocks : min(take, q.blocks - p.unit);
-    s.full = take == q.units; s.head = p.unit == 0; s.nth = nth++; s.pos = p.pos;
+    s.full = take == q.units;
+    s.slot = 2 * (int)blockIdx.x + (nth++ == 0 ? 0 : 1);
+    s.parts = 0;
+    if (!s.full && p.unit == 0) {
+      const long long last = p.pos + q.units - 1;                  // the item's last unit; the piece it lies in is the last one that begins at or before it
+      s.parts = (int)(((last + 1) * p.active - 1) / p.total) - (int)blockIdx.x + 1;
+    }
     p.left -= take; p.pos += take; p.unit += take;
     if (p.unit == q.units) {
       p.unit = 0;
@@ -92,13 +102,6 @@ struct TaWalk {
     }
     return true;
   }
-};
-
-// What the softmax groups keep of the walk, in shared memory: thread 0 finds the next segment while the present one is worked on (their registers hold a row of scores).
-struct TaGroups {
-  TaWalk walk;
-  TaSeg seg[2];
-  int more[2];
 };
 
 __device__ __forceinline__ bool bar256_and(bool pred) {
@@ -119,32 +122,116 @@ __device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
-template <int DK, int DV>
+// 128 threads of softmax group g.
+__device__ __forceinline__ void bar_group(int g) { asm volatile("bar.sync %0, 128;" :: "r"(3 + g) : "memory"); }
+
+// 64 bytes of a row in two stores.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// One block's step of a softmax thread: NC = 128 / FOLD of the block's scores, from column `at` on.  Returns the factor that the sum and O were scaled by in `l`, `m`.
+template <int DV, int FOLD>
+__device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first, bool edge, const uint32_t* see, float& m, float& l) {
+  constexpr float kTau = 8.0f;         // O and the sum are rescaled only where a row's maximum has grown by more than 2^kTau
+  constexpr int NC = 128 / FOLD, CH = NC < 64 ? NC : 64;
+  const uint32_t s_at = s_t + fold * NC;
+  float sv[CH];
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < NC; c += CH) {
+#pragma unroll
+    for (int k = 0; k < CH; k += 32) tmem_ld_x32(s_at + c + k, reinterpret_cast<uint32_t*>(sv) + k);
+    tc_wait_ld();
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) if (!((see[(c + i) >> 5] >> (i & 31)) & 1)) sv[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
+  }
+  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  float alpha = 1.0f;
+  const bool grow = top > m + kTau || (m == -INFINITY && top > -INFINITY);
+  if (grow) { alpha = fast_exp2(m - top); m = top; }
+  if (!first && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+    for (int c = 0; c < DV / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld_x32(s_t + 128 + c * 32, o);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      tmem_st_x32(s_t + 128 + c * 32, o);
+    }
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < NC; c += CH) {
+    if constexpr (NC > CH) {                                       // (all 128 at once do not fit the registers: read again)
+#pragma unroll
+      for (int k = 0; k < CH; k += 32) tmem_ld_x32(s_at + c + k, reinterpret_cast<uint32_t*>(sv) + k);
+      tc_wait_ld();
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) if (!((see[(c + i) >> 5] >> (i & 31)) & 1)) sv[i] = -INFINITY;
+      }
+    }
+    uint32_t pk[CH / 2];
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+      const float p0 = fast_exp2(sv[2 * i] - ref), p1 = fast_exp2(sv[2 * i + 1] - ref);
+      rs[i & 1] += p0; rs[2 + (i & 1)] += p1;
+      pk[i] = pack_bf16x2(p0, p1);
+    }
+    if constexpr (FOLD == 4) tmem_st_x16(s_t + fold * 16, pk);
+    else tmem_st_x32(s_t + (fold * NC + c) / 2, pk);
+  }
+  if constexpr (FOLD > 1) {                                        // the other copies' places
+    uint32_t z[NC / 2];
+#pragma unroll
+    for (int i = 0; i < NC / 2; ++i) z[i] = 0;
+#pragma unroll
+    for (int f = 1; f < FOLD; ++f) {
+      const int x = (fold + f) & (FOLD - 1);
+      if constexpr (FOLD == 4) tmem_st_x16(s_t + x * 16, z);
+      else tmem_st_x32(s_t + x * 32, z);
+    }
+  }
+  l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+  tc_wait_st();
+}
+
+template <int DK, int DV, int FOLD>
 __global__ void __launch_bounds__(kTaThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV);
+  constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV), kStage = FOLD > 1 ? 32768 : 0;
   uint8_t* sQ = smem;                                             // pair x [128 rows] (64-column halves of 128 B, swizzled)
-  uint8_t* ring = smem + a.pair * kQ;
-  const int slots = min(10, (int)((kTaTiles * 32768 - a.pair * kQ) / kSlot));
+  float* s_stage = (float*)(smem + kQ);                           // FOLD > 1: [2 groups][32 columns][96 lanes of the copies]
+  uint8_t* ring = smem + a.pair * kQ + kStage;
+  const int slots = min(10, (int)((kTaTiles * 32768 - a.pair * kQ - kStage) / kSlot));
   uint64_t* bars = (uint64_t*)(smem + kTaTiles * 32768);
   uint64_t* q_full = bars; uint64_t* q_empty = bars + 1;
   uint64_t* s_full = bars + 2; uint64_t* p_ready = bars + 4; uint64_t* o_full = bars + 6;      // [2] each, by group
   uint64_t* t_full = bars + 8; uint64_t* t_empty = bars + 18;                                  // [10] each
-  uint32_t* tmem_slot = (uint32_t*)(bars + 28);
+  uint64_t* g_full = bars + 28; uint64_t* g_empty = bars + 32;                                 // [kTaSegs] each
+  uint32_t* tmem_slot = (uint32_t*)(bars + 36);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   int* s_odd = (int*)(tmem_slot + 2);                             // [8] tree nodes of the segment whose value rows are not finite, as bits
-  float* s_x = (float*)(bars + 36);                               // [2][128]: what the groups tell each other about a row
+  float* s_x = (float*)(bars + 42);                               // [2][128]: what the groups tell each other about a row
   long long* s_scan = (long long*)s_x;                            // prologue only
   TaPiece* s_piece = (TaPiece*)(s_x + 256);
-  TaGroups* s_groups = (TaGroups*)(s_x + 256);                    // behind the prologue
+  TaSeg* s_seg = (TaSeg*)(s_piece + 1);                           // [kTaSegs]; n_tiles = 0: no more
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1); mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 128); mbar_init(&o_full[i], 1); }
     for (int i = 0; i < 10; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 1); }
+    for (int i = 0; i < kTaSegs; ++i) { mbar_init(&g_full[i], 1); mbar_init(&g_empty[i], 4); }      // (a softmax thread and the warps 8, 9, 10 give a segment back)
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) s_odd[i] = 0;
     fence_barrier_init();
@@ -163,7 +250,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
     if (lane == 31) s_scan[warp] = incl;
-    if (threadIdx.x == 0) { s_piece->left = 0; s_piece->total = 0; }
+    if (threadIdx.x == 0) { s_piece->left = 0; s_piece->total = 0; if (a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -172,7 +259,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const long long excl = front + incl - mine;
     // at least two units a piece: a part costs more to write and join than a block to work on
     const int active = (int)min((long long)gridDim.x, a.whole ? total : (total + 1) / 2);
-    if ((int)blockIdx.x < active) {
+    if ((int)blockIdx.x < active && mine > 0) {
       const long long lo = blockIdx.x * total / active, hi = (blockIdx.x + 1ll) * total / active;
       if (excl <= lo && lo < excl + mine) {
         long long at = excl;
@@ -184,29 +271,45 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     __syncthreads();
   }
-  TaWalk walk;
-  walk.p = *s_piece;
-  walk.at = -1; walk.nth = 0;
-  __syncthreads();                                                // s_x is the groups' from here on
   const uint32_t tmem_base = *tmem_slot;
-  const int G = a.hq / a.hkv, tpt = 128 / G;
-  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0);
+  const int G = a.hq / a.hkv, tpt = 128 / FOLD / G;
 
-  if (warp == 8) {
-    TaSeg s;
+  if (warp == 11) {
+    // ---------------------------------------------------------------- segments
+    if (lane == 0) {
+      TaWalk walk;
+      walk.p = *s_piece;
+      walk.at = -1; walk.nth = 0;
+      for (int k = 0;; ++k) {
+        const int i = k % kTaSegs;
+        if (!mbar_wait(&g_empty[i], ((k / kTaSegs) & 1) ^ 1, abort_flag, a.status, 840, k)) break;
+        TaSeg s;
+        const bool more = walk.next(a, s);
+        if (!more) s.n_tiles = 0;
+        s_seg[i] = s;
+        mbar_arrive(&g_full[i]);
+        if (!more) break;
+      }
+    }
+  } else if (warp == 8) {
     // ---------------------------------------------------------------- K and V: the lanes fetch and issue a page each
     const int ppb = 128 / a.page_size;
     const uint32_t page_bytes = (uint32_t)a.page_size * 128;
     int slot = 0; uint32_t ph = 0;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
-      if (s.n <= 0) continue;
-      const int* bt = a.block_table + (size_t)s.seq * a.max_pages;
-      const int last_page = (s.q.len + a.page_size - 1) / a.page_size - 1;
-      int page = lane < ppb ? bt[min(s.lo * ppb + lane, last_page)] : 0;
-      for (int j = 0; j < s.n && ok; ++j) {
+    for (int k = 0; ok; ++k) {
+      const int i = k % kTaSegs;
+      ok = __all_sync(0xffffffffu, mbar_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 801, k));
+      if (!ok || s_seg[i].n_tiles == 0) break;
+      const int lo = s_seg[i].lo, n = s_seg[i].n, kvh = s_seg[i].kvh, len = s_seg[i].q.len;
+      const int* bt = a.block_table + (size_t)s_seg[i].seq * a.max_pages;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&g_empty[i]);
+      const int last_page = (len + a.page_size - 1) / a.page_size - 1;
+      int page = n > 0 && lane < ppb ? bt[min(lo * ppb + lane, last_page)] : 0;
+      for (int j = 0; j < n && ok; ++j) {
         const int now = page;
-        if (j + 1 < s.n && lane < ppb) page = bt[min((s.lo + j + 1) * ppb + lane, last_page)];      // (pages behind the end: the last one again; nothing of them counts)
+        if (j + 1 < n && lane < ppb) page = bt[min((lo + j + 1) * ppb + lane, last_page)];      // (pages behind the end: the last one again; nothing of them counts)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           ok = ok && mbar_wait(&t_empty[slot], ph ^ 1, abort_flag, a.status, 800, j);
@@ -218,8 +321,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           __syncwarp();
           if (lane < ppb) {
             uint8_t* dst = ring + slot * kSlot + lane * page_bytes;
-            tma_load_3d(dst, tm, &t_full[slot], 0, s.kvh, now * a.page_size);
-            if (D > 64) tma_load_3d(dst + 16384, tm, &t_full[slot], 64, s.kvh, now * a.page_size);
+            tma_load_3d(dst, tm, &t_full[slot], 0, kvh, now * a.page_size);
+            if (D > 64) tma_load_3d(dst + 16384, tm, &t_full[slot], 64, kvh, now * a.page_size);
           }
           if (++slot == slots) { slot = 0; ph ^= 1; }
         }
@@ -227,23 +330,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   } else if (warp == 10) {
     if (lane == 0) {
-      TaSeg s;
       uint32_t ph = 0;
-      while (walk.next(a, s)) {
-        if (s.n <= 0) continue;
-        if (!mbar_wait(q_empty, ph ^ 1, abort_flag, a.status, 810, s.seq)) break;
-        mbar_expect_tx(q_full, (uint32_t)(2 * DK * G * tpt) * s.n_tiles);
-        for (int t = 0; t < s.n_tiles; ++t) {
-          const int tok = s.q.begin + (s.tile + t) * tpt;
-          tma_load_3d(sQ + t * kQ, &tmQ, q_full, 0, s.kvh * G, tok);
-          if constexpr (DK > 64) tma_load_3d(sQ + t * kQ + 16384, &tmQ, q_full, 64, s.kvh * G, tok);
+      for (int k = 0;; ++k) {
+        const int i = k % kTaSegs;
+        if (!mbar_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 811, k) || s_seg[i].n_tiles == 0) break;
+        const int n = s_seg[i].n, n_tiles = s_seg[i].n_tiles, kvh = s_seg[i].kvh, begin = s_seg[i].q.begin + s_seg[i].tile * tpt;
+        mbar_arrive(&g_empty[i]);
+        if (n <= 0) continue;
+        if (!mbar_wait(q_empty, ph ^ 1, abort_flag, a.status, 810, k)) break;
+        mbar_expect_tx(q_full, (uint32_t)(2 * DK * G * tpt) * FOLD * n_tiles);
+        for (int t = 0; t < n_tiles * FOLD; ++t) {
+          uint8_t* dst = FOLD > 1 ? sQ + t * (128 / FOLD) * 128 : sQ + t * kQ;      // a copy of the rows, or the second tile
+          const int tok = begin + (FOLD > 1 ? 0 : t * tpt);
+          tma_load_3d(dst, &tmQ, q_full, 0, kvh * G, tok);
+          if constexpr (DK > 64) tma_load_3d(dst + 16384, &tmQ, q_full, 64, kvh * G, tok);
         }
         ph ^= 1;
       }
     }
   } else if (warp == 9) {
     if (lane == 0) {
-      TaSeg s;
       constexpr uint32_t idesc_s = make_idesc(128, 128, 1, 1, 0, 0);
       constexpr uint32_t idesc_o = make_idesc(128, DV, 1, 1, 0, 1);            // B (= V) is MN-major
       const uint32_t q_addr = smem_u32(sQ), r_addr = smem_u32(ring);
@@ -252,11 +358,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       uint32_t k_ph = 0, v_ph = 0;
       auto step_on = [&](int& slot, uint32_t& ph) { slot += 2; if (slot >= slots) { slot -= slots; ph ^= 1; } };
       bool ok = true;
-      while (ok && walk.next(a, s)) {
-        if (s.n <= 0) continue;
-        const bool two = s.n_tiles == 2;
-        const int steps = two ? 2 * s.n : s.n;
-        if (!mbar_wait(q_full, q_ph, abort_flag, a.status, 820, s.seq)) break;
+      for (int k = 0; ok; ++k) {
+        const int sg = k % kTaSegs;
+        if (!mbar_wait(&g_full[sg], (k / kTaSegs) & 1, abort_flag, a.status, 824, k) || s_seg[sg].n_tiles == 0) break;
+        const bool two = s_seg[sg].n_tiles == 2;
+        const int n = s_seg[sg].n, steps = two ? 2 * n : n;
+        mbar_arrive(&g_empty[sg]);
+        if (n <= 0) continue;
+        if (!mbar_wait(q_full, q_ph, abort_flag, a.status, 820, k)) break;
         q_ph ^= 1;
         // step i: group i & 1; KV block i, or i / 2 where the groups share the blocks
         auto issue_s = [&](int i) -> bool {
@@ -295,34 +404,40 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
     }
   } else {
-    // ---------------------------------------------------------------- softmax: one row per thread
+    // ---------------------------------------------------------------- softmax: one TMEM lane per thread
     const int g = warp >> 2;                                                   // group
-    const int r = threadIdx.x & 127;
+    const int r = threadIdx.x & 127, fold = r / (128 / FOLD), rr = r % (128 / FOLD);      // lane; copy of the rows; row (fold is the same for a warp)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem_base + g * 256 + lane_off;
-    const int t_local = r / G, h_local = r - t_local * G;
+    const int t_local = rr / G, h_local = rr - t_local * G;
     uint32_t s_ph = 0, o_ph0 = 0, o_ph1 = 0;
     uint32_t t0 = 0;                                                           // ring tiles in front of the segment
-    constexpr float kTau = 8.0f;       // O and the sum are rescaled only where a row's maximum has grown by more than 2^kTau
-    bool ok = true;
-    if (threadIdx.x == 0) { s_groups->walk = walk; s_groups->more[0] = s_groups->walk.next(a, s_groups->seg[0]); }
-    bar256_and(true);
-    for (int turn = 0; s_groups->more[turn]; turn ^= 1) {
-      const TaSeg& s = s_groups->seg[turn];
-      if (threadIdx.x == 0) s_groups->more[turn ^ 1] = s_groups->walk.next(a, s_groups->seg[turn ^ 1]);
-      const bool two = s.n_tiles == 2;
+    bool ok = bar256_and(mbar_wait(&g_full[0], 0, abort_flag, a.status, 834, 0));
+    for (int k = 0; ok && s_seg[k % kTaSegs].n_tiles > 0; ++k) {
+      const TaSeg& s = s_seg[k % kTaSegs];
+      const bool two = FOLD == 1 && s.n_tiles == 2;
+      const int n = s.n, ctx = s.q.ctx, len = s.q.len, blk0 = s.lo;
       const int node = (s.tile + (two ? g : 0)) * tpt + t_local;               // of the sequence
       const bool live = t_local < tpt && node < s.q.nodes;
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int tok = s.q.begin + min(node, s.q.nodes - 1);
       const unsigned long long* mrow = a.mask + (size_t)tok * a.words;
-      const int ctx = s.q.ctx, len = s.q.len;
       const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first place of the context that the row sees
       float m = -INFINITY, l = 0.f;
       bool first = true;
-      for (int b = two ? 0 : g; b < s.n && ok; b += two ? 1 : 2) {
-        const int kv0 = (s.lo + b) * 128;
+      for (int b = two ? 0 : g; b < n && ok; b += two ? 1 : 2) {
+        const int kv0 = (blk0 + b) * 128;
         const bool tail = kv0 + 128 > min(ctx, len);                           // tree nodes, or places behind the end
+        const bool edge = tail || kv0 < lo;
+        uint32_t see[4 / FOLD];
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4 / FOLD; ++c) {
+            const int k0 = kv0 + (fold * (4 / FOLD) + c) * 32;
+            see[c] = low_bits(ctx - k0) & ~low_bits(lo - k0);
+            if (tail) see[c] = (see[c] | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
+          }
+        }
         ok = mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b);
         if (!ok) break;
         s_ph ^= 1;
@@ -342,12 +457,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               uint32_t* x = reinterpret_cast<uint32_t*>(&v);
               bool put = false;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int e = 0; e < 4; ++e) {
                 uint32_t keep = kv0 + r < len ? 0xffffffffu : 0u;
-                if ((x[k] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
-                if ((x[k] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
+                if ((x[e] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
+                if ((x[e] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
                 put |= keep != 0xffffffffu;
-                x[k] &= keep;
+                x[e] &= keep;
               }
               if (put) *w = v;
               odd |= put;
@@ -360,167 +475,126 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!ok) break;
         tc_fence_after();
         __syncwarp();
-        if (warp_live) {
-          const bool edge = tail || kv0 < lo;
-          auto see_of = [&](int c) -> uint32_t {
-            const int k0 = kv0 + c * 32;
-            uint32_t see = low_bits(ctx - k0) & ~low_bits(lo - k0);
-            if (tail) see = (see | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
-            return see;
-          };
-          uint32_t see[4];
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            float sv[64];
-            tmem_ld_x32(s_t + c * 32, reinterpret_cast<uint32_t*>(sv));
-            tmem_ld_x32(s_t + c * 32 + 32, reinterpret_cast<uint32_t*>(sv) + 32);
-            if (edge) { see[c] = see_of(c); see[c + 1] = see_of(c + 1); }
-            tc_wait_ld();
-            if (edge) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i) if (!((see[c + (i >> 5)] >> (i & 31)) & 1)) sv[i] = -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          float alpha = 1.0f;
-          const bool grow = top > m + kTau || (m == -INFINITY && top > -INFINITY);
-          if (grow) { alpha = fast_exp2(m - top); m = top; }
-          if (!first && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
-            for (int c = 0; c < DV / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_x32(s_t + 128 + c * 32, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_x32(s_t + 128 + c * 32, o);
-            }
-          }
-          first = false;
-          const float ref = m == -INFINITY ? 0.f : m;
-          float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            float sv[64];
-            tmem_ld_x32(s_t + c * 32, reinterpret_cast<uint32_t*>(sv));
-            tmem_ld_x32(s_t + c * 32 + 32, reinterpret_cast<uint32_t*>(sv) + 32);
-            tc_wait_ld();
-            if (edge) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i) if (!((see[c + (i >> 5)] >> (i & 31)) & 1)) sv[i] = -INFINITY;
-            }
-            uint32_t pk[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float p0 = fast_exp2(sv[2 * i] - ref), p1 = fast_exp2(sv[2 * i + 1] - ref);
-              rs[i & 1] += p0; rs[2 + (i & 1)] += p1;
-              pk[i] = pack_bf16x2(p0, p1);
-            }
-            tmem_st_x32(s_t + c * 16, pk);
-          }
-          l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-          tc_wait_st();
-        }
+        if (warp_live) softmax_step<DV, FOLD>(s_t, fold, first, edge, see, m, l);
+        first = false;
         tc_fence_before();
         mbar_arrive(&p_ready[g]);
       }
-      t0 += 2 * s.n;
-      // ---- the segment's rows.  Both groups hold a share of every row (split: each writes half of the columns), or each has its own (one tile and one block: group 0)
-      const bool split = !two && s.n > 1;
-      const bool has = two || split || g == 0;                                 // this group writes something
-      float w0 = 0.f, w1 = 0.f, lse;                                           // factors of the accumulators (not split: w0 that of this group's)
+      t0 += 2 * n;
+      // ---- the segment's rows.  Two tiles: each group writes its own.  One tile: both groups (and all copies) hold a share of every row, and each group
+      // writes half of the columns.
+      const int own = two ? g : 0;
+      const bool both = !two && n > 1;                                         // accumulator 1 holds something of this group's rows too
+      float w0, w1 = 0.f, lse;                                                 // factors of the lane's accumulators
       s_x[g * 128 + r] = m;
       ok = bar256_and(ok);                                                     // all 256 threads leave together
       if (!ok) break;
-      if (split) {
-        const float mo = s_x[(g ^ 1) * 128 + r];
+      if (two) {
+        w0 = l == 0.f ? 0.f : 1.0f / l;
+        lse = l == 0.f ? -INFINITY : m + log2f(l);
+      } else {
+        float ms[2 * FOLD], top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 2 * FOLD; ++x) { ms[x] = s_x[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr]; top = fmaxf(top, ms[x]); }
         bar256_and(true);
         s_x[g * 128 + r] = l;
         bar256_and(true);
-        const float lo_ = s_x[(g ^ 1) * 128 + r], top = fmaxf(m, mo), ref = top == -INFINITY ? 0.f : top;
-        const float am = exp2f(m - ref), ao = exp2f(mo - ref);                 // -inf: 0
-        const float sum = g == 0 ? am * l + ao * lo_ : ao * lo_ + am * l;      // (in the same order in both groups)
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, e0 = 0.f, e1 = 0.f;
+#pragma unroll
+        for (int x = 0; x < 2 * FOLD; ++x) {                                   // (2^-inf = 0)
+          const float e = exp2f(ms[x] - ref);
+          sum += e * s_x[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr];
+          if (x == fold) e0 = e;
+          if (x == FOLD + fold) e1 = e;
+        }
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        w0 = (g == 0 ? am : ao) * inv;
-        w1 = (g == 0 ? ao : am) * inv;
+        w0 = e0 * inv;
+        w1 = e1 * inv;
         lse = sum == 0.f ? -INFINITY : ref + log2f(sum);
-      } else {
-        w0 = l == 0.f ? 0.f : 1.0f / l;
-        lse = l == 0.f ? -INFINITY : m + log2f(l);
       }
       uint32_t any_odd = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) any_odd |= (uint32_t)s_odd[i];
-      const int own = two ? g : 0;                                             // the accumulator that w0 goes with
-      if (s.n > 0 && has) {
-        ok = mbar_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, s.seq);
-        if (split) ok = ok && mbar_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, s.seq);
+      if (n > 0) {
+        ok = mbar_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, k);
+        if (both) ok = ok && mbar_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, k);
+        o_ph0 ^= 1;
+        if (two || n > 1) o_ph1 ^= 1;
       }
-      if (s.n > 0) o_ph0 ^= 1;
-      if (two ? s.n > 0 : s.n > 1) o_ph1 ^= 1;
       tc_fence_after();
-      __syncwarp();
-      if (ok && has && warp_live) {
-        const int head = s.kvh * G + h_local;
-        const long prow = ((long)(2 * blockIdx.x + (s.nth == 0 ? 0 : 1)) * a.pair + (two ? g : 0)) * 128 + r;      // of the parts
-        constexpr int kC = DV / 32;
-        const int c0 = split && g == 1 ? kC / 2 : 0, c1 = split && g == 0 ? kC / 2 : kC;
-        for (int c = c0; c < c1; ++c) {
-          float o[32];
-          __syncwarp();
-          if (s.n > 0) {
-            uint32_t o0[32], o1[32];
-            tmem_ld_x32(tmem_base + lane_off + own * 256 + 128 + c * 32, o0);
-            if (split) tmem_ld_x32(tmem_base + lane_off + 256 + 128 + c * 32, o1);
-            tc_wait_ld();
+      const int head = s.kvh * G + h_local;
+      const long prow = ((long)s.slot * a.pair + (two ? g : 0)) * 128 + rr;    // of the parts
+      const bool full = s.full;
+      constexpr int kC = DV / 32;
+      const int c0 = !two && g == 1 ? kC / 2 : 0, c1 = !two && g == 0 ? kC / 2 : kC;
+      for (int c = c0; c < c1; ++c) {
+        float o[32];
+        __syncwarp();
+        if (ok && n > 0 && warp_live) {
+          uint32_t o0[32], o1[32];
+          tmem_ld_x32(tmem_base + lane_off + own * 256 + 128 + c * 32, o0);
+          if (both) tmem_ld_x32(tmem_base + lane_off + 256 + 128 + c * 32, o1);
+          tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = split ? fmaf(__uint_as_float(o0[i]), w0, __uint_as_float(o1[i]) * w1) : __uint_as_float(o0[i]) * w0;
-          } else {
+          for (int i = 0; i < 32; ++i) o[i] = both ? fmaf(__uint_as_float(o0[i]), w0, __uint_as_float(o1[i]) * w1) : __uint_as_float(o0[i]) * w0;
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if constexpr (FOLD > 1) {                                              // the copies' shares go to the first one's threads
+          float* st = s_stage + g * 32 * 96 + (r - 128 / FOLD);
+          if (fold > 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) st[i * 96] = o[i];
           }
-          if (live) {
-            if (any_odd) {
-              for (int x = 0; x < min(256, a.words * 64); ++x) {
-                if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
-                const int at = ctx + x;
-                const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
-                if (slot < 0 || slot >= a.num_slots) continue;
-                const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
+          bar_group(g);
+          if (fold == 0) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
-              }
+            for (int f = 1; f < FOLD; ++f) {
+              const float* sf = s_stage + g * 32 * 96 + (f - 1) * (128 / FOLD) + rr;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] += sf[i * 96];
             }
-            if (s.full) {
-              uint4* dst = reinterpret_cast<uint4*>(a.out + ((size_t)tok * a.hq + head) * DV + c * 32);
+          }
+          bar_group(g);
+        }
+        if (ok && live && fold == 0) {
+          if (any_odd) {
+            for (int x = 0; x < min(256, a.words * 64); ++x) {
+              if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
+              const int at = ctx + x;
+              const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
+              if (slot < 0 || slot >= a.num_slots) continue;
+              const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
 #pragma unroll
-              for (int v = 0; v < 4; ++v)
-                dst[v] = make_uint4(pack_bf16x2(o[v * 8], o[v * 8 + 1]), pack_bf16x2(o[v * 8 + 2], o[v * 8 + 3]), pack_bf16x2(o[v * 8 + 4], o[v * 8 + 5]),
-                                    pack_bf16x2(o[v * 8 + 6], o[v * 8 + 7]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + prow * DV + c * 32);
-#pragma unroll
-              for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+              for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
             }
+          }
+          if (full) {
+            __nv_bfloat16* dst = a.out + ((size_t)tok * a.hq + head) * DV + c * 32;
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
+            store32(dst, w);
+            store32(dst + 16, w + 8);
+          } else {
+            float* dst = a.part_o + prow * DV + c * 32;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) store32(dst + v * 8, reinterpret_cast<const uint32_t*>(o) + v * 8);
           }
         }
-        if (live && !s.full && c0 == 0) a.part_lse[prow] = lse;
       }
-      if (threadIdx.x == 0 && !s.full && s.head) {
-        const long long last = s.pos + s.q.units - 1;                          // the item's last unit, and the piece it lies in
-        const int owner = (int)(((last + 1) * s_groups->walk.p.active - 1) / s_groups->walk.p.total);
-        a.part_of[blockIdx.x] = make_int4(s.seq, s.item, owner - (int)blockIdx.x + 1, 2 * (int)blockIdx.x + (s.nth == 0 ? 0 : 1));
-      }
+      if (live && fold == 0 && !full && c0 == 0) a.part_lse[prow] = lse;
+      if (threadIdx.x == 0 && s.parts > 0) a.part_of[blockIdx.x] = make_int4(s.seq, s.item, s.parts, s.slot);
       if (any_odd) {
         bar256_and(true);
         if (threadIdx.x < 8) s_odd[threadIdx.x] = 0;
       }
       tc_fence_before();
-      ok = bar256_and(ok);                                                     // both accumulators and s_x are free again
-      if (!ok) break;
+      ok = ok && mbar_wait(&g_full[(k + 1) % kTaSegs], ((k + 1) / kTaSegs) & 1, abort_flag, a.status, 834, k + 1);
+      ok = bar256_and(ok);                                                     // both accumulators, s_x and the segment are free again
+      if (threadIdx.x == 0) mbar_arrive(&g_empty[k % kTaSegs]);
     }
   }
   pdl_trigger();                       // a long kernel: its dependents are released at its end
@@ -543,7 +617,7 @@ tree_join_kernel(const TreeAttnArgs a) {
   if (of.z <= 0) return;
   TaSeq q;
   q.load(a, of.x);
-  const int G = a.hq / a.hkv, tpt = 128 / G, pairs = q.items / a.hkv;
+  const int G = a.hq / a.hkv, tpt = 128 / a.fold / G, pairs = q.items / a.hkv;
   const int kvh = of.y / pairs, tile = (of.y - kvh * pairs) * a.pair;
   const int lane = threadIdx.x & 31;
   const int per_block = a.pair * 128 / (int)gridDim.y;
@@ -576,9 +650,9 @@ tree_join_kernel(const TreeAttnArgs a) {
   }
 }
 
-template <int DK, int DV>
+template <int DK, int DV, int FOLD>
 static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const void* v_cache, TreeAttnArgs a, int grid, cudaStream_t stream) {
-  const int G = a.hq / a.hkv, tpt = 128 / G;
+  const int G = a.hq / a.hkv, tpt = 128 / FOLD / G;
   CUtensorMap tmQ, tmK, tmV;
   {
     uint64_t dims[3] = {DK, (uint64_t)a.hq, (uint64_t)a.total_tokens};
@@ -597,10 +671,10 @@ static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
   if (!attr[dev & 63]) {
-    GB_CUDA_OK(cudaFuncSetAttribute(tree_attn_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTaSmem));
+    GB_CUDA_OK(cudaFuncSetAttribute(tree_attn_kernel<DK, DV, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTaSmem));
     attr[dev & 63] = true;
   }
-  launch_k(tree_attn_kernel<DK, DV>, grid, kTaThreads, kTaSmem, stream, tmQ, tmK, tmV, a);
+  launch_k(tree_attn_kernel<DK, DV, FOLD>, grid, kTaThreads, kTaSmem, stream, tmQ, tmK, tmV, a);
   GB_CUDA_OK(cudaGetLastError());
   if (!a.whole) {
     launch_k(tree_join_kernel<DV>, dim3(grid, 4 * a.pair), 256, 0, stream, a);
@@ -613,9 +687,13 @@ static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const
 
 using namespace gb;
 
-// Blocks of the launch, and whether the items stay whole: bounds by what the host knows (at most max_pages pages and max_nodes nodes a sequence).
-static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int* pair, int* whole) {
-  const int tpt = 128 / (hq / hkv), tiles = (max_nodes + tpt - 1) / tpt;
+// Blocks of the launch, how the rows lie in a tile, and whether the items stay whole: bounds by what the host knows (at most max_pages pages and max_nodes nodes a
+// sequence).
+static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int* pair, int* fold, int* whole) {
+  const int G = hq / hkv;
+  const long rows = (long)max_nodes * G;
+  *fold = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+  const int tpt = 128 / *fold / G, tiles = (max_nodes + tpt - 1) / tpt;
   *pair = tiles > 1 ? 2 : 1;
   const long blocks = std::max(1l, ((long)max_pages * page_size + 127) / 128), items = (long)n_seqs * hkv * ((tiles + *pair - 1) / *pair);
   *whole = blocks <= 2;
@@ -624,9 +702,9 @@ static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_node
 
 // Floats of the workspace that gb_tree_attn wants.
 GB_API int gb_tree_attn_workspace(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int dv) {
-  int pair, whole;
-  const long grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &pair, &whole);
-  return whole ? 4 : (int)(grid * 4 + 2 * grid * pair * 128 * (dv + 1));          // (at most 148 * 2 * 2 * 128 rows)
+  int pair, fold, whole;
+  const long grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &pair, &fold, &whole);
+  return whole ? 4 : (int)((grid + 1) / 2 * 8 + 2 * grid * pair * 128 * (dv + 1));          // (at most 148 * 2 * 2 * 128 rows)
 }
 
 GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const void* v_cache, void* out, float* workspace, const int* cu_q, const int* kv_len,
@@ -640,15 +718,22 @@ GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const voi
   if (window > 0 && positions == nullptr) return fail("tree_attn: a window needs the nodes' positions%s");
   TreeAttnArgs a;
   memset(&a, 0, sizeof(a));
-  const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &a.pair, &a.whole);
+  const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &a.pair, &a.fold, &a.whole);
   a.cu_q = cu_q; a.kv_len = kv_len; a.block_table = block_table; a.mask = (const unsigned long long*)mask; a.positions = positions; a.n_seqs = n_seqs;
   a.max_pages = max_pages; a.page_size = page_size; a.words = words; a.window = window; a.hq = hq; a.hkv = hkv; a.total_tokens = tokens;
   a.num_slots = num_slots; a.out = (__nv_bfloat16*)out; a.v_cache = (const __nv_bfloat16*)v_cache; a.status = (KernelStatus*)status;
   if (!a.whole) {
     a.part_of = (int4*)workspace;
-    a.part_o = workspace + grid * 4;
+    a.part_o = workspace + (grid + 1) / 2 * 8;                     // on a 32-byte boundary
     a.part_lse = a.part_o + 2l * grid * a.pair * 128 * dv;
   }
-  if (dk == 64) return dv == 64 ? tree_attn_launch<64, 64>(q, q_ts, k_cache, v_cache, a, grid, stream) : tree_attn_launch<64, 128>(q, q_ts, k_cache, v_cache, a, grid, stream);
-  return dv == 64 ? tree_attn_launch<128, 64>(q, q_ts, k_cache, v_cache, a, grid, stream) : tree_attn_launch<128, 128>(q, q_ts, k_cache, v_cache, a, grid, stream);
+#define GB_TREE(K, V, F) if (dk == K && dv == V && a.fold == F) return tree_attn_launch<K, V, F>(q, q_ts, k_cache, v_cache, a, grid, stream);
+#define GB_TREE_FOLDS(K, V) GB_TREE(K, V, 1) GB_TREE(K, V, 2) GB_TREE(K, V, 4)
+  GB_TREE_FOLDS(64, 64)
+  GB_TREE_FOLDS(64, 128)
+  GB_TREE_FOLDS(128, 64)
+  GB_TREE_FOLDS(128, 128)
+#undef GB_TREE_FOLDS
+#undef GB_TREE
+  return fail("tree_attn: no such form%s");
 }

@@ -63,6 +63,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         out = torch.empty(t, hq, dv, dtype=q.dtype, device=dev)
     elif out.shape != (t, hq, dv) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out: a contiguous tensor [{t}, {hq}, {dv}] of the queries' type is needed")
+    elif out.data_ptr() % 32:
+        raise ValueError("out: a 32-byte boundary is needed")
     if dev.type != "cuda":
         return tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window, positions, out)
     if t == 0 or b == 0:
