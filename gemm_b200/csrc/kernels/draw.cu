@@ -3,16 +3,18 @@
 //   w_i = 2^((x_i - max x) log2(e) / T).  In the order (x descending, id ascending): the first top_k ids; of these the ids that have less than top_p of the
 //   mass in front of them; of these the ids with w_i >= min_p.  The draw is the first id, in id order, at which the mass so far exceeds u times the kept mass.
 //
-// All three filters cut that order at one place, so what is kept is {key > tau} and the first m ids with key = tau.  No sort: tau comes from a histogram over
-// 1/16-wide steps below the maximum and a radix search over the keys of the step that holds the cut.
+// All three filters cut that order at one place, so what is kept is {key > tau} and the first m ids with key = tau.  No sort: tau comes from radix searches.
 //
 // Masses are whole numbers: w_i is rounded to a multiple of 2^-44 (the rounding moves a border of the draw by 2^-45 of the largest weight; 2^18 of them stay
 // below 2^63).  Sums are then exact in any order: the atomics of the histograms, the split over blocks and the order of the warps change nothing, and the
 // draw agrees with one in 64-bit floats except where u falls within some 1e-12 of a border (32-bit sums over a vocabulary: a row in a thousand).
 // 2^t: table of 2^(j/32) and a polynomial of degree 5 for the rest (P. T. P. Tang, "Table-driven implementation of the exponential function", 1989), in 64-bit floats.
 //
-// A cluster of up to eight blocks holds a row in its shared memory (bulk copies), so that HBM is read once whatever the number of passes; block totals and
-// histograms are exchanged through distributed shared memory, and every block reduces them for itself: one cluster barrier per step.
+// A cluster of up to eight blocks holds a row in its shared memory (bulk copies), so that HBM is read once whatever the number of passes.  Every instruction
+// per logit and every step of the whole cluster counts, so a row with a top-k or a top-p is pruned first: the k'-th largest of 4096 maxima of small groups of logits
+// is a lower bound of the k'-th largest logit, and the logits above it (few more than k') go to the first block, which finishes alone while the
+// others make room for the next row.  Rows that this does not settle (more than kDrPrune to keep, a flat top-p, equal logits), and rows without a limit, take the
+// cluster's path: histograms over 1/16-wide steps below the maximum, exchanged through distributed shared memory.
 #include "sm100.cuh"
 #include "host_common.h"
 #include <float.h>
@@ -23,6 +25,9 @@ namespace gb {
 constexpr int kDrThreads = 512, kDrWarps = 16;
 constexpr int kDrBins = 512;               // steps of 1/16 below the maximum; the last one takes all that lies further down
 constexpr int kDrList = 256;               // candidates a warp lists
+constexpr int kDrCand = 2048;              // candidates of a row in the first block
+constexpr int kDrGroups = 4096;            // groups of logits whose maxima prune a row
+constexpr int kDrPrune = 1000;             // k' at most: a quarter of the groups, so that few logits beyond the k'-th lie above the bound
 constexpr int kDrMass = 44;                // fraction bits of a weight
 
 struct DrawArgs {
@@ -53,7 +58,15 @@ struct DrawShared {
   int list_n[kDrWarps];
   uint64_t bar;
   int abort_flag;
-  unsigned short list[kDrWarps][kDrList];
+  float bound;                             // written by the first block into all
+  int cand_n[8];                           // of every block, written by it into all
+  unsigned long long cand_mass[8], cand_all[8];      // mass of its candidates, and of all its logits
+  int cand_own;
+  union {
+    float group[kDrGroups];                // first block: maxima of the groups
+    uint2 cand[kDrCand];                   // first block: key and id; a share of the places for every block
+    unsigned short list[kDrWarps][kDrList];
+  };
 };
 
 __device__ __forceinline__ uint32_t dr_mapa(uint32_t addr, int cta) {
@@ -70,6 +83,10 @@ __device__ __forceinline__ unsigned long long dr_peer64(const void* p, int cta) 
   unsigned long long v;
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
   return v;
+}
+__device__ __forceinline__ void dr_put32(void* p, int cta, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" :: "r"(dr_mapa(smem_u32(p), cta)), "r"(v) : "memory"); }
+__device__ __forceinline__ void dr_put64(void* p, int cta, unsigned long long v) {
+  asm volatile("st.shared::cluster.b64 [%0], %1;" :: "r"(dr_mapa(smem_u32(p), cta)), "l"(v) : "memory");
 }
 __device__ __forceinline__ void dr_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -88,8 +105,9 @@ template <> struct DrawKey<__nv_bfloat16> {
 };
 
 // 2^t in units of 2^-44, for t <= 0; t = -46 and below (and NaN): 0.
-__device__ __forceinline__ unsigned long long dr_weight(double t, const double* table) {
-  if (!(t > -46.0)) return 0;
+template <typename F>
+__device__ __forceinline__ unsigned long long dr_weight(double t, F entry) {
+  if (!(t > -46.0)) t = -47.0;                                    // (rounds to 0)
   constexpr double kRound = 6755399441055744.0;                   // 1.5 * 2^52: the sum's low bits are the rounded number
   const double m = fma(t, 32.0, kRound);
   const int k = __double2loint(m);
@@ -98,7 +116,7 @@ __device__ __forceinline__ unsigned long long dr_weight(double t, const double* 
   constexpr double c1 = 0.69314718055994531, c2 = 0.24022650695910072, c3 = 0.05550410866482158, c4 = 0.009618129107628477, c5 = 0.0013333558146428443;
   double p = fma(r, c5, c4);
   p = fma(r, p, c3); p = fma(r, p, c2); p = fma(r, p, c1); p = fma(r, p, 1.0);
-  p *= table[k & 31];
+  p *= entry(k & 31);
   p = __hiloint2double(__double2hiint(p) + ((k >> 5) + kDrMass) * 1048576, __double2loint(p));     // times 2^(k >> 5), in units
   return (unsigned long long)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;    // 2^52: rounded to a whole number
 }
@@ -155,9 +173,18 @@ draw_kernel(const DrawArgs a) {
   if (body > 0) mbar_wait(&s.bar, 0, (volatile int*)&s.abort_flag, a.status, 700, row);
   __syncthreads();
 
-  // ---- maximum
+  // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces
   float mx = -INFINITY;
-  for (int i = tid; i < n; i += kDrThreads) mx = fmaxf(mx, Key::value(x[i]));
+  {
+    const int pieces = kDrGroups / kDrThreads / C;
+    for (int p = 0; p < pieces; ++p) {
+      float gm = -INFINITY;
+#pragma unroll 4
+      for (int i = p * kDrThreads + tid; i < n; i += pieces * kDrThreads) gm = fmaxf(gm, Key::value(x[i]));
+      dr_put32(&s.group[(rank * pieces + p) * kDrThreads + tid], 0, __float_as_uint(gm));
+      mx = fmaxf(mx, gm);
+    }
+  }
   mx = warp_max(mx);
   if (lane == 0) s.red[warp] = mx;
   if (tid == 0) s.first_max = 0x7fffffff;
@@ -173,24 +200,230 @@ draw_kernel(const DrawArgs a) {
   if (tid == 0) s.max_x = mx;
   __syncthreads();
   dr_cluster_sync();
-  for (int c = 0; c < C; ++c) mx = fmaxf(mx, __uint_as_float(dr_peer32(&s.max_x, c)));
+  mx = warp_max(lane < C ? __uint_as_float(dr_peer32(&s.max_x, lane)) : -INFINITY);
   if (greedy || mx == -INFINITY) {
     // the lowest id of the maximum; a row without any logit to draw from answers 0, as the arg-max does
-    if (rank == 0 && tid == 0) {
+    if (rank == 0 && warp == 0) {
       int at = 0x7fffffff;
-      if (mx > -INFINITY)
-        for (int c = 0; c < C; ++c) if (__uint_as_float(dr_peer32(&s.max_x, c)) == mx) at = min(at, (int)dr_peer32(&s.first_max, c));
-      a.out[row] = at == 0x7fffffff ? 0 : at;
-      if (a.logprob != nullptr) a.logprob[row] = mx > -INFINITY ? 0.f : -INFINITY;
+      if (mx > -INFINITY && lane < C && __uint_as_float(dr_peer32(&s.max_x, lane)) == mx) at = (int)dr_peer32(&s.first_max, lane);
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0) {
+        a.out[row] = at == 0x7fffffff ? 0 : at;
+        if (a.logprob != nullptr) a.logprob[row] = mx > -INFINITY ? 0.f : -INFINITY;
+      }
     }
     dr_cluster_sync();                                             // nobody leaves while another one reads its shared memory
     return;
   }
 
   const double scale = 1.4426950408889634 / (double)temp, dmx = (double)mx;
-  auto weight = [&](float v) -> unsigned long long { return v == mx ? 1ull << kDrMass : dr_weight(((double)v - dmx) * scale, s.table); };
+  auto weight = [&](float v) -> unsigned long long {
+    return v == mx ? 1ull << kDrMass : dr_weight(((double)v - dmx) * scale, [&](int j) { return s.table[j]; });
+  };
+  // the same where the whole warp asks: the table lies in the lanes (a shuffle has no bank conflicts)
+  const double lane_entry = s.table[lane];
+  auto weight_all = [&](float v) -> unsigned long long {
+    const unsigned long long w = dr_weight(((double)v - dmx) * scale, [&](int j) { return __shfl_sync(0xffffffffu, lane_entry, j); });
+    return v == mx ? 1ull << kDrMass : w;
+  };
   auto bin_of = [&](float v) -> int { return min(kDrBins - 1, (int)fminf((mx - v) * 16.0f, 1e6f)); };       // monotone in v (mx = inf: all in the last bin)
-  // a warp owns a run of the block's ids
+  const unsigned long long min_w = min_p > 0.f ? (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << kDrMass)) : 0ull;
+  auto value_of = [&](unsigned key) -> float {                     // the logit of a key
+    if (sizeof(T) == 2) key = (key << 16) | ((key & 0x8000u) ? 0u : 0xffffu);
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+  };
+  auto logprob_of = [&](float v, unsigned long long all) -> float {
+    return (float)((v == mx ? 0.0 : ((double)v - dmx) * scale) * 0.69314718055994531 - log((double)all * (1.0 / (double)(1ull << kDrMass))));
+  };
+  auto spot_of = [&](unsigned long long all) -> unsigned long long {         // u below 0 or NaN: the first id; 1 and above: the last
+    const double spot = (double)u * (double)all;
+    return spot > 0.0 ? min(spot >= (double)all ? all - 1 : (unsigned long long)spot, all - 1) : 0ull;
+  };
+  auto top_p_target = [&](unsigned long long all) -> unsigned long long {    // kept: while less than this lies in front
+    const double goal = ceil((double)top_p * (double)all);
+    return goal >= (double)all ? all : goal < 1.0 ? 1ull : (unsigned long long)goal;
+  };
+
+  // ---- pruned rows
+  const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f;
+  if (has_k ? top_k <= kDrPrune : has_p) {
+    const int want = has_k ? top_k : kDrPrune;
+    if (rank == 0) {
+      s.count[0][tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kDrGroups / kDrThreads; ++i) {
+        const float v = s.group[i * kDrThreads + tid];
+        if (v > mx - kDrBins / 16.0f) atomicAdd(&s.count[0][bin_of(v)], 1u);
+      }
+      __syncthreads();
+      dr_find(s.count[0][tid], want, s);
+      // at least `want` logits lie in the bin and above; fewer in reach: all of them count
+      const float bound = s.found_at >= 0 && s.found_at < kDrBins - 1 ? fmaxf(mx - (s.found_at + 1) * 0.0625f - fmaf(fabsf(mx), 2.5e-7f, 1e-5f), -FLT_MAX) : -FLT_MAX;
+      if (tid < C) dr_put32(&s.bound, tid, __float_as_uint(bound));
+    }
+    if (tid == 0) s.cand_own = 0;
+    __syncthreads();
+    dr_cluster_sync();
+    const float bound = s.bound;
+    {
+      const int cap = kDrCand / C;
+      unsigned long long mass = 0, all = 0;
+      auto take = [&](float v, int i) {
+        const int at = atomicAdd(&s.cand_own, 1);
+        if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i) << 32 | Key::of(v));
+      };
+      if (has_k) {
+#pragma unroll 4
+        for (int i = tid; i < n; i += kDrThreads) { const float v = Key::value(x[i]); if (v >= bound) take(v, i); }
+      } else {
+        for (int b = warp * 32; b < n; b += kDrThreads) {
+          const int i = b + lane;
+          const float v = i < n ? Key::value(x[i]) : -INFINITY;
+          const unsigned long long w = weight_all(v);
+          all += w;
+          if (v >= bound) { mass += w; take(v, i); }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { mass += __shfl_xor_sync(0xffffffffu, mass, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
+        if (lane == 0) { s.warp_mass[warp] = mass; s.scan[warp] = all; }
+        __syncthreads();
+        if (tid < C) {
+          mass = 0; all = 0;
+          for (int w = 0; w < kDrWarps; ++w) { mass += s.warp_mass[w]; all += s.scan[w]; }
+          dr_put64(&s.cand_mass[rank], tid, mass);
+          dr_put64(&s.cand_all[rank], tid, all);
+        }
+      }
+      __syncthreads();
+      if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
+      dr_cluster_sync();
+      bool settled = true;
+      int found = 0;
+      unsigned long long c_mass = 0, c_all = 0;
+      for (int c = 0; c < C; ++c) {
+        found += s.cand_n[c];
+        settled &= s.cand_n[c] <= cap;
+        if (!has_k) { c_mass += s.cand_mass[c]; c_all += s.cand_all[c]; }
+      }
+      if (!has_k) settled &= c_mass >= top_p_target(c_all);
+      if (settled) {
+        if (rank != 0) return;                                     // (nobody reads this block's shared memory any more)
+        // ---- the first block, alone: four candidates a thread
+        constexpr int kOwn = kDrCand / kDrThreads;
+        unsigned key[kOwn], id[kOwn];
+        unsigned long long w[kOwn];
+        unsigned low = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) {
+          const int at = k * kDrThreads + tid;
+          const bool in = at % cap < s.cand_n[at / cap];
+          const uint2 e = in ? s.cand[at] : make_uint2(0u, 0u);
+          key[k] = e.x; id[k] = e.y;                               // key 0: no candidate
+          w[k] = in ? weight(value_of(e.x)) : 0ull;
+          if (in) low = min(low, e.x);
+        }
+        low = __reduce_min_sync(0xffffffffu, low);
+        if (tid == 0) s.first_max = -1;
+        __syncthreads();
+        if (lane == 0) atomicMin((unsigned*)&s.first_max, low);
+        __syncthreads();
+        low = (unsigned)s.first_max;
+        // Searches the numbers of(k) in [base, base + range] for the one at which the running sum of val(k), from the top down (or from the bottom up), reaches `target`;
+        // `before`: the sum in front of it.
+        auto search = [&](unsigned base, unsigned range, bool up, bool mass, unsigned long long target, unsigned long long& before, auto of, auto val) -> unsigned {
+          unsigned prefix = 0;
+          before = 0;
+          for (int bits = 32 - __clz(range); bits > 0;) {
+            const int shift = max(0, bits - 9);
+            s.count[0][tid] = 0;
+            if (mass) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kOwn; ++k) {
+              const unsigned long long v = val(k);
+              const unsigned off = min(of(k) - base, range);
+              if (v == 0 || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
+              const int d = (off >> shift) & 511;
+              if (!mass) atomicAdd(&s.count[0][d], 1u);
+              else {
+                const unsigned l = (unsigned)v, old = atomicAdd(&s.lo[0][d], l);
+                const unsigned h = (unsigned)(v >> 32) + (old + l < old ? 1u : 0u);
+                if (h != 0) atomicAdd(&s.hi[0][d], h);
+              }
+            }
+            __syncthreads();
+            const int d = up ? tid : 511 - tid;
+            const unsigned long long v = mass ? ((unsigned long long)s.hi[0][d] << 32) + s.lo[0][d] : s.count[0][d];
+            dr_find(v, target - before, s);
+            const int hit = s.found_at < 0 ? 0 : s.found_at;
+            prefix = prefix << (bits - shift) | (unsigned)(up ? hit : 511 - hit);
+            before += s.found_before;
+            bits = shift;
+            __syncthreads();
+          }
+          return base + prefix;
+        };
+        auto sum = [&](unsigned long long v) -> unsigned long long {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == 0) s.scan[warp] = v;
+          __syncthreads();
+          v = 0;
+          for (int x = 0; x < kDrWarps; ++x) v += s.scan[x];
+          __syncthreads();
+          return v;
+        };
+        const unsigned top = Key::of(mx);
+        unsigned tau = 0;                                          // kept: key > tau, and the first `ties` ids of key tau
+        unsigned long long ties = 0, before;
+        auto key_of = [&](int k) { return key[k]; };
+        auto id_of = [&](int k) { return id[k]; };
+        const bool cut_k = has_k && found > top_k;
+        if (cut_k) {
+          tau = search(low, top - low, false, false, (unsigned long long)top_k, before, key_of, [&](int k) -> unsigned long long { return key[k] != 0; });
+          ties = (unsigned long long)top_k - before;
+        }
+        // of equal keys at the cut the first ids stay; the others are struck out
+        auto strike = [&]() {
+          unsigned long long n_tie = 0;
+#pragma unroll
+          for (int k = 0; k < kOwn; ++k) n_tie += key[k] != 0 && key[k] == tau;
+          n_tie = sum(n_tie);
+          unsigned last = 0xffffffffu;
+          if (n_tie > ties && ties > 0) last = search(0, (unsigned)a.vocab - 1, true, false, ties, before, id_of, [&](int k) -> unsigned long long { return key[k] != 0 && key[k] == tau; });
+#pragma unroll
+          for (int k = 0; k < kOwn; ++k) if (key[k] < tau || (key[k] == tau && (ties == 0 || id[k] > last))) { key[k] = 0; w[k] = 0; }
+        };
+        if (cut_k) strike();
+        if (has_p) {
+          unsigned long long m = 0;
+#pragma unroll
+          for (int k = 0; k < kOwn; ++k) m += w[k];
+          m = sum(m);
+          const unsigned long long target = top_p_target(has_k ? m : c_all);
+          tau = search(low, top - low, false, true, target, before, key_of, [&](int k) -> unsigned long long { return w[k]; });
+          const unsigned long long wt = weight(value_of(tau));
+          ties = wt > 0 ? (target - before + wt - 1) / wt : 0;
+          strike();
+        }
+        unsigned long long m = 0;
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) { if (w[k] < min_w) w[k] = 0; m += w[k]; }
+        m = sum(m);
+        const unsigned token = search(0, (unsigned)a.vocab - 1, true, true, spot_of(m) + 1, before, id_of, [&](int k) -> unsigned long long { return w[k]; });
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k)
+          if (w[k] != 0 && id[k] == token) {
+            a.out[row] = (int)token;
+            if (a.logprob != nullptr) a.logprob[row] = logprob_of(value_of(key[k]), m);
+          }
+        return;
+      }
+    }
+  }
+
+  // ---- the cluster's path.  A warp owns a run of the block's ids
   const int run = (n + kDrWarps - 1) / kDrWarps, r0 = min(n, warp * run), rn = min(n, r0 + run) - r0;
   bool listed = false;
   int list_n = 0;
@@ -293,11 +526,7 @@ draw_kernel(const DrawArgs a) {
   // ---- top-k
   unsigned long long tie_mass = 0;                                 // of the ids kept at tau
   int tau_bin = -1;
-  auto value_of = [&](unsigned key) -> float {                     // the logit of a key
-    if (sizeof(T) == 2) key = (key << 16) | ((key & 0x8000u) ? 0u : 0xffffu);
-    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-  };
-  if (top_k > 0 && top_k < a.vocab) {
+  if (has_k) {
     clear(false);
     each([&](float e, bool in) { put(in ? bin_of(e) : 0, in); });
     __syncthreads();
@@ -321,9 +550,9 @@ draw_kernel(const DrawArgs a) {
     ++step;
   }
   // ---- top-p of what is left
-  if (top_p < 1.f) {
+  if (has_p) {
     clear(true);
-    each([&](float e, bool in) { if (in && Key::of(e) > tau) { const unsigned long long w = weight(e); if (w) put_mass(bin_of(e), w); } });
+    each([&](float e, bool in) { const unsigned long long w = weight_all(e); if (in && Key::of(e) > tau && w) put_mass(bin_of(e), w); });
     __syncthreads();
     dr_cluster_sync();
     unsigned long long all = gather(tid, true);
@@ -334,8 +563,7 @@ draw_kernel(const DrawArgs a) {
     all = tie_mass;
     for (int w = 0; w < kDrWarps; ++w) all += s.warp_mass[w];
     __syncthreads();
-    const double goal = ceil((double)top_p * (double)all);
-    const unsigned long long target = goal >= (double)all ? all : goal < 1.0 ? 1ull : (unsigned long long)goal;
+    const unsigned long long target = top_p_target(all);
     const unsigned old_tau = tau;
     const unsigned long long old_ties = ties;
     const unsigned long long above = cut(true, target, old_tau, tie_mass, tau_bin);
@@ -345,15 +573,13 @@ draw_kernel(const DrawArgs a) {
     ++step;
   }
   // ---- the draw, in id order: blocks, warps, sixteenths of a warp's ids, ids
-  const unsigned long long min_w = min_p > 0.f ? (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << kDrMass)) : 0ull;
   unsigned long long wt = ties > 0 ? weight(value_of(tau)) : 0;
   if (wt < min_w) wt = 0;
-  auto kept = [&](float e, bool in, bool& tie) -> unsigned long long {
+  auto kept = [&](float e, bool in, bool& tie) -> unsigned long long {       // (the whole warp)
     const unsigned k = Key::of(e);
     tie = in && k == tau;
-    if (!in || k <= tau) return 0;
-    const unsigned long long w = weight(e);
-    return w >= min_w ? w : 0;
+    const unsigned long long w = weight_all(e);
+    return in && k > tau && w >= min_w ? w : 0;
   };
   unsigned long long mass = 0;
   int n_tie = 0;
@@ -379,9 +605,7 @@ draw_kernel(const DrawArgs a) {
     all += m; all_ties += t;
   }
   all += min(all_ties, ties) * wt;
-  const double spot = (double)u * (double)all;
-  unsigned long long r = spot > 0.0 ? (spot >= (double)all ? all - 1 : (unsigned long long)spot) : 0ull;        // (u below 0 or NaN: 0; 1 and above: the last id)
-  if (r >= all) r = all - 1;
+  const unsigned long long r = spot_of(all);
   // mass in front of a place with m above tau and t ties in front of it
   auto front = [&](unsigned long long m, unsigned long long t) { return m + min(t, ties) * wt; };
   const bool here = front(gt, nt) <= r && r < front(gt + s.total[0], nt + (unsigned)s.ties);
@@ -396,8 +620,9 @@ draw_kernel(const DrawArgs a) {
     auto at_of = [&](int i) { return w0 + (wn >= 0 ? (int)s.list[w][i] : i); };
     __syncthreads();                                               // warp_mass and warp_ties are used again
     mass = 0; n_tie = 0;
-    for (int i = warp * piece + lane; i < min(m, (warp + 1) * piece); i += 32) {
-      const float e = Key::value(x[at_of(i)]);
+    for (int b = warp * piece; b < min(m, (warp + 1) * piece); b += 32) {
+      const int i = b + lane;
+      const float e = i < m ? Key::value(x[at_of(i)]) : -INFINITY;           // (a piece is a multiple of 32)
       bool tie;
       mass += kept(e, e > -INFINITY, tie);
       n_tie += tie;
@@ -428,7 +653,7 @@ draw_kernel(const DrawArgs a) {
           if (lane == __ffs(hit) - 1) {
             a.out[row] = i0 + at_of(i);
             if (a.logprob != nullptr)
-              a.logprob[row] = (float)((e == mx ? 0.0 : ((double)e - dmx) * scale) * 0.69314718055994531 - log((double)all * (1.0 / (double)(1ull << kDrMass))));
+              a.logprob[row] = logprob_of(e, all);
           }
           done = true;
         }
@@ -442,13 +667,13 @@ draw_kernel(const DrawArgs a) {
 
 template <typename T>
 static int draw_launch(DrawArgs a, cudaStream_t stream) {
-  // Blocks per row: enough that a block's share of the row fits shared memory beside a second block's.
+  // Blocks per row.  A block's passes cost less than its share of the cluster's steps below some 20,000 logits; few rows take as many blocks as there is room for.  Two blocks share an SM where 90 KB hold a share.
   int c = 1;
-  while (c < 8 && ((long)a.vocab > (long)c * 4096 || (long)((a.vocab + c - 1) / c) * (long)sizeof(T) > 90000)) c *= 2;
+  while (c < 8 && (a.vocab > c * 20480 || (long)((a.vocab + c - 1) / c) * (long)sizeof(T) > 90000 || (a.vocab > c * 4096 && a.rows * c * 2 <= sm_count()))) c *= 2;
   a.ctas = c;
   a.per = ((a.vocab + c - 1) / c + 15) / 16 * 16;
   const size_t smem = (size_t)a.per * sizeof(T) + 32;
-  if (smem > 200 * 1024) return fail("draw: the vocabulary does not fit the shared memory of eight blocks%s");
+  if (smem > 202000) return fail("draw: the vocabulary does not fit the shared memory of eight blocks%s");
   static size_t attr[64];
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
