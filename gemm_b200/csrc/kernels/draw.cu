@@ -11,10 +11,13 @@
 // 2^t: table of 2^(j/32) and a polynomial of degree 5 for the rest (P. T. P. Tang, "Table-driven implementation of the exponential function", 1989), in 64-bit floats.
 //
 // A cluster of up to eight blocks holds a row in its shared memory (bulk copies), so that HBM is read once whatever the number of passes.  Every instruction
-// per logit and every step of the whole cluster counts, so a row with a top-k or a top-p is pruned first: the k'-th largest of 4096 maxima of small groups of logits
-// is a lower bound of the k'-th largest logit, and the logits above it (few more than k') go to the first block, which finishes alone while the
-// others make room for the next row.  Rows that this does not settle (more than kDrPrune to keep, a flat top-p, equal logits), and rows without a limit, take the
-// cluster's path: histograms over 1/16-wide steps below the maximum, exchanged through distributed shared memory.
+// per logit and every step of the whole cluster counts, so most of a row's work is left to one block while the others make room for the next row:
+//   top-k         the k-th largest of 4096 maxima of small groups of logits is a lower bound of the k-th largest logit; the logits above it, few more than k,
+//                 go to the first block, which finishes alone: by comparing all pairs, or by radix searches if they are many;
+//   top-p alone   one pass for all weights and their histogram; then the candidates go to the first block, or, if they are too many, those of the cut's step;
+//   neither       one pass for the blocks' masses, and a second one in the block in which the draw falls.
+// Rows that this does not settle (a large top-k, equal logits) take the cluster's path: histograms over 1/16-wide steps below the maximum and over the keys of
+// the step that holds the cut, exchanged through distributed shared memory.
 #include "sm100.cuh"
 #include "host_common.h"
 #include <float.h>
@@ -26,6 +29,7 @@ constexpr int kDrThreads = 512, kDrWarps = 16;
 constexpr int kDrBins = 512;               // steps of 1/16 below the maximum; the last one takes all that lies further down
 constexpr int kDrList = 256;               // candidates a warp lists
 constexpr int kDrCand = 2048;              // candidates of a row in the first block
+constexpr int kDrPairs = 256;              // candidates that are compared with one another
 constexpr int kDrGroups = 4096;            // groups of logits whose maxima prune a row
 constexpr int kDrPrune = 1000;             // k' at most: a quarter of the groups, so that few logits beyond the k'-th lie above the bound
 constexpr int kDrMass = 44;                // fraction bits of a weight
@@ -41,7 +45,7 @@ struct DrawArgs {
   KernelStatus* status;
 };
 
-struct DrawShared {
+struct alignas(16) DrawShared {
   unsigned count[2][kDrBins];              // histogram, by step parity
   unsigned lo[2][kDrBins], hi[2][kDrBins]; // its masses in two words
   double table[32];
@@ -50,8 +54,8 @@ struct DrawShared {
   unsigned long long scan[kDrWarps];
   unsigned long long found_before;
   int found_at;
-  float red[kDrWarps];
-  float max_x;                             // this block's, read by the others
+  float red[2 * kDrWarps];
+  float max_x, low_x;                      // this block's maximum and its lowest group's, read by the others
   int first_max;
   unsigned long long total[2];             // this block's kept mass, read by the others
   int ties;
@@ -60,8 +64,10 @@ struct DrawShared {
   int abort_flag;
   float bound;                             // written by the first block into all
   int cand_n[8];                           // of every block, written by it into all
-  unsigned long long cand_mass[8], cand_all[8];      // mass of its candidates, and of all its logits
+  int cand_in[8];
   int cand_own;
+  unsigned tau, last;                      // written by the first block into all: the cut
+  unsigned long long block_mass[8];        // kept mass of every block, written by it into all
   union {
     float group[kDrGroups];                // first block: maxima of the groups
     uint2 cand[kDrCand];                   // first block: key and id; a share of the places for every block
@@ -130,9 +136,10 @@ __device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long
   if (lane == 31) s.scan[warp] = incl;
   if (threadIdx.x == 0) { s.found_at = -1; s.found_before = 0; }
   __syncthreads();
-  unsigned long long front = 0;
-  for (int w = 0; w < warp; ++w) front += s.scan[w];
-  incl += front;
+  unsigned long long front = lane < warp ? s.scan[lane] : 0ull;    // (16 warps: the lanes fetch, and add up)
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) front += __shfl_xor_sync(0xffffffffu, front, o);
+  incl += __shfl_sync(0xffffffffu, front, 0);
   if (v != 0 && incl - v < target && target <= incl) { s.found_at = threadIdx.x; s.found_before = incl - v; }
   __syncthreads();
 }
@@ -173,23 +180,50 @@ draw_kernel(const DrawArgs a) {
   if (body > 0) mbar_wait(&s.bar, 0, (volatile int*)&s.abort_flag, a.status, 700, row);
   __syncthreads();
 
-  // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces
-  float mx = -INFINITY;
+  // f(value, index in the block) for the thread's share of the block's logits: 16 bytes at a time, and the ragged ends.  Step: threads between two of a thread's turns
+  const int nv = body / kVec;
+  auto vec_at = [&](int j, float* v) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(x + head + j * kVec);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = sizeof(T) == 4 ? __uint_as_float(w[e & 3]) : __uint_as_float(e & 1 ? w[(e >> 1) & 3] & 0xffff0000u : w[(e >> 1) & 3] << 16);
+  };
+  auto ends = [&](auto f) {                                        // head and tail: a thread each
+    if (tid < head) f(Key::value(x[tid]), tid);
+    if (tid < n - head - body) f(Key::value(x[head + body + tid]), head + body + tid);
+  };
+
+  // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces.  (fmaxf passes over NaN.)
+  float mx = -INFINITY, low = INFINITY;
   {
     const int pieces = kDrGroups / kDrThreads / C;
+    const bool fine = nv < pieces * kDrThreads;                    // few logits: groups of single ones rather than empty groups
     for (int p = 0; p < pieces; ++p) {
       float gm = -INFINITY;
-#pragma unroll 4
-      for (int i = p * kDrThreads + tid; i < n; i += pieces * kDrThreads) gm = fmaxf(gm, Key::value(x[i]));
+      if (fine) {
+        for (int i = p * kDrThreads + tid; i < n; i += pieces * kDrThreads) gm = fmaxf(gm, Key::value(x[i]));
+      } else {
+        if (p == 0) ends([&](float v, int) { gm = fmaxf(gm, v); });
+#pragma unroll 2
+        for (int j = p * kDrThreads + tid; j < nv; j += pieces * kDrThreads) {
+          float v[kVec];
+          vec_at(j, v);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) gm = fmaxf(gm, v[e]);
+        }
+      }
       dr_put32(&s.group[(rank * pieces + p) * kDrThreads + tid], 0, __float_as_uint(gm));
       mx = fmaxf(mx, gm);
+      if (gm > -INFINITY) low = fminf(low, gm);
     }
   }
   mx = warp_max(mx);
-  if (lane == 0) s.red[warp] = mx;
+  low = -warp_max(-low);
+  if (lane == 0) { s.red[warp] = mx; s.red[kDrWarps + warp] = -low; }
   if (tid == 0) s.first_max = 0x7fffffff;
   __syncthreads();
   mx = warp_max(s.red[lane & (kDrWarps - 1)]);
+  low = -warp_max(s.red[kDrWarps + (lane & (kDrWarps - 1))]);
   const bool greedy = !(temp > 0.f);
   if (greedy) {
     int at = 0x7fffffff;
@@ -197,9 +231,10 @@ draw_kernel(const DrawArgs a) {
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0 && at != 0x7fffffff) atomicMin(&s.first_max, at);
   }
-  if (tid == 0) s.max_x = mx;
+  if (tid == 0) { s.max_x = mx; s.low_x = low; }
   __syncthreads();
   dr_cluster_sync();
+  low = -warp_max(lane < C ? -__uint_as_float(dr_peer32(&s.low_x, lane)) : -INFINITY);
   mx = warp_max(lane < C ? __uint_as_float(dr_peer32(&s.max_x, lane)) : -INFINITY);
   if (greedy || mx == -INFINITY) {
     // the lowest id of the maximum; a row without any logit to draw from answers 0, as the arg-max does
@@ -244,10 +279,242 @@ draw_kernel(const DrawArgs a) {
     return goal >= (double)all ? all : goal < 1.0 ? 1ull : (unsigned long long)goal;
   };
 
-  // ---- pruned rows
   const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f;
-  if (has_k ? top_k <= kDrPrune : has_p) {
-    const int want = has_k ? top_k : kDrPrune;
+  // all values of the block with the whole warp in step: f(values, of how many, index of the first)
+  auto each_vec = [&](auto f) {
+    for (int b = warp * 32; b < nv; b += kDrThreads) {
+      const int j = b + lane;
+      float v[kVec];
+      vec_at(min(j, nv - 1), v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = j < nv && v[e] == v[e] ? v[e] : -INFINITY;
+      f(v, head + j * kVec);
+    }
+    if (warp == 0) {                                               // the ragged ends: fewer than 16 in all
+      float v[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
+      int i = lane;
+      if (lane < head) v[0] = Key::value(x[i]);
+      else if (lane - head < n - head - body) { i = body + lane; v[0] = Key::value(x[i]); }
+      f(v, i);
+    }
+  };
+  auto sum = [&](unsigned long long v) -> unsigned long long {     // over the block
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) s.scan[warp] = v;
+    __syncthreads();
+    v = s.scan[lane & (kDrWarps - 1)];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    return v;
+  };
+
+  // ---- The first block, alone, over the row's candidates: `found` of them, number q at cand_at(q).  A superset of what top-k and top-p keep; `target`: mass
+  // in front of which top-p keeps (0: top-p of the candidates that top-k keeps).
+  auto finish = [&](int found, unsigned long long target, auto cand_at) {
+    const bool cut_k = has_k && found > top_k;
+    if (found <= kDrPairs) {
+      // Few: every candidate against every other one.  Its rank, the mass in front of it, and the kept mass at lower ids are plain sums.
+      uint4* pair = reinterpret_cast<uint4*>(&s.lo[0][0]);         // key, id, mass (8 KB: lo and hi lie one behind the other)
+      const int q = tid & (kDrPairs - 1), half = tid / kDrPairs;
+      const uint2 e = q < found ? cand_at(q) : make_uint2(0u, 0u);
+      unsigned long long w = q < found ? weight(value_of(e.x)) : 0ull;
+      if (half == 0) pair[q] = make_uint4(e.x, e.y, (unsigned)w, (unsigned)(w >> 32));
+      __syncthreads();
+      const int j0 = half ? (found + 1) / 2 : 0, j1 = half ? found : (found + 1) / 2;
+      int place = 0;
+      unsigned long long front = 0;
+#pragma unroll 4
+      for (int j = j0; j < j1; ++j) {
+        const uint4 o = pair[j];
+        const bool ahead = o.x > e.x || (o.x == e.x && o.y < e.y);
+        place += ahead;
+        front += ahead ? (unsigned long long)o.w << 32 | o.z : 0ull;
+      }
+      unsigned long long* other = reinterpret_cast<unsigned long long*>(&s.count[0][0]);      // [kDrPairs], then the places
+      int* other_place = (int*)(other + kDrPairs);
+      if (half) { other[q] = front; other_place[q] = place; }
+      __syncthreads();
+      if (!half) { front += other[q]; place += other_place[q]; }
+      bool keep = !half && q < found && (!cut_k || place < top_k);
+      if (has_p) {
+        const unsigned long long goal = target != 0 ? target : top_p_target(sum(keep ? w : 0ull));
+        keep = keep && front < goal;
+      }
+      keep = keep && w >= min_w;
+      if (!keep) w = 0;
+      const unsigned long long all = sum(half ? 0ull : w), r = spot_of(all);
+      if (!half) pair[q] = make_uint4(e.x, e.y, (unsigned)w, (unsigned)(w >> 32));
+      __syncthreads();
+      unsigned long long below = 0;
+#pragma unroll 4
+      for (int j = j0; j < j1; ++j) {
+        const uint4 o = pair[j];
+        below += o.y < e.y ? (unsigned long long)o.w << 32 | o.z : 0ull;
+      }
+      if (half) other[q] = below;
+      __syncthreads();
+      if (!half && w != 0) {
+        below += other[q];
+        if (below <= r && r < below + w) {
+          a.out[row] = (int)e.y;
+          if (a.logprob != nullptr) a.logprob[row] = logprob_of(value_of(e.x), all);
+        }
+      }
+      return;
+    }
+    // Many: radix searches, four candidates a thread
+    constexpr int kOwn = kDrCand / kDrThreads;
+    unsigned key[kOwn], id[kOwn], least = 0xffffffffu;
+    unsigned long long w[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int q = k * kDrThreads + tid;
+      const uint2 e = q < found ? cand_at(q) : make_uint2(0u, 0u); // key 0: no candidate
+      key[k] = e.x; id[k] = e.y;
+      w[k] = q < found ? weight(value_of(e.x)) : 0ull;
+      if (q < found) least = min(least, e.x);
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (tid == 0) s.first_max = -1;
+    __syncthreads();
+    if (lane == 0) atomicMin((unsigned*)&s.first_max, least);
+    __syncthreads();
+    least = (unsigned)s.first_max;
+    // Searches the numbers of(k) in [base, base + range] for the one at which the running sum of val(k), from the top down (or from the bottom up), reaches `goal`;
+    // `before`: the sum in front of it.
+    auto search = [&](unsigned base, unsigned range, bool up, bool mass, unsigned long long goal, unsigned long long& before, auto of, auto val) -> unsigned {
+      unsigned prefix = 0;
+      before = 0;
+      for (int bits = 32 - __clz(range); bits > 0;) {
+        const int shift = max(0, bits - 9);
+        s.count[0][tid] = 0;
+        if (mass) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) {
+          const unsigned long long v = val(k);
+          const unsigned off = min(of(k) - base, range);
+          if (v == 0 || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
+          const int d = (off >> shift) & 511;
+          if (!mass) atomicAdd(&s.count[0][d], 1u);
+          else {
+            const unsigned l = (unsigned)v, old = atomicAdd(&s.lo[0][d], l);
+            const unsigned h = (unsigned)(v >> 32) + (old + l < old ? 1u : 0u);
+            if (h != 0) atomicAdd(&s.hi[0][d], h);
+          }
+        }
+        __syncthreads();
+        const int d = up ? tid : 511 - tid;
+        const unsigned long long v = mass ? ((unsigned long long)s.hi[0][d] << 32) + s.lo[0][d] : s.count[0][d];
+        dr_find(v, goal - before, s);
+        const int hit = s.found_at < 0 ? 0 : s.found_at;
+        prefix = prefix << (bits - shift) | (unsigned)(up ? hit : 511 - hit);
+        before += s.found_before;
+        bits = shift;
+        __syncthreads();
+      }
+      return base + prefix;
+    };
+    const unsigned top = Key::of(mx);
+    unsigned tau = 0;                                              // kept: key > tau, and the first `ties` ids of key tau
+    unsigned long long ties = 0, before;
+    auto key_of = [&](int k) { return key[k]; };
+    auto id_of = [&](int k) { return id[k]; };
+    auto strike = [&]() {                                          // takes the others out
+      unsigned long long n_tie = 0;
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) n_tie += key[k] != 0 && key[k] == tau;
+      n_tie = sum(n_tie);
+      unsigned last = 0xffffffffu;
+      if (n_tie > ties && ties > 0) last = search(0, (unsigned)a.vocab - 1, true, false, ties, before, id_of, [&](int k) -> unsigned long long { return key[k] != 0 && key[k] == tau; });
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) if (key[k] < tau || (key[k] == tau && (ties == 0 || id[k] > last))) { key[k] = 0; w[k] = 0; }
+    };
+    auto mass_of = [&]() {
+      unsigned long long m = 0;
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) m += w[k];
+      return sum(m);
+    };
+    if (cut_k) {
+      tau = search(least, top - least, false, false, (unsigned long long)top_k, before, key_of, [&](int k) -> unsigned long long { return key[k] != 0; });
+      ties = (unsigned long long)top_k - before;
+      strike();
+    }
+    if (has_p) {
+      const unsigned long long goal = target != 0 ? target : top_p_target(mass_of());
+      tau = search(least, top - least, false, true, goal, before, key_of, [&](int k) -> unsigned long long { return w[k]; });
+      const unsigned long long wt = weight(value_of(tau));
+      ties = wt > 0 ? (goal - before + wt - 1) / wt : 0;
+      strike();
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) if (w[k] < min_w) w[k] = 0;
+    const unsigned long long m = mass_of();
+    const unsigned token = search(0, (unsigned)a.vocab - 1, true, true, spot_of(m) + 1, before, id_of, [&](int k) -> unsigned long long { return w[k]; });
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      if (w[k] != 0 && id[k] == token) {
+        a.out[row] = (int)token;
+        if (a.logprob != nullptr) a.logprob[row] = logprob_of(value_of(key[k]), m);
+      }
+  };
+
+  // The first id of this block at which the mass of what keeps(key, id) and min-p leave, with `front` in front of the block, exceeds r.  Steps of 512 x 32 ids: a
+  // warp's 1024 in turn, then the warp that holds the place looks closer.
+  auto locate = [&](unsigned long long front, unsigned long long r, unsigned long long all, auto keeps) {
+    auto mass_at = [&](int i) -> unsigned long long {              // (the whole warp)
+      const float v = i < n ? Key::value(x[i]) : -INFINITY;
+      const unsigned long long w = weight_all(v);
+      return i < n && w >= min_w && keeps(Key::of(v), (unsigned)(i0 + i)) ? w : 0ull;
+    };
+    const int run = (n + kDrThreads - 1) / kDrThreads * 32;        // a warp's run of ids
+    unsigned long long mine = 0;
+    for (int b = 0; b < run; b += 64) {
+      mine += mass_at(warp * run + b + lane);
+      if (b + 32 < run) mine += mass_at(warp * run + b + 32 + lane);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s.warp_mass[warp] = mine;
+    __syncthreads();
+    int w = 0;
+    for (; w < kDrWarps - 1 && r >= front + s.warp_mass[w]; ++w) front += s.warp_mass[w];
+    __syncthreads();
+    // the run again, a piece of it per warp
+    const int piece = (run / 32 + kDrWarps - 1) / kDrWarps * 32;
+    mine = 0;
+    for (int b = warp * piece; b < min(run, (warp + 1) * piece); b += 32) mine += mass_at(w * run + b + lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s.warp_mass[warp] = mine;
+    __syncthreads();
+    int p = 0;
+    for (; p < kDrWarps - 1 && r >= front + s.warp_mass[p]; ++p) front += s.warp_mass[p];
+    if (warp != 0) return;
+    for (int b = p * piece; b < min(run, (p + 1) * piece); b += 32) {
+      const int i = w * run + b + lane;
+      unsigned long long incl = mass_at(i);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
+      const unsigned hit = __ballot_sync(0xffffffffu, r < front + incl);
+      if (hit != 0) {
+        if (lane == __ffs(hit) - 1) {
+          a.out[row] = i0 + i;
+          if (a.logprob != nullptr) a.logprob[row] = logprob_of(Key::value(x[i]), all);
+        }
+        return;
+      }
+      front += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  };
+
+  // ---- rows with a top-k: pruned
+  if (has_k && top_k <= kDrPrune) {
     if (rank == 0) {
       s.count[0][tid] = 0;
       __syncthreads();
@@ -257,8 +524,8 @@ draw_kernel(const DrawArgs a) {
         if (v > mx - kDrBins / 16.0f) atomicAdd(&s.count[0][bin_of(v)], 1u);
       }
       __syncthreads();
-      dr_find(s.count[0][tid], want, s);
-      // at least `want` logits lie in the bin and above; fewer in reach: all of them count
+      dr_find(s.count[0][tid], top_k, s);
+      // at least top_k logits lie in the bin and above; fewer in reach: all of them count
       const float bound = s.found_at >= 0 && s.found_at < kDrBins - 1 ? fmaxf(mx - (s.found_at + 1) * 0.0625f - fmaf(fabsf(mx), 2.5e-7f, 1e-5f), -FLT_MAX) : -FLT_MAX;
       if (tid < C) dr_put32(&s.bound, tid, __float_as_uint(bound));
     }
@@ -266,161 +533,207 @@ draw_kernel(const DrawArgs a) {
     __syncthreads();
     dr_cluster_sync();
     const float bound = s.bound;
-    {
-      const int cap = kDrCand / C;
-      unsigned long long mass = 0, all = 0;
-      auto take = [&](float v, int i) {
-        const int at = atomicAdd(&s.cand_own, 1);
-        if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i) << 32 | Key::of(v));
-      };
-      if (has_k) {
-#pragma unroll 4
-        for (int i = tid; i < n; i += kDrThreads) { const float v = Key::value(x[i]); if (v >= bound) take(v, i); }
-      } else {
-        for (int b = warp * 32; b < n; b += kDrThreads) {
-          const int i = b + lane;
-          const float v = i < n ? Key::value(x[i]) : -INFINITY;
-          const unsigned long long w = weight_all(v);
-          all += w;
-          if (v >= bound) { mass += w; take(v, i); }
-        }
+    const int cap = kDrCand / C;                                   // places of a block
+    auto take = [&](float v, int i) {
+      const int at = atomicAdd(&s.cand_own, 1);
+      if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i) << 32 | Key::of(v));
+    };
+    ends([&](float v, int i) { if (v >= bound) take(v, i); });
+#pragma unroll 2
+    for (int j = tid; j < nv; j += kDrThreads) {
+      float v[kVec];
+      vec_at(j, v);
+      float most = v[0];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { mass += __shfl_xor_sync(0xffffffffu, mass, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
-        if (lane == 0) { s.warp_mass[warp] = mass; s.scan[warp] = all; }
-        __syncthreads();
-        if (tid < C) {
-          mass = 0; all = 0;
-          for (int w = 0; w < kDrWarps; ++w) { mass += s.warp_mass[w]; all += s.scan[w]; }
-          dr_put64(&s.cand_mass[rank], tid, mass);
-          dr_put64(&s.cand_all[rank], tid, all);
-        }
+      for (int e = 1; e < kVec; ++e) most = fmaxf(most, v[e]);
+      if (most >= bound) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) if (v[e] >= bound) take(v[e], head + j * kVec + e);
       }
-      __syncthreads();
-      if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
-      dr_cluster_sync();
-      bool settled = true;
+    }
+    __syncthreads();
+    if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
+    dr_cluster_sync();
+    bool settled = true;
+    for (int c = 0; c < C; ++c) settled &= s.cand_n[c] <= cap;
+    if (settled) {
+      if (rank != 0) return;                                       // (nobody reads this block's shared memory any more)
       int found = 0;
-      unsigned long long c_mass = 0, c_all = 0;
-      for (int c = 0; c < C; ++c) {
-        found += s.cand_n[c];
-        settled &= s.cand_n[c] <= cap;
-        if (!has_k) { c_mass += s.cand_mass[c]; c_all += s.cand_all[c]; }
+      for (int c = 0; c < C; ++c) found += s.cand_n[c];
+      finish(found, 0, [&](int q) -> uint2 {
+        int c = 0;
+        while (q >= s.cand_n[c]) q -= s.cand_n[c++];
+        return s.cand[c * cap + q];
+      });
+      return;
+    }
+  }
+  // ---- rows with a top-p alone: one pass for all weights and their histogram, over steps that suit the row: to twice the depth of its lowest group, at most
+  // 45 halvings.  The step of the cut is then known, with the mass in front of it.
+  if (has_p && !has_k) {
+    const float depth = fminf(2.0f * (mx - low), 32.0f * temp), steps = kDrBins / depth;
+    auto step_of = [&](float v) -> int { return max(0, min(kDrBins - 1, (int)fminf((mx - v) * steps, 1e6f))); };      // monotone in v
+    s.count[0][tid] = 0; s.lo[0][tid] = 0; s.hi[0][tid] = 0;
+    __syncthreads();
+    each_vec([&](const float* v, int) {
+      unsigned long long w[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w[e] = weight_all(v[e]);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (w[e] == 0) continue;
+        const int b = step_of(v[e]);
+        const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[0][b], l);
+        const unsigned h = (unsigned)(w[e] >> 32) + (old + l < old ? 1u : 0u);
+        if (h != 0) atomicAdd(&s.hi[0][b], h);
+        atomicAdd(&s.count[0][b], 1u);
       }
-      if (!has_k) settled &= c_mass >= top_p_target(c_all);
-      if (settled) {
-        if (rank != 0) return;                                     // (nobody reads this block's shared memory any more)
-        // ---- the first block, alone: four candidates a thread
+    });
+    __syncthreads();
+    dr_cluster_sync();
+    unsigned n_at[8];                                              // logits of the thread's step in every block
+    unsigned long long at = 0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      n_at[c] = c < C ? dr_peer32(&s.count[0][tid], c) : 0u;
+      if (c < C) at += ((unsigned long long)dr_peer32(&s.hi[0][tid], c) << 32) + dr_peer32(&s.lo[0][tid], c);
+    }
+    const unsigned long long target = top_p_target(sum(at));
+    dr_find(at, target, s);
+    const int cut = s.found_at;
+    const unsigned long long before = s.found_before;
+    // how many of each block lie above the cut's step, and in it
+    if (tid < 8) s.cand_n[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const unsigned m = __reduce_add_sync(0xffffffffu, tid < cut ? n_at[c] : 0u);
+      if (lane == 0 && m != 0) atomicAdd(&s.cand_n[c], (int)m);
+      if (tid == cut) s.cand_in[c] = n_at[c];
+    }
+    __syncthreads();
+    int above = 0, in_cut = 0, my_above = 0, my_cut = 0;
+    for (int c = 0; c < C; ++c) {
+      if (c == rank) { my_above = above + in_cut; my_cut = in_cut; }
+      above += s.cand_n[c]; in_cut += s.cand_in[c];
+    }
+    const bool few = above + in_cut <= kDrCand, some = in_cut <= kDrCand && min_w == 0;
+    if (cut >= 0 && cut < kDrBins - 1 && (few || some)) {
+      // the candidates, or those of the cut's step, to the first block; each block keeps its own of the latter too
+      if (tid == 0) s.cand_own = 0;
+      __syncthreads();
+      const int base = few ? my_above : my_cut;
+      const float bound = fmaxf(mx - (cut + 1) / steps - fmaf(fabsf(mx) + depth, 1e-6f, 1e-4f), -FLT_MAX);       // (a little below the step: which step a logit is of is asked anew)
+      each_vec([&](const float* v, int i) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          if (!(v[e] >= bound)) continue;
+          const int b = step_of(v[e]);
+          if (b > cut || (!few && b < cut) || weight(v[e]) == 0) continue;
+          const int k = atomicAdd(&s.cand_own, 1);
+          const unsigned long long entry = (unsigned long long)(unsigned)(i0 + i + e) << 32 | Key::of(v[e]);
+          if (base + k < kDrCand) dr_put64(&s.cand[base + k], 0, entry);
+          if (!few && rank != 0 && k < kDrCand) s.cand[k] = make_uint2((unsigned)entry, (unsigned)(entry >> 32));
+        }
+      });
+      __syncthreads();
+      const int own = min(s.cand_own, kDrCand);
+      dr_cluster_sync();
+      if (few) {
+        if (rank != 0) return;
+        finish(above + in_cut, target, [&](int q) { return s.cand[q]; });
+        return;
+      }
+      // Many above the cut: the first block finds the cut in its step, every block then knows its kept mass, and the block in which the draw falls goes through
+      // its logits once more.
+      if (rank == 0) {
         constexpr int kOwn = kDrCand / kDrThreads;
-        unsigned key[kOwn], id[kOwn];
+        unsigned key[kOwn], id[kOwn], least = 0xffffffffu, most = 0;
         unsigned long long w[kOwn];
-        unsigned low = 0xffffffffu;
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
-          const int at = k * kDrThreads + tid;
-          const bool in = at % cap < s.cand_n[at / cap];
-          const uint2 e = in ? s.cand[at] : make_uint2(0u, 0u);
-          key[k] = e.x; id[k] = e.y;                               // key 0: no candidate
-          w[k] = in ? weight(value_of(e.x)) : 0ull;
-          if (in) low = min(low, e.x);
+          const int q = k * kDrThreads + tid;
+          const uint2 e = q < in_cut ? s.cand[q] : make_uint2(0u, 0u);
+          key[k] = e.x; id[k] = e.y;
+          w[k] = q < in_cut ? weight(value_of(e.x)) : 0ull;
+          if (q < in_cut) { least = min(least, e.x); most = max(most, e.x); }
         }
-        low = __reduce_min_sync(0xffffffffu, low);
-        if (tid == 0) s.first_max = -1;
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (tid == 0) { s.first_max = -1; s.tau = 0; }
         __syncthreads();
-        if (lane == 0) atomicMin((unsigned*)&s.first_max, low);
+        if (lane == 0) { atomicMin((unsigned*)&s.first_max, least); atomicMax(&s.tau, most); }
         __syncthreads();
-        low = (unsigned)s.first_max;
-        // Searches the numbers of(k) in [base, base + range] for the one at which the running sum of val(k), from the top down (or from the bottom up), reaches `target`;
-        // `before`: the sum in front of it.
-        auto search = [&](unsigned base, unsigned range, bool up, bool mass, unsigned long long target, unsigned long long& before, auto of, auto val) -> unsigned {
+        least = (unsigned)s.first_max; most = s.tau;
+        // the key at which the mass reaches the target, and, of equal keys, the id
+        unsigned found[2] = {0, 0};
+        unsigned long long goal = target - before;
+#pragma unroll
+        for (int by_id = 0; by_id < 2; ++by_id) {
+          const unsigned first = by_id ? 0u : least, range = by_id ? (unsigned)a.vocab - 1 : most - least;
           unsigned prefix = 0;
-          before = 0;
           for (int bits = 32 - __clz(range); bits > 0;) {
             const int shift = max(0, bits - 9);
-            s.count[0][tid] = 0;
-            if (mass) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+            __syncthreads();
+            s.lo[1][tid] = 0; s.hi[1][tid] = 0;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kOwn; ++k) {
-              const unsigned long long v = val(k);
-              const unsigned off = min(of(k) - base, range);
-              if (v == 0 || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
+              const unsigned off = min((by_id ? id[k] : key[k]) - first, range);
+              if (w[k] == 0 || (by_id && key[k] != found[0]) || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
               const int d = (off >> shift) & 511;
-              if (!mass) atomicAdd(&s.count[0][d], 1u);
-              else {
-                const unsigned l = (unsigned)v, old = atomicAdd(&s.lo[0][d], l);
-                const unsigned h = (unsigned)(v >> 32) + (old + l < old ? 1u : 0u);
-                if (h != 0) atomicAdd(&s.hi[0][d], h);
-              }
+              const unsigned l = (unsigned)w[k], old = atomicAdd(&s.lo[1][d], l);
+              const unsigned h = (unsigned)(w[k] >> 32) + (old + l < old ? 1u : 0u);
+              if (h != 0) atomicAdd(&s.hi[1][d], h);
             }
             __syncthreads();
-            const int d = up ? tid : 511 - tid;
-            const unsigned long long v = mass ? ((unsigned long long)s.hi[0][d] << 32) + s.lo[0][d] : s.count[0][d];
-            dr_find(v, target - before, s);
+            const int d = by_id ? tid : 511 - tid;
+            dr_find(((unsigned long long)s.hi[1][d] << 32) + s.lo[1][d], goal, s);
             const int hit = s.found_at < 0 ? 0 : s.found_at;
-            prefix = prefix << (bits - shift) | (unsigned)(up ? hit : 511 - hit);
-            before += s.found_before;
+            prefix = prefix << (bits - shift) | (unsigned)(by_id ? hit : 511 - hit);
+            goal -= s.found_before;
             bits = shift;
-            __syncthreads();
           }
-          return base + prefix;
-        };
-        auto sum = [&](unsigned long long v) -> unsigned long long {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (lane == 0) s.scan[warp] = v;
-          __syncthreads();
-          v = 0;
-          for (int x = 0; x < kDrWarps; ++x) v += s.scan[x];
-          __syncthreads();
-          return v;
-        };
-        const unsigned top = Key::of(mx);
-        unsigned tau = 0;                                          // kept: key > tau, and the first `ties` ids of key tau
-        unsigned long long ties = 0, before;
-        auto key_of = [&](int k) { return key[k]; };
-        auto id_of = [&](int k) { return id[k]; };
-        const bool cut_k = has_k && found > top_k;
-        if (cut_k) {
-          tau = search(low, top - low, false, false, (unsigned long long)top_k, before, key_of, [&](int k) -> unsigned long long { return key[k] != 0; });
-          ties = (unsigned long long)top_k - before;
+          found[by_id] = first + prefix;
         }
-        // of equal keys at the cut the first ids stay; the others are struck out
-        auto strike = [&]() {
-          unsigned long long n_tie = 0;
-#pragma unroll
-          for (int k = 0; k < kOwn; ++k) n_tie += key[k] != 0 && key[k] == tau;
-          n_tie = sum(n_tie);
-          unsigned last = 0xffffffffu;
-          if (n_tie > ties && ties > 0) last = search(0, (unsigned)a.vocab - 1, true, false, ties, before, id_of, [&](int k) -> unsigned long long { return key[k] != 0 && key[k] == tau; });
-#pragma unroll
-          for (int k = 0; k < kOwn; ++k) if (key[k] < tau || (key[k] == tau && (ties == 0 || id[k] > last))) { key[k] = 0; w[k] = 0; }
-        };
-        if (cut_k) strike();
-        if (has_p) {
-          unsigned long long m = 0;
-#pragma unroll
-          for (int k = 0; k < kOwn; ++k) m += w[k];
-          m = sum(m);
-          const unsigned long long target = top_p_target(has_k ? m : c_all);
-          tau = search(low, top - low, false, true, target, before, key_of, [&](int k) -> unsigned long long { return w[k]; });
-          const unsigned long long wt = weight(value_of(tau));
-          ties = wt > 0 ? (target - before + wt - 1) / wt : 0;
-          strike();
-        }
-        unsigned long long m = 0;
-#pragma unroll
-        for (int k = 0; k < kOwn; ++k) { if (w[k] < min_w) w[k] = 0; m += w[k]; }
-        m = sum(m);
-        const unsigned token = search(0, (unsigned)a.vocab - 1, true, true, spot_of(m) + 1, before, id_of, [&](int k) -> unsigned long long { return w[k]; });
-#pragma unroll
-        for (int k = 0; k < kOwn; ++k)
-          if (w[k] != 0 && id[k] == token) {
-            a.out[row] = (int)token;
-            if (a.logprob != nullptr) a.logprob[row] = logprob_of(value_of(key[k]), m);
-          }
-        return;
+        __syncthreads();
+        if (tid < C) { dr_put32(&s.tau, tid, found[0]); dr_put32(&s.last, tid, found[1]); }
       }
+      dr_cluster_sync();
+      const unsigned tau = s.tau, last = s.last;
+      auto keeps = [&](unsigned key, unsigned id) { return key > tau || (key == tau && id <= last); };
+      unsigned long long mine = tid < cut ? ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid] : 0ull;
+      for (int q = tid; q < own; q += kDrThreads) {
+        const uint2 e = s.cand[q];
+        if (keeps(e.x, e.y)) mine += weight(value_of(e.x));
+      }
+      mine = sum(mine);
+      if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
+      dr_cluster_sync();
+      unsigned long long all = 0, front = 0;
+      for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
+      const unsigned long long r = spot_of(all);
+      if (r < front || r >= front + mine) return;
+      locate(front, r, all, keeps);
+      return;
     }
+  }
+  // ---- rows without a limit, or with min-p alone: one pass for the blocks' masses
+  if (!has_k && !has_p) {
+    unsigned long long mine = 0;
+    each_vec([&](const float* v, int) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) { const unsigned long long w = weight_all(v[e]); mine += w >= min_w ? w : 0ull; }
+    });
+    mine = sum(mine);
+    if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
+    dr_cluster_sync();
+    unsigned long long all = 0, front = 0;
+    for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
+    const unsigned long long r = spot_of(all);
+    if (r < front || r >= front + mine) return;
+    locate(front, r, all, [&](unsigned, unsigned) { return true; });
+    return;
   }
 
   // ---- the cluster's path.  A warp owns a run of the block's ids
@@ -438,7 +751,7 @@ draw_kernel(const DrawArgs a) {
       f(v, in && v > -INFINITY);
     }
   };
-  int step = 0;                                                    // parity of the histogram in use
+  int step = 1;                                                    // parity of the histogram in use (not the one that other blocks may still be reading)
   auto clear = [&](bool mass) {
     for (int i = tid; i < kDrBins; i += kDrThreads) { s.count[step & 1][i] = 0; if (mass) { s.lo[step & 1][i] = 0; s.hi[step & 1][i] = 0; } }
     __syncthreads();
