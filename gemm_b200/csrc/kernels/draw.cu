@@ -85,6 +85,11 @@ __device__ __forceinline__ uint32_t dr_peer32(const void* p, int cta) {
   asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
   return v;
 }
+__device__ __forceinline__ uint4 dr_peer128(const void* p, int cta) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
+  return v;
+}
 __device__ __forceinline__ unsigned long long dr_peer64(const void* p, int cta) {
   unsigned long long v;
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(dr_mapa(smem_u32(p), cta)) : "memory");
@@ -446,11 +451,13 @@ draw_kernel(const DrawArgs a) {
       strike();
     }
     if (has_p) {
-      const unsigned long long goal = target != 0 ? target : top_p_target(mass_of());
-      tau = search(least, top - least, false, true, goal, before, key_of, [&](int k) -> unsigned long long { return w[k]; });
-      const unsigned long long wt = weight(value_of(tau));
-      ties = wt > 0 ? (goal - before + wt - 1) / wt : 0;
-      strike();
+      const unsigned long long have = mass_of(), goal = target != 0 ? target : top_p_target(have);
+      if (have > goal) {                                           // (else all are kept: min-p has left out what lies behind)
+        tau = search(least, top - least, false, true, goal, before, key_of, [&](int k) -> unsigned long long { return w[k]; });
+        const unsigned long long wt = weight(value_of(tau));
+        ties = wt > 0 ? (goal - before + wt - 1) / wt : 0;
+        strike();
+      }
     }
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) if (w[k] < min_w) w[k] = 0;
@@ -513,9 +520,12 @@ draw_kernel(const DrawArgs a) {
     }
   };
 
-  // ---- rows with a top-k: pruned
-  if (has_k && top_k <= kDrPrune) {
-    if (rank == 0) {
+  // ---- rows with a top-k: pruned.  With min-p alone the bound is known
+  if (has_k ? top_k <= kDrPrune : !has_p && min_w != 0) {
+    if (tid == 0) s.cand_own = 0;
+    float bound = fmaxf(mx + temp * logf(fminf(min_p, 1.0f)) - fmaf(fabsf(mx), 2.5e-7f, 1e-5f) - temp * 1e-5f, -FLT_MAX);
+    if (!has_k) __syncthreads();
+    if (has_k && rank == 0) {
       s.count[0][tid] = 0;
       __syncthreads();
 #pragma unroll
@@ -526,13 +536,14 @@ draw_kernel(const DrawArgs a) {
       __syncthreads();
       dr_find(s.count[0][tid], top_k, s);
       // at least top_k logits lie in the bin and above; fewer in reach: all of them count
-      const float bound = s.found_at >= 0 && s.found_at < kDrBins - 1 ? fmaxf(mx - (s.found_at + 1) * 0.0625f - fmaf(fabsf(mx), 2.5e-7f, 1e-5f), -FLT_MAX) : -FLT_MAX;
-      if (tid < C) dr_put32(&s.bound, tid, __float_as_uint(bound));
+      const float low_bound = s.found_at >= 0 && s.found_at < kDrBins - 1 ? fmaxf(mx - (s.found_at + 1) * 0.0625f - fmaf(fabsf(mx), 2.5e-7f, 1e-5f), -FLT_MAX) : -FLT_MAX;
+      if (tid < C) dr_put32(&s.bound, tid, __float_as_uint(low_bound));
     }
-    if (tid == 0) s.cand_own = 0;
-    __syncthreads();
-    dr_cluster_sync();
-    const float bound = s.bound;
+    if (has_k) {
+      __syncthreads();
+      dr_cluster_sync();
+      bound = s.bound;
+    }
     const int cap = kDrCand / C;                                   // places of a block
     auto take = [&](float v, int i) {
       const int at = atomicAdd(&s.cand_own, 1);
@@ -591,25 +602,57 @@ draw_kernel(const DrawArgs a) {
     });
     __syncthreads();
     dr_cluster_sync();
-    unsigned n_at[8];                                              // logits of the thread's step in every block
+    // The blocks' histograms, four steps of one block a turn (16-byte loads; single ones took 7500 cycles, these 3000): lanes 8 apart hold the same block.
     unsigned long long at = 0;
+    unsigned n_at[2 * 4];
+    const int block = lane & 7;
+    unsigned long long part[2 * 4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      n_at[c] = c < C ? dr_peer32(&s.count[0][tid], c) : 0u;
-      if (c < C) at += ((unsigned long long)dr_peer32(&s.hi[0][tid], c) << 32) + dr_peer32(&s.lo[0][tid], c);
+    for (int k = 0; k < 2; ++k) {
+      const int quad = (tid >> 3) + k * (kDrThreads / 8);
+      uint4 c4 = make_uint4(0, 0, 0, 0), l4 = c4, h4 = c4;
+      if (block < C) { c4 = dr_peer128(&s.count[0][quad * 4], block); l4 = dr_peer128(&s.lo[0][quad * 4], block); h4 = dr_peer128(&s.hi[0][quad * 4], block); }
+      n_at[k * 4] = c4.x; n_at[k * 4 + 1] = c4.y; n_at[k * 4 + 2] = c4.z; n_at[k * 4 + 3] = c4.w;
+      part[k * 4] = (unsigned long long)h4.x << 32; part[k * 4 + 1] = (unsigned long long)h4.y << 32; part[k * 4 + 2] = (unsigned long long)h4.z << 32;
+      part[k * 4 + 3] = (unsigned long long)h4.w << 32;
+      part[k * 4] += l4.x; part[k * 4 + 1] += l4.y; part[k * 4 + 2] += l4.z; part[k * 4 + 3] += l4.w;
     }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                                  // (sums: in the other parity, which no other block reads)
+      const int b = ((tid >> 3) + (k >> 2) * (kDrThreads / 8)) * 4 + (k & 3);
+      if (block == k) { s.lo[1][b] = (unsigned)part[k]; s.hi[1][b] = (unsigned)(part[k] >> 32); }
+    }
+    __syncthreads();
+    at = (unsigned long long)s.hi[1][tid] << 32 | s.lo[1][tid];
     const unsigned long long target = top_p_target(sum(at));
     dr_find(at, target, s);
-    const int cut = s.found_at;
+    int cut = s.found_at;
     const unsigned long long before = s.found_before;
+    // min-p may cut higher up: what lies more than a step below its weight is kept by neither
+    const int full_cut = cut;
+    if (min_w != 0 && cut > 0) cut = min(cut, step_of(mx + temp * logf(fminf(min_p, 1.0f)) - fmaf(fabsf(mx) + depth, 1e-6f, 1e-4f)) + 1);
     // how many of each block lie above the cut's step, and in it
-    if (tid < 8) s.cand_n[tid] = 0;
+    if (tid < 8) { s.cand_n[tid] = 0; s.cand_in[tid] = 0; }
     __syncthreads();
+    {
+      unsigned up = 0, in = 0;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const unsigned m = __reduce_add_sync(0xffffffffu, tid < cut ? n_at[c] : 0u);
-      if (lane == 0 && m != 0) atomicAdd(&s.cand_n[c], (int)m);
-      if (tid == cut) s.cand_in[c] = n_at[c];
+      for (int k = 0; k < 8; ++k) {
+        const int b = ((tid >> 3) + (k >> 2) * (kDrThreads / 8)) * 4 + (k & 3);
+        if (b < cut) up += n_at[k];
+        if (b == cut) in += n_at[k];
+      }
+      up += __shfl_xor_sync(0xffffffffu, up, 8); up += __shfl_xor_sync(0xffffffffu, up, 16);
+      in += __shfl_xor_sync(0xffffffffu, in, 8); in += __shfl_xor_sync(0xffffffffu, in, 16);
+      if (lane < 8) {
+        if (up != 0) atomicAdd(&s.cand_n[block], (int)up);
+        if (in != 0) atomicAdd(&s.cand_in[block], (int)in);
+      }
     }
     __syncthreads();
     int above = 0, in_cut = 0, my_above = 0, my_cut = 0;
@@ -618,6 +661,7 @@ draw_kernel(const DrawArgs a) {
       above += s.cand_n[c]; in_cut += s.cand_in[c];
     }
     const bool few = above + in_cut <= kDrCand, some = in_cut <= kDrCand && min_w == 0;
+    cut = few || some ? cut : full_cut;
     if (cut >= 0 && cut < kDrBins - 1 && (few || some)) {
       // the candidates, or those of the cut's step, to the first block; each block keeps its own of the latter too
       if (tid == 0) s.cand_own = 0;
@@ -718,7 +762,7 @@ draw_kernel(const DrawArgs a) {
       return;
     }
   }
-  // ---- rows without a limit, or with min-p alone: one pass for the blocks' masses
+  // ---- rows without a limit, or with min-p alone (too many for the first block): one pass for the blocks' masses
   if (!has_k && !has_p) {
     unsigned long long mine = 0;
     each_vec([&](const float* v, int) {
@@ -980,9 +1024,9 @@ draw_kernel(const DrawArgs a) {
 
 template <typename T>
 static int draw_launch(DrawArgs a, cudaStream_t stream) {
-  // Blocks per row.  A block's passes cost less than its share of the cluster's steps below some 20,000 logits; few rows take as many blocks as there is room for.  Two blocks share an SM where 90 KB hold a share.
+  // Blocks per row: as few as hold it with two blocks to an SM (the steps of a cluster cost every block of it); few rows take as many as there is room for.
   int c = 1;
-  while (c < 8 && (a.vocab > c * 20480 || (long)((a.vocab + c - 1) / c) * (long)sizeof(T) > 90000 || (a.vocab > c * 4096 && a.rows * c * 2 <= sm_count()))) c *= 2;
+  while (c < 8 && ((long)((a.vocab + c - 1) / c) * (long)sizeof(T) > 90000 || (a.vocab > c * 4096 && a.rows * c * 2 <= sm_count()))) c *= 2;
   a.ctas = c;
   a.per = ((a.vocab + c - 1) / c + 15) / 16 * 16;
   const size_t smem = (size_t)a.per * sizeof(T) + 32;
