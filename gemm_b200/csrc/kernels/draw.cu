@@ -202,7 +202,7 @@ draw_kernel(const DrawArgs a) {
   float mx = -INFINITY, low = INFINITY;
   {
     const int pieces = kDrGroups / kDrThreads / C;
-    const bool fine = nv < pieces * kDrThreads;                    // few logits: groups of single ones rather than empty groups
+    const bool fine = 2 * nv < pieces * kDrThreads;                // few logits: groups of single ones rather than empty groups
     for (int p = 0; p < pieces; ++p) {
       float gm = -INFINITY;
       if (fine) {
@@ -545,23 +545,27 @@ draw_kernel(const DrawArgs a) {
       bound = s.bound;
     }
     const int cap = kDrCand / C;                                   // places of a block
-    auto take = [&](float v, int i) {
-      const int at = atomicAdd(&s.cand_own, 1);
-      if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i) << 32 | Key::of(v));
-    };
-    ends([&](float v, int i) { if (v >= bound) take(v, i); });
-#pragma unroll 2
-    for (int j = tid; j < nv; j += kDrThreads) {
-      float v[kVec];
-      vec_at(j, v);
+    each_vec([&](const float* v, int i) {
       float most = v[0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) most = fmaxf(most, v[e]);
-      if (most >= bound) {
+      if (!__any_sync(0xffffffffu, most >= bound)) return;
+      int mine = 0;                                                // one addition to the block's count per warp and vector
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) if (v[e] >= bound) take(v[e], head + j * kVec + e);
-      }
-    }
+      for (int e = 0; e < kVec; ++e) mine += v[e] >= bound;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
+      int at = 0;
+      if (lane == 31) at = atomicAdd(&s.cand_own, incl);
+      at = __shfl_sync(0xffffffffu, at, 31) + incl - mine;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (v[e] >= bound) {
+          if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i + e) << 32 | Key::of(v[e]));
+          ++at;
+        }
+    });
     __syncthreads();
     if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
     dr_cluster_sync();
@@ -581,6 +585,7 @@ draw_kernel(const DrawArgs a) {
   }
   // ---- rows with a top-p alone: one pass for all weights and their histogram, over steps that suit the row: to twice the depth of its lowest group, at most
   // 45 halvings.  The step of the cut is then known, with the mass in front of it.
+  bool by_min_p = false;
   if (has_p && !has_k) {
     const float depth = fminf(2.0f * (mx - low), 32.0f * temp), steps = kDrBins / depth;
     auto step_of = [&](float v) -> int { return max(0, min(kDrBins - 1, (int)fminf((mx - v) * steps, 1e6f))); };      // monotone in v
@@ -634,8 +639,10 @@ draw_kernel(const DrawArgs a) {
     int cut = s.found_at;
     const unsigned long long before = s.found_before;
     // min-p may cut higher up: what lies more than a step below its weight is kept by neither
-    const int full_cut = cut;
-    if (min_w != 0 && cut > 0) cut = min(cut, step_of(mx + temp * logf(fminf(min_p, 1.0f)) - fmaf(fabsf(mx) + depth, 1e-6f, 1e-4f)) + 1);
+    const float min_off = min_w != 0 ? -temp * logf(fminf(min_p, 1.0f)) : 0.f, slack = fmaf(fabsf(mx) + depth + min_off, 1e-6f, 1e-4f);
+    const int full_cut = cut, min_step = min_w != 0 ? step_of(mx - min_off - slack) + 1 : kDrBins;         // no logit of this step or below has the weight
+    const int all_step = min_w != 0 ? step_of(mx - min_off + slack) : kDrBins;                             // all logits above this step have it
+    if (cut > 0) cut = min(cut, min_step);
     // how many of each block lie above the cut's step, and in it
     if (tid < 8) { s.cand_n[tid] = 0; s.cand_in[tid] = 0; }
     __syncthreads();
@@ -660,9 +667,9 @@ draw_kernel(const DrawArgs a) {
       if (c == rank) { my_above = above + in_cut; my_cut = in_cut; }
       above += s.cand_n[c]; in_cut += s.cand_in[c];
     }
-    const bool few = above + in_cut <= kDrCand, some = in_cut <= kDrCand && min_w == 0;
-    cut = few || some ? cut : full_cut;
-    if (cut >= 0 && cut < kDrBins - 1 && (few || some)) {
+    const bool few = above + in_cut <= kDrCand, some = in_cut <= kDrCand && full_cut < all_step;      // (some: min-p leaves all that top-p leaves)
+    by_min_p = !few && min_step < full_cut && full_cut > 0;                    // min-p cuts first: nothing of top-p is left to do
+    if (cut >= 0 && cut < kDrBins - 1 && (few || some) && !by_min_p) {
       // the candidates, or those of the cut's step, to the first block; each block keeps its own of the latter too
       if (tid == 0) s.cand_own = 0;
       __syncthreads();
@@ -763,7 +770,7 @@ draw_kernel(const DrawArgs a) {
     }
   }
   // ---- rows without a limit, or with min-p alone (too many for the first block): one pass for the blocks' masses
-  if (!has_k && !has_p) {
+  if (!has_k && (!has_p || by_min_p)) {
     unsigned long long mine = 0;
     each_vec([&](const float* v, int) {
 #pragma unroll
