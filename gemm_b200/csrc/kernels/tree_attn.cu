@@ -22,28 +22,31 @@
 namespace gb {
 
 constexpr int kTaThreads = 384;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads; 11: segments
-constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, with folded rows one to join them in, the rest is the ring
+constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, one in which rows are joined and put in order, the rest is the ring
 constexpr int kTaSegs = 4;          // segments handed out ahead
 constexpr int kTaSmem = 1024 + kTaTiles * 32768 + 2048;
 
 struct TreeAttnArgs {
   const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
   int n_seqs, max_pages, page_size, words, window, hq, hkv, total_tokens;
+  int G, tpt;                        // query heads per KV head; nodes per tile
   int pair;                          // tiles per item: 1 or 2
   int fold;                          // copies of the rows in a tile: 1, 2 or 4 (pair = 1, and at most 128 / fold rows in any sequence)
   int whole;                         // items are not cut (short contexts): no parts
+  int head;                          // cost of an item's start and end, in blocks of one tile
   __nv_bfloat16* out;                // [T, hq, DV]
   float* part_o; float* part_lse;    // [2 * grid][pair * 128][DV], [2 * grid][pair * 128]
-  int4* part_of;                     // [grid]: the item that begins in a piece and goes on behind it {sequence, item of it, parts, first part's slot}; parts = 0: none
+  int4* part_of;                     // [grid]: the item that begins in a piece and goes on behind it {parts, first part's slot | KV head << 16, its first token, nodes from there on};
+                                     // parts = 0: none
   const __nv_bfloat16* v_cache; long num_slots;
   KernelStatus* status;
 };
 
 // Shape of a sequence's work.
 struct TaSeq {
-  int begin, nodes, len, ctx, first, blocks, units, tiles, items;
+  int begin, nodes, len, ctx, first, blocks, units, tiles, pairs, items, head;
   __device__ __forceinline__ void load(const TreeAttnArgs& a, int s) {
-    const int G = a.hq / a.hkv, tpt = 128 / a.fold / G;
+    const int tpt = a.tpt;
     begin = min(max(a.cu_q[s], 0), a.total_tokens);
     nodes = max(min(a.cu_q[s + 1], a.total_tokens) - begin, 0);
     const int kv = a.kv_len[s];
@@ -53,14 +56,18 @@ struct TaSeq {
     blocks = max(0, (len + 127) / 128 - first);
     units = a.whole ? 1 : max(1, blocks);
     tiles = (nodes + tpt - 1) / tpt;
-    items = (tiles + a.pair - 1) / a.pair * a.hkv;
+    pairs = (tiles + a.pair - 1) >> (a.pair - 1);
+    items = pairs * a.hkv;
+    head = a.whole ? 0 : a.head;
   }
+  // The line that is cut: an item takes `head` (its start and its end, in blocks of one tile) and, per block, one for each of its tiles.
+  __device__ __forceinline__ long long cost(const TreeAttnArgs& a) const { return a.whole ? items : (long long)a.hkv * (pairs * head + (long long)tiles * units); }
 };
 
-// The pieces: [c * total / active, (c + 1) * total / active) of the line of units.
+// The pieces: [c * total / active, (c + 1) * total / active) of the line.
 struct TaPiece {
   long long total, pos, left;
-  int active, seq, item, unit;
+  int active, seq, item, off;             // off: place in the item
 };
 
 // The part of an item that a block works on.
@@ -73,34 +80,49 @@ struct TaSeg {
   int parts;                              // the item begins here and is cut: into so many parts
 };
 
+// Begin of piece c, and the piece that holds a place.  (64-bit division takes some hundred instructions: where 32 bits do, they are used.)
+__device__ __forceinline__ long long ta_begin(int c, long long total, int active) {
+  return total < (1 << 22) ? (long long)((unsigned)c * (unsigned)total / (unsigned)active) : c * total / active;             // (c <= 148)
+}
+__device__ __forceinline__ int ta_piece_of(long long at, long long total, int active) {
+  return total < (1 << 22) ? (int)(((unsigned)(at + 1) * (unsigned)active - 1) / (unsigned)total) : (int)(((at + 1) * active - 1) / total);
+}
+
 struct TaWalk {
   TaPiece p;
   TaSeq q;
   int at, nth;
   __device__ __forceinline__ bool next(const TreeAttnArgs& a, TaSeg& s) {
-    if (p.left <= 0) return false;
-    if (at != p.seq) { q.load(a, p.seq); at = p.seq; }
-    const int take = (int)min((long long)(q.units - p.unit), p.left);
-    const int pairs = q.items / a.hkv;
-    s.q = q; s.seq = p.seq; s.item = p.item;
-    s.kvh = p.item / pairs; s.tile = (p.item - s.kvh * pairs) * a.pair; s.n_tiles = min(a.pair, q.tiles - s.tile);
-    s.lo = q.first + (a.whole ? 0 : p.unit); s.n = a.whole ? q.blocks : min(take, q.blocks - p.unit);
-    s.full = take == q.units;
-    s.slot = 2 * (int)blockIdx.x + (nth++ == 0 ? 0 : 1);
-    s.parts = 0;
-    if (!s.full && p.unit == 0) {
-      const long long last = p.pos + q.units - 1;                  // the item's last unit; the piece it lies in is the last one that begins at or before it
-      s.parts = (int)(((last + 1) * p.active - 1) / p.total) - (int)blockIdx.x + 1;
-    }
-    p.left -= take; p.pos += take; p.unit += take;
-    if (p.unit == q.units) {
-      p.unit = 0;
-      if (++p.item == q.items) {
-        p.item = 0;
-        if (p.left > 0) do { ++p.seq; q.load(a, p.seq); at = p.seq; } while (q.items == 0 && p.seq + 1 < a.n_seqs);
+    while (p.left > 0) {
+      if (at != p.seq) { q.load(a, p.seq); at = p.seq; }
+      const int kvh = p.item / q.pairs, tile = (p.item - kvh * q.pairs) * a.pair, n_tiles = min(a.pair, q.tiles - tile), w = a.whole ? 1 : n_tiles;
+      const int cost = q.head + w * q.units;
+      const int take = (int)min((long long)(cost - p.off), p.left);
+      // block b belongs to the piece that holds place head + b * w of the item
+      auto block_at = [&](int o) { return o <= q.head ? 0 : (o - q.head + w - 1) >> (w - 1); };
+      const int b0 = block_at(p.off), b1 = block_at(p.off + take);
+      const long long pos = p.pos - p.off;                         // the item's
+      s.q = q; s.seq = p.seq; s.item = p.item; s.kvh = kvh; s.tile = tile; s.n_tiles = n_tiles;
+      p.left -= take; p.pos += take; p.off += take;
+      if (p.off == cost) {
+        p.off = 0;
+        if (++p.item == q.items) {
+          p.item = 0;
+          if (p.left > 0) do { ++p.seq; q.load(a, p.seq); at = p.seq; } while (q.items == 0 && p.seq + 1 < a.n_seqs);
+        }
       }
+      if (b1 == b0) continue;                                      // (the piece ends or begins beside the item's first or last block)
+      s.full = b0 == 0 && b1 == s.q.units;
+      s.lo = s.q.first + (a.whole ? 0 : b0); s.n = a.whole ? s.q.blocks : min(b1 - b0, s.q.blocks - b0);
+      s.slot = 2 * (int)blockIdx.x + (nth++ == 0 ? 0 : 1);
+      s.parts = 0;
+      if (!s.full && b0 == 0) {
+        const long long last = pos + s.q.head + (long long)(s.q.units - 1) * w;      // the place of the item's last block; the piece that holds it is the last one that begins there or before
+        s.parts = ta_piece_of(last, p.total, p.active) - (int)blockIdx.x + 1;
+      }
+      return true;
     }
-    return true;
+    return false;
   }
 };
 
@@ -208,9 +230,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV), kStage = FOLD > 1 ? 32768 : 0;
+  constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV), kStage = 32768;
   uint8_t* sQ = smem;                                             // pair x [128 rows] (64-column halves of 128 B, swizzled)
-  float* s_stage = (float*)(smem + kQ);                           // FOLD > 1: [2 groups][32 columns][96 lanes of the copies]
+  uint8_t* s_stage = smem + a.pair * kQ;                          // FOLD > 1: [2 groups][32 columns][96 lanes of the copies]; else [2 groups][128 rows] of 128 B
   uint8_t* ring = smem + a.pair * kQ + kStage;
   const int slots = min(10, (int)((kTaTiles * 32768 - a.pair * kQ - kStage) / kSlot));
   uint64_t* bars = (uint64_t*)(smem + kTaTiles * 32768);
@@ -222,9 +244,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   int* s_odd = (int*)(tmem_slot + 2);                             // [8] tree nodes of the segment whose value rows are not finite, as bits
   float* s_x = (float*)(bars + 42);                               // [2][128]: what the groups tell each other about a row
-  long long* s_scan = (long long*)s_x;                            // prologue only
-  TaPiece* s_piece = (TaPiece*)(s_x + 256);
-  TaSeg* s_seg = (TaSeg*)(s_piece + 1);                           // [kTaSegs]; n_tiles = 0: no more
+  TaSeg* s_seg = (TaSeg*)(s_x + 256);                           // [kTaSegs]; n_tiles = 0: no more
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -238,57 +258,61 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
   }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   pdl_wait();
-  // ---- the block's piece of the line
-  {
-    const int per = (a.n_seqs + kTaThreads - 1) / kTaThreads;
-    const int i0 = min(a.n_seqs, (int)threadIdx.x * per), i1 = min(a.n_seqs, i0 + per);
+  const uint32_t tmem_base = *tmem_slot;
+  const int G = a.G, tpt = a.tpt;
+
+  if (warp == 11) {
+    // ---------------------------------------------------------------- segments: this block's piece of the line, handed to the other warps
+    const int per = (a.n_seqs + 31) / 32, i0 = min(a.n_seqs, lane * per), i1 = min(a.n_seqs, i0 + per);
+    TaWalk walk;
+    walk.at = -1; walk.nth = 0;
     long long mine = 0;
-    TaSeq q;
-    for (int i = i0; i < i1; ++i) { q.load(a, i); mine += (long long)q.items * q.units; }
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) { TaSeq q; q.load(a, i); mine += q.cost(a); }
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
-    if (lane == 31) s_scan[warp] = incl;
-    if (threadIdx.x == 0) { s_piece->left = 0; s_piece->total = 0; if (a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0); }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    long long total = 0, front = 0;
-    for (int w = 0; w < kTaThreads / 32; ++w) { if (w == warp) front = total; total += s_scan[w]; }
-    const long long excl = front + incl - mine;
-    // at least two units a piece: a part costs more to write and join than a block to work on
-    const int active = (int)min((long long)gridDim.x, a.whole ? total : (total + 1) / 2);
-    if ((int)blockIdx.x < active && mine > 0) {
-      const long long lo = blockIdx.x * total / active, hi = (blockIdx.x + 1ll) * total / active;
-      if (excl <= lo && lo < excl + mine) {
+    const long long total = __shfl_sync(0xffffffffu, incl, 31);
+    // at least two blocks a piece: a part costs more to write and join than a block to work on (and every piece inside an item must get a block of it)
+    const int active = (int)min((long long)gridDim.x, a.whole ? total : max(total / (2 * a.pair), min(total, 1ll)));
+    walk.p.total = total; walk.p.active = active; walk.p.left = 0;
+    if ((int)blockIdx.x < active) {
+      const long long lo = ta_begin(blockIdx.x, total, active), excl = incl - mine;
+      int seq = 0, in_seq = 0;
+      const bool here = excl <= lo && lo < incl;
+      if (here) {
         long long at = excl;
-        int i = i0;
-        for (;; ++i) { q.load(a, i); const long long c = (long long)q.items * q.units; if (lo < at + c) break; at += c; }
-        s_piece->total = total; s_piece->pos = lo; s_piece->left = hi - lo; s_piece->active = active; s_piece->seq = i;
-        s_piece->item = (int)((lo - at) / q.units); s_piece->unit = (int)((lo - at) % q.units);
+        for (seq = i0;; ++seq) { walk.q.load(a, seq); const long long c = walk.q.cost(a); if (lo < at + c) break; at += c; }
+        in_seq = (int)(lo - at);
       }
+      const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+      walk.p.seq = __shfl_sync(0xffffffffu, seq, src);
+      in_seq = __shfl_sync(0xffffffffu, in_seq, src);
+      walk.q.load(a, walk.p.seq);
+      walk.at = walk.p.seq;
+      const TaSeq& q = walk.q;
+      const int head_cost = a.whole ? q.pairs : q.pairs * q.head + q.tiles * q.units;          // a KV head's; all of its pairs but the last cost the same
+      const int kvh = in_seq / head_cost, in_head = in_seq - kvh * head_cost, pair_cost = a.whole ? 1 : q.head + a.pair * q.units;
+      const int pair = min(in_head / pair_cost, q.pairs - 1);
+      walk.p.item = kvh * q.pairs + pair; walk.p.off = in_head - pair * pair_cost;
+      walk.p.pos = lo; walk.p.left = ta_begin(blockIdx.x + 1, total, active) - lo;
     }
-    __syncthreads();
-  }
-  const uint32_t tmem_base = *tmem_slot;
-  const int G = a.hq / a.hkv, tpt = 128 / FOLD / G;
-
-  if (warp == 11) {
-    // ---------------------------------------------------------------- segments
     if (lane == 0) {
-      TaWalk walk;
-      walk.p = *s_piece;
-      walk.at = -1; walk.nth = 0;
+      if (a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0);
       for (int k = 0;; ++k) {
         const int i = k % kTaSegs;
-        if (!mbar_wait(&g_empty[i], ((k / kTaSegs) & 1) ^ 1, abort_flag, a.status, 840, k)) break;
         TaSeg s;
         const bool more = walk.next(a, s);
         if (!more) s.n_tiles = 0;
+        if (!mbar_wait(&g_empty[i], ((k / kTaSegs) & 1) ^ 1, abort_flag, a.status, 840, k)) break;
         s_seg[i] = s;
         mbar_arrive(&g_full[i]);
         if (!more) break;
+        if (s.parts > 0) a.part_of[blockIdx.x] = make_int4(s.parts, s.slot | s.kvh << 16, s.q.begin + s.tile * tpt, s.q.nodes - s.tile * tpt);
       }
     }
   } else if (warp == 8) {
@@ -528,6 +552,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool full = s.full;
       constexpr int kC = DV / 32;
       const int c0 = !two && g == 1 ? kC / 2 : 0, c1 = !two && g == 0 ? kC / 2 : kC;
+      if constexpr (FOLD == 1) {
+        if (!two) bar256_and(true);                                            // (the other group has read the sums)
+        reinterpret_cast<int*>(s_x)[g * 128 + r] = !live ? -1 : full ? tok * a.hq + head : (int)prow;         // where the row goes
+      }
       for (int c = c0; c < c1; ++c) {
         float o[32];
         __syncwarp();
@@ -543,7 +571,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
         if constexpr (FOLD > 1) {                                              // the copies' shares go to the first one's threads
-          float* st = s_stage + g * 32 * 96 + (r - 128 / FOLD);
+          float* st = (float*)s_stage + g * 32 * 96 + (r - 128 / FOLD);
           if (fold > 0) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) st[i * 96] = o[i];
@@ -552,41 +580,78 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (fold == 0) {
 #pragma unroll
             for (int f = 1; f < FOLD; ++f) {
-              const float* sf = s_stage + g * 32 * 96 + (f - 1) * (128 / FOLD) + rr;
+              const float* sf = (const float*)s_stage + g * 32 * 96 + (f - 1) * (128 / FOLD) + rr;
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] += sf[i * 96];
             }
           }
           bar_group(g);
         }
-        if (ok && live && fold == 0) {
-          if (any_odd) {
-            for (int x = 0; x < min(256, a.words * 64); ++x) {
-              if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
-              const int at = ctx + x;
-              const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
-              if (slot < 0 || slot >= a.num_slots) continue;
-              const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
+        if (any_odd && ok && live && fold == 0) {
+          for (int x = 0; x < min(256, a.words * 64); ++x) {
+            if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
+            const int at = ctx + x;
+            const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
+            if (slot < 0 || slot >= a.num_slots) continue;
+            const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
+            for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
+          }
+        }
+        if constexpr (FOLD > 1) {                                              // few rows: a thread stores its own
+          if (ok && live && fold == 0) {
+            if (full) {
+              __nv_bfloat16* dst = a.out + ((size_t)tok * a.hq + head) * DV + c * 32;
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
+              store32(dst, w);
+              store32(dst + 16, w + 8);
+            } else {
+              float* dst = a.part_o + prow * DV + c * 32;
+#pragma unroll
+              for (int v = 0; v < 4; ++v) store32(dst + v * 8, reinterpret_cast<const uint32_t*>(o) + v * 8);
             }
           }
+        } else {
+          // Through shared memory, so that eight lanes store 128 bytes of a row (a lane per row: 32 lines a store, 4000 to 8000 cycles a segment; so: 1300).
+          // 128 bytes per row and turn: 32 columns of a part, or 64 of the output in two turns.
+          uint8_t* mine = s_stage + g * 16384 + r * 128;
+          const int half = full ? (c - c0) & 1 : 0;
           if (full) {
-            __nv_bfloat16* dst = a.out + ((size_t)tok * a.hq + head) * DV + c * 32;
-            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
-            store32(dst, w);
-            store32(dst + 16, w + 8);
+            for (int v = 0; v < 4; ++v)
+              *reinterpret_cast<uint4*>(mine + (((half * 4 + v) ^ (r & 7)) << 4)) =
+                  make_uint4(pack_bf16x2(o[v * 8], o[v * 8 + 1]), pack_bf16x2(o[v * 8 + 2], o[v * 8 + 3]), pack_bf16x2(o[v * 8 + 4], o[v * 8 + 5]),
+                             pack_bf16x2(o[v * 8 + 6], o[v * 8 + 7]));
           } else {
-            float* dst = a.part_o + prow * DV + c * 32;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) store32(dst + v * 8, reinterpret_cast<const uint32_t*>(o) + v * 8);
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<float4*>(mine + ((v ^ (r & 7)) << 4)) = make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+          }
+          const bool last = c == c1 - 1;
+          if (!full || half == 1 || last) {
+            const int chunk = r & 7, cols = full && half == 0 ? 4 : 8;         // (DV = 64 and one tile: 32 columns a group)
+            bar_group(g);
+            int to[8];
+            uint4 v[8];
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+              const int row = it * 16 + (r >> 3);
+              to[it] = reinterpret_cast<const int*>(s_x)[g * 128 + row];
+              v[it] = *reinterpret_cast<const uint4*>(s_stage + g * 16384 + row * 128 + ((chunk ^ (row & 7)) << 4));
+            }
+            if (ok && chunk < cols) {
+              char* base = full ? (char*)(a.out + (c - half) * 32 + chunk * 8) : (char*)(a.part_o + c * 32 + chunk * 4);
+              const size_t pitch = full ? DV * 2 : DV * 4;
+#pragma unroll
+              for (int it = 0; it < 8; ++it) if (to[it] >= 0) *reinterpret_cast<uint4*>(base + to[it] * pitch) = v[it];
+            }
+            bar_group(g);
           }
         }
       }
       if (live && fold == 0 && !full && c0 == 0) a.part_lse[prow] = lse;
-      if (threadIdx.x == 0 && s.parts > 0) a.part_of[blockIdx.x] = make_int4(s.seq, s.item, s.parts, s.slot);
       if (any_odd) {
         bar256_and(true);
         if (threadIdx.x < 8) s_odd[threadIdx.x] = 0;
@@ -607,52 +672,62 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp == 9) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-// Joins the parts of the items that were cut: out = sum_i 2^(lse_i - max) O_i / sum_i 2^(lse_i - max), in the order of the parts.  One warp per row.
+// Joins the parts of the items that were cut: out = sum_i 2^(lse_i - max) O_i / sum_i 2^(lse_i - max), in the order of the parts.  One warp per row.  (Four rows to a warp
+// and one load after the other: 9 to 17 us.)
 template <int DV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 8)
 tree_join_kernel(const TreeAttnArgs a) {
   pdl_wait();
   pdl_trigger();
   const int4 of = a.part_of[blockIdx.x];
-  if (of.z <= 0) return;
-  TaSeq q;
-  q.load(a, of.x);
-  const int G = a.hq / a.hkv, tpt = 128 / a.fold / G, pairs = q.items / a.hkv;
-  const int kvh = of.y / pairs, tile = (of.y - kvh * pairs) * a.pair;
-  const int lane = threadIdx.x & 31;
-  const int per_block = a.pair * 128 / (int)gridDim.y;
-  for (int k = threadIdx.x >> 5; k < per_block; k += 8) {
-    const int row = blockIdx.y * per_block + k;                                // of the item
-    const int r = row & 127, t_local = r / G, node = (tile + (row >> 7)) * tpt + t_local;
-    if (t_local >= tpt || node >= q.nodes) continue;
-    auto at = [&](int i) { return (long)(i == 0 ? of.w : 2 * ((int)blockIdx.x + i)) * (a.pair * 128) + row; };
-    float top = -INFINITY;
-    for (int i = lane; i < of.z; i += 32) top = fmaxf(top, a.part_lse[at(i)]);
-    top = warp_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    constexpr int kV = DV / 32;
-    float acc[kV], den = 0.f;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);          // of the item
+  const int r = row & 127, t_local = r / a.G, node = (row >> 7) * a.tpt + t_local;
+  if (of.x <= 0 || t_local >= a.tpt || node >= of.w) return;
+  const int slot = of.y & 0xffff, kvh = of.y >> 16;
+  constexpr int kV = DV / 32;
+  auto at = [&](int i) { return (size_t)(i == 0 ? slot : 2 * ((int)blockIdx.x + i)) * (a.pair * 128) + row; };
+  // four parts at a time, all their loads in flight
+  float top = -INFINITY, acc[kV], den = 0.f;
 #pragma unroll
-    for (int v = 0; v < kV; ++v) acc[v] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < of.z; ++i) {
-      const float lse = a.part_lse[at(i)];
-      const float w = exp2f(lse - ref);
-      const float* o = a.part_o + at(i) * DV + lane * kV;
+  for (int v = 0; v < kV; ++v) acc[v] = 0.f;
+  for (int i0 = 0; i0 < of.x; i0 += 4) {
+    float lse[4], o[4][kV];
 #pragma unroll
-      for (int v = 0; v < kV; ++v) acc[v] += lse == -INFINITY ? 0.f : w * o[v];
+    for (int k = 0; k < 4; ++k) {
+      lse[k] = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) o[k][v] = 0.f;
+      if (i0 + k >= of.x) continue;
+      lse[k] = a.part_lse[at(i0 + k)];
+      const float* p = a.part_o + at(i0 + k) * DV + lane * kV;
+      if constexpr (kV == 4) { const float4 x = *reinterpret_cast<const float4*>(p); o[k][0] = x.x; o[k][1] = x.y; o[k][2] = x.z; o[k][3] = x.w; }
+      else { const float2 x = *reinterpret_cast<const float2*>(p); o[k][0] = x.x; o[k][1] = x.y; }
+    }
+    float m = top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fmaxf(m, lse[k]);
+    const float ref = m == -INFINITY ? 0.f : m, scale = exp2f(top - ref);      // (nothing so far: 0)
+    top = m;
+#pragma unroll
+    for (int v = 0; v < kV; ++v) acc[v] *= scale;
+    den *= scale;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = exp2f(lse[k] - ref);
+#pragma unroll
+      for (int v = 0; v < kV; ++v) acc[v] += lse[k] == -INFINITY ? 0.f : w * o[k][v];
       den += w;
     }
-    const float inv = den == 0.f ? 0.f : 1.0f / den;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((size_t)(q.begin + node) * a.hq + kvh * G + (r - t_local * G)) * DV + lane * kV);
-#pragma unroll
-    for (int v = 0; v < kV / 2; ++v) dst[v] = pack_bf16x2(acc[2 * v] * inv, acc[2 * v + 1] * inv);
   }
+  const float inv = den == 0.f ? 0.f : 1.0f / den;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ((size_t)(of.z + node) * a.hq + kvh * a.G + (r - t_local * a.G)) * DV + lane * kV);
+#pragma unroll
+  for (int v = 0; v < kV / 2; ++v) dst[v] = pack_bf16x2(acc[2 * v] * inv, acc[2 * v + 1] * inv);
 }
 
 template <int DK, int DV, int FOLD>
 static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const void* v_cache, TreeAttnArgs a, int grid, cudaStream_t stream) {
-  const int G = a.hq / a.hkv, tpt = 128 / FOLD / G;
+  const int G = a.G, tpt = a.tpt;
   CUtensorMap tmQ, tmK, tmV;
   {
     uint64_t dims[3] = {DK, (uint64_t)a.hq, (uint64_t)a.total_tokens};
@@ -677,7 +752,7 @@ static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const
   launch_k(tree_attn_kernel<DK, DV, FOLD>, grid, kTaThreads, kTaSmem, stream, tmQ, tmK, tmV, a);
   GB_CUDA_OK(cudaGetLastError());
   if (!a.whole) {
-    launch_k(tree_join_kernel<DV>, dim3(grid, 4 * a.pair), 256, 0, stream, a);
+    launch_k(tree_join_kernel<DV>, dim3(grid, a.pair * 128 / a.fold / 8), 256, 0, stream, a);
     GB_CUDA_OK(cudaGetLastError());
   }
   return 0;
@@ -714,13 +789,15 @@ GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const voi
   if ((dk != 64 && dk != 128) || (dv != 64 && dv != 128)) return fail("tree_attn: heads of 64 or 128 columns%s");
   if (hq < 1 || hkv < 1 || hq % hkv || hq / hkv > 128) return fail("tree_attn: bad head counts%s");
   if (page_size < 8 || page_size > 128 || 128 % page_size) return fail("tree_attn: page_size must be 8..128 and divide 128%s");
-  if (max_nodes < 1 || words < 1 || max_pages < 0 || window < 0 || num_slots < 1) return fail("tree_attn: bad sizes%s");
+  if (max_nodes < 1 || words < 1 || max_pages < 0 || window < 0 || num_slots < 1 || hkv > 32767) return fail("tree_attn: bad sizes%s");
   if (window > 0 && positions == nullptr) return fail("tree_attn: a window needs the nodes' positions%s");
   TreeAttnArgs a;
   memset(&a, 0, sizeof(a));
   const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &a.pair, &a.fold, &a.whole);
   a.cu_q = cu_q; a.kv_len = kv_len; a.block_table = block_table; a.mask = (const unsigned long long*)mask; a.positions = positions; a.n_seqs = n_seqs;
   a.max_pages = max_pages; a.page_size = page_size; a.words = words; a.window = window; a.hq = hq; a.hkv = hkv; a.total_tokens = tokens;
+  a.head = a.pair == 2 ? 6 : 2;
+  a.G = hq / hkv; a.tpt = 128 / a.fold / a.G;
   a.num_slots = num_slots; a.out = (__nv_bfloat16*)out; a.v_cache = (const __nv_bfloat16*)v_cache; a.status = (KernelStatus*)status;
   if (!a.whole) {
     a.part_of = (int4*)workspace;
