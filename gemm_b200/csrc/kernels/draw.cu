@@ -1041,9 +1041,9 @@ static int draw_launch(DrawArgs a, cudaStream_t stream) {
   static size_t attr[64];
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
-  if (smem > attr[dev & 63]) {
+  if (dev > 63 || smem > attr[dev]) {
     GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attr[dev & 63] = smem;
+    if (dev < 64) attr[dev] = smem;
   }
   launch_k_cluster(draw_kernel<T>, (unsigned)(a.rows * c), kDrThreads, smem, stream, (unsigned)c, a);
   GB_CUDA_OK(cudaGetLastError());

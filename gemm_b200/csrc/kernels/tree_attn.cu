@@ -147,6 +147,11 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 // 128 threads of softmax group g.
 __device__ __forceinline__ void bar_group(int g) { asm volatile("bar.sync %0, 128;" :: "r"(3 + g) : "memory"); }
 
+// Two floats in a 64-bit register: one issue slot adds both.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 // 64 bytes of a row in two stores.
 __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
@@ -188,6 +193,8 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
     }
   }
   const float ref = m == -INFINITY ? 0.f : m;
+  const uint64_t ref2 = pair2(-ref, -ref);
+  uint64_t rs2[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};
   float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < NC; c += CH) {
@@ -203,8 +210,16 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
     uint32_t pk[CH / 2];
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
-      const float p0 = fast_exp2(sv[2 * i] - ref), p1 = fast_exp2(sv[2 * i + 1] - ref);
-      rs[i & 1] += p0; rs[2 + (i & 1)] += p1;
+      // (in pairs where a thread has all 128 columns: 3% on wide trees; with folded rows it costs as much)
+      float p0, p1;
+      if constexpr (FOLD == 1) {
+        unpair2(add2(pair2(sv[2 * i], sv[2 * i + 1]), ref2), p0, p1);
+        p0 = fast_exp2(p0); p1 = fast_exp2(p1);
+        rs2[i & 1] = add2(rs2[i & 1], pair2(p0, p1));
+      } else {
+        p0 = fast_exp2(sv[2 * i] - ref); p1 = fast_exp2(sv[2 * i + 1] - ref);
+        rs[i & 1] += p0; rs[2 + (i & 1)] += p1;
+      }
       pk[i] = pack_bf16x2(p0, p1);
     }
     if constexpr (FOLD == 4) tmem_st_x16(s_t + fold * 16, pk);
@@ -221,6 +236,7 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
       else tmem_st_x32(s_t + x * 32, z);
     }
   }
+  if constexpr (FOLD == 1) unpair2(add2(rs2[0], rs2[1]), rs[0], rs[2]);
   l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
   tc_wait_st();
 }
@@ -462,7 +478,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (tail) see[c] = (see[c] | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
           }
         }
-        ok = mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b));        // (a warp leaves as one)
         if (!ok) break;
         s_ph ^= 1;
         if (tail && (!two || g == 0)) {
@@ -470,7 +486,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // finite is taken out, noted, and put back at the end for the rows that see it.  (Behind the wait for S, which tells that the products in front are done:
           // in front of it the place's tile before this one may still be on its way, and its barrier two phases from the one waited for.)
           const uint32_t t = t0 + 2 * b + 1;
-          ok = mbar_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b);
+          ok = __all_sync(0xffffffffu, mbar_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b));
           if (ok && kv0 + r >= min(ctx, len)) {
             uint8_t* row = ring + (t % slots) * kSlot + r * 128;
             bool odd = false;
@@ -745,9 +761,9 @@ static int tree_attn_launch(const void* q, long q_ts, const void* k_cache, const
   static bool attr[64];
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
-  if (!attr[dev & 63]) {
+  if (dev > 63 || !attr[dev]) {
     GB_CUDA_OK(cudaFuncSetAttribute(tree_attn_kernel<DK, DV, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTaSmem));
-    attr[dev & 63] = true;
+    if (dev < 64) attr[dev] = true;
   }
   launch_k(tree_attn_kernel<DK, DV, FOLD>, grid, kTaThreads, kTaSmem, stream, tmQ, tmK, tmV, a);
   GB_CUDA_OK(cudaGetLastError());

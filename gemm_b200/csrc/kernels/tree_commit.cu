@@ -120,8 +120,8 @@ tree_commit_kernel(const __grid_constant__ TreeCommitArgs a) {
 
 using namespace gb;
 
-// caches[i]: num_slots rows of row_bytes[i] bytes (host arrays).  No caches: the walk alone.
-GB_API int gb_tree_commit(const void* const* caches, const int* row_bytes, int n_caches, long num_slots, const int* tokens, const int* parents, const int* sampled,
+// caches[i]: num_slots rows, bytes[i] in all (host arrays; a cache without bytes is passed over).  No caches: the walk alone.
+GB_API int gb_tree_commit(const void* const* caches, const long long* bytes, int n_caches, long num_slots, const int* tokens, const int* parents, const int* sampled,
                           const int* cu_q, const int* kv_len, const int* block_table, int max_pages, int page_size, int n_seqs, int total_tokens, int max_nodes,
                           int* count, int* path, int* next_token, int* new_len, cudaStream_t stream) {
   if (n_seqs <= 0) return 0;
@@ -129,9 +129,16 @@ GB_API int gb_tree_commit(const void* const* caches, const int* row_bytes, int n
   TreeCommitArgs a;
   int done = 0;
   do {
-    memset(&a, 0, sizeof(a));
-    a.n_caches = std::min(n_caches - done, kTcCaches);
-    for (int i = 0; i < a.n_caches; ++i) { a.cache[i] = const_cast<void*>(caches[done + i]); a.row_bytes[i] = row_bytes[done + i]; }
+    a.n_caches = 0;
+    a.count = a.path = a.next_token = a.new_len = nullptr;
+    const int n_here = std::min(n_caches - done, kTcCaches);
+    for (int i = 0; i < n_here; ++i) {
+      const long long row = num_slots > 0 ? bytes[done + i] / num_slots : 0;
+      if (row <= 0) continue;
+      if (row > (1 << 30)) return fail("tree_commit: rows of at most 2^30 bytes%s");
+      a.cache[a.n_caches] = const_cast<void*>(caches[done + i]);
+      a.row_bytes[a.n_caches++] = (int)row;
+    }
     // enough blocks to fill the GPU a few times over, no more walks than that
     a.per_block = std::max(1, (int)((long)a.n_caches * n_seqs / (16l * sm_count())));
     a.tokens = tokens; a.parents = parents; a.sampled = sampled; a.cu_q = cu_q; a.kv_len = kv_len; a.block_table = block_table; a.max_pages = max_pages;
@@ -139,7 +146,7 @@ GB_API int gb_tree_commit(const void* const* caches, const int* row_bytes, int n
     if (done == 0) { a.count = count; a.path = path; a.next_token = next_token; a.new_len = new_len; }
     launch_k(tree_commit_kernel, dim3(std::max(1, (a.n_caches + a.per_block - 1) / a.per_block), n_seqs), kTcThreads, 0, stream, a);
     GB_CUDA_OK(cudaGetLastError());
-    done += a.n_caches;
+    done += n_here;
   } while (done < n_caches);
   return 0;
 }

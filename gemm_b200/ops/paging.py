@@ -1,28 +1,21 @@
 """Tables of a forward pass over a paged KV cache, built on the GPU from the lengths of its requests (csrc/kernels/paging.cu)."""
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
 
 from .. import _native
 
-_c, _i = ctypes.c_void_p, ctypes.c_int
-
 MAX_SEQS = 8192
 MAX_NODES = 256                   # nodes of a tree of drafted tokens: four 64-bit words of mask
 
 
-def _p(t):
-    return _c(t.data_ptr()) if t is not None else _c(0)
-
-
-def check_int32(device, **tensors) -> None:
+def check_int32(device, names: str, *tensors) -> None:
     """Raise ``ValueError`` unless every tensor is a contiguous int32 one on ``device``."""
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name}: a contiguous int32 tensor on {device} is needed, not {t.dtype} on {t.device}")
+    for i, t in enumerate(tensors):
+        if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError(f"{names.split()[i]}: a contiguous int32 tensor on {device} is needed, not {t.dtype} on {t.device}")
 
 
 class BatchTables(NamedTuple):
@@ -49,29 +42,32 @@ def batch_tables(q_lens: torch.Tensor, ctx_lens: torch.Tensor, page_ptr: torch.T
     which comes in front of it; -1 at a root.  The slot of a node still goes by its index, its position is ``ctx + depth``, and ``mask`` has a bit for
     each of its ancestors and for itself: what ``ops.tree.tree_attention`` takes."""
     b, dev = q_lens.numel(), q_lens.device
-    check_int32(dev, q_lens=q_lens, ctx_lens=ctx_lens, page_ptr=page_ptr, pages=pages)
+    check_int32(dev, "q_lens ctx_lens page_ptr pages", q_lens, ctx_lens, page_ptr, pages)
     if ctx_lens.numel() != b or page_ptr.numel() != b + 1:
         raise ValueError(f"{b} lengths go with as many context lengths and one more page pointer, not {ctx_lens.numel()} and {page_ptr.numel()}")
     if b > MAX_SEQS or page_size < 1 or total_tokens < 0 or max_pages < 0:
         raise ValueError(f"batch_tables: at most {MAX_SEQS} sequences, pages of at least one token, no negative sizes")
     words = 0
     if parents is not None:
-        check_int32(dev, parents=parents)
+        check_int32(dev, "parents", parents)
         if parents.numel() != total_tokens or not 1 <= max_nodes <= MAX_NODES:
             raise ValueError(f"a parent for each of the {total_tokens} tokens is needed, and trees of 1 to {MAX_NODES} nodes")
         words = mask_words(max_nodes)
     if dev.type != "cuda":
         return batch_tables_ref(q_lens, ctx_lens, page_ptr, pages, page_size, total_tokens, max_pages, parents, max_nodes)
     with _native.on_device(dev):
-        i32 = dict(dtype=torch.int32, device=dev)
-        cu, kv, pos, slots = (torch.empty(n, **i32) for n in (b + 1, b, total_tokens, total_tokens))
-        table = torch.empty(b, max_pages, **i32)
+        # one buffer for all that is int32, every table on a 16-byte boundary
+        sizes = []
+        for n in (b + 1, b, total_tokens, total_tokens, b * max_pages):
+            sizes += (n, -n % 4)
+        cu, _, kv, _, pos, _, slots, _, table, _ = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
         mask = torch.empty(total_tokens, words, dtype=torch.int64, device=dev) if words else None
-        rc = _native.cuda().gb_batch_tables(_p(q_lens), _p(ctx_lens), _p(page_ptr), _p(pages), _i(pages.numel()), _i(b), _i(page_size), _i(total_tokens),
-                                            _i(max_pages), _p(parents), _i(max_nodes), _p(cu), _p(kv), _p(pos), _p(slots), _p(table), _p(mask),
-                                            _c(_native.stream()))
+        rc = _native.entry("gb_batch_tables", "ppppiiiiipippppppp")(
+            q_lens.data_ptr(), ctx_lens.data_ptr(), page_ptr.data_ptr(), pages.data_ptr(), pages.numel(), b, page_size, total_tokens, max_pages,
+            parents.data_ptr() if words else None, max_nodes, cu.data_ptr(), kv.data_ptr(), pos.data_ptr(), slots.data_ptr(), table.data_ptr(),
+            mask.data_ptr() if words else None, _native.stream())
         _native.check(rc, "gb_batch_tables")
-    return BatchTables(cu, kv, pos, slots, table, mask)
+    return BatchTables(cu, kv, pos, slots, table.view(b, max_pages), mask)
 
 
 def batch_tables_ref(q_lens, ctx_lens, page_ptr, pages, page_size, total_tokens, max_pages, parents=None, max_nodes=0) -> BatchTables:

@@ -96,7 +96,7 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
     least one); of these the ids with at least ``min_p`` times the largest probability.  The draw is the first id, in id order, at which the kept probability so
     far exceeds ``uniform`` of it all.  ``temperature <= 0``: the lowest id of the largest logit.  NaN counts as -inf; a row without any logit above -inf answers
     id 0 with logarithm -inf.  Probabilities below 2^-45 of the largest count as zero."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] < 1:
+    if logits.dim() != 2 or (logits.dtype is not torch.float32 and logits.dtype is not torch.bfloat16) or logits.shape[1] < 1:
         raise ValueError("logits: a tensor [B, V] in f32 or bf16 is needed")
     b, v = logits.shape
     dev = logits.device
@@ -108,11 +108,11 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
     for name, x, dt, none in (("temperature", temperature, torch.float32, 1.0), ("top_k", top_k, torch.int32, 0), ("top_p", top_p, torch.float32, 1.0),
                               ("min_p", min_p, torch.float32, 0.0)):
         if torch.is_tensor(x):
-            if x.dtype != dt or x.shape != (b,) or x.device != dev or not x.is_contiguous():
+            if x.dtype is not dt or x.shape != (b,) or x.device != dev or not x.is_contiguous():
                 raise ValueError(f"{name}: a contiguous {dt} tensor [{b}] beside the logits is needed")
             given.append((x, none))
         else:
-            given.append((None, none if x is None else x))
+            given.append((None, none if x is None else type(none)(x)))
     if not logits.is_cuda:
         token, logprob = draw_ref(logits, uniform, *(x if x is not None else y for x, y in given))
         return (token, logprob) if want_logprob else token
@@ -120,8 +120,10 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
     with _native.on_device(dev):
         out = torch.empty(b, dtype=torch.int32, device=dev)
         logprob = torch.empty(b, dtype=torch.float32, device=dev) if want_logprob else None
-        rc = _native.cuda().gb_draw(_p(logits), _l(logits.stride(0) if b > 1 else v), _i(0 if logits.dtype == torch.float32 else 1), _i(b), _i(v), _p(uniform), _p(t),
-                                    _f(t0), _p(k), _i(k0), _p(p), _f(p0), _p(m), _f(m0), _p(out), _p(logprob), _c(_native.status_ptr()), _c(_native.stream()))
+        ptr = lambda x: x.data_ptr() if x is not None else None                # noqa: E731
+        rc = _native.entry("gb_draw", "pliiipp" + "fpipfpf" + "pppp")(
+            logits.data_ptr(), logits.stride(0) if b > 1 else v, 0 if logits.dtype is torch.float32 else 1, b, v, uniform.data_ptr(), ptr(t), t0, ptr(k), k0, ptr(p),
+            p0, ptr(m), m0, out.data_ptr(), ptr(logprob), _native.status_ptr(), _native.stream())
         _native.check(rc, "gb_draw", n=1 if b else 0)
     return (out, logprob) if want_logprob else out
 

@@ -7,8 +7,9 @@ parent, which has a lower index.  Node i is cached at place ``ctx + i`` of the s
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
+from operator import attrgetter
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -16,14 +17,8 @@ import torch
 from .. import _native
 from .paging import MAX_NODES, check_int32
 
-_c, _i, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
-
-
-def _p(t):
-    return _c(t.data_ptr()) if t is not None else _c(0)
-
-
 _TILE, _PAGES = (64, 128), (8, 16, 32, 64, 128)
+_nbytes = attrgetter("nbytes")
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor,
@@ -36,32 +31,34 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not finite."""
     t, hq, dk = q.shape
     slots, hkv, dv = v_cache.shape
-    dev = q.device
+    dev, dtype = q.device, q.dtype
     b = kv_len.numel()
-    if q.stride(2) != 1 or q.stride(1) != dk or (t > 1 and q.stride(0) < hq * dk):
+    q_ts, q_hs, q_es = q.stride()
+    if q_es != 1 or q_hs != dk or (t > 1 and q_ts < hq * dk):
         raise ValueError("q: the heads of a token lie one after the other")
-    if k_cache.shape != (slots, hkv, dk) or not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.dtype != v_cache.dtype or k_cache.dtype != q.dtype:
+    if k_cache.shape != (slots, hkv, dk) or not (k_cache.is_contiguous() and v_cache.is_contiguous()) or v_cache.dtype is not dtype or k_cache.dtype is not dtype:
         raise ValueError("contiguous caches of the same slots, heads and type as the queries are needed")
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"tree_attention takes bf16 or f32, not {q.dtype}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise ValueError(f"tree_attention takes bf16 or f32, not {dtype}")
     if hkv < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads do not share {hkv} KV heads evenly")
-    check_int32(dev, cu_q=cu_q, kv_len=kv_len, block_table=block_table)
+    check_int32(dev, "cu_q kv_len block_table", cu_q, kv_len, block_table)
     if cu_q.numel() != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b or page_size < 1:
         raise ValueError("cu_q, kv_len and block_table name different numbers of sequences")
-    if k_cache.device != dev or v_cache.device != dev or mask.device != dev or mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != t or not mask.is_contiguous():
+    if mask.dtype is not torch.int64 or mask.dim() != 2 or not mask.is_contiguous() or mask.device != dev or k_cache.device != dev or v_cache.device != dev:
         raise ValueError("mask: a contiguous int64 tensor [T, words] beside the queries is needed")
-    if not 1 <= max_nodes <= MAX_NODES or mask.shape[1] * 64 < max_nodes or mask.shape[1] > MAX_NODES // 64:
-        raise ValueError(f"trees of 1 to {MAX_NODES} nodes with a mask bit each, not {max_nodes} in {mask.shape[1]} words")
+    rows, words = mask.shape
+    if rows != t or not 1 <= max_nodes <= MAX_NODES or words * 64 < max_nodes or words > MAX_NODES // 64:
+        raise ValueError(f"trees of 1 to {MAX_NODES} nodes with a mask bit each, not {max_nodes} in a mask [{rows}, {words}]")
     if window < 0 or (window > 0 and positions is None):
         raise ValueError("a window needs the nodes' positions")
     if positions is not None:
-        check_int32(dev, positions=positions)
+        check_int32(dev, "positions", positions)
         if positions.numel() != t:
             raise ValueError("positions: one for each node")
     if out is None:
-        out = torch.empty(t, hq, dv, dtype=q.dtype, device=dev)
-    elif out.shape != (t, hq, dv) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        out = torch.empty(t, hq, dv, dtype=dtype, device=dev)
+    elif out.shape != (t, hq, dv) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out: a contiguous tensor [{t}, {hq}, {dv}] of the queries' type is needed")
     elif out.data_ptr() % 32:
         raise ValueError("out: a 32-byte boundary is needed")
@@ -69,23 +66,25 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         return tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window, positions, out)
     if t == 0 or b == 0:
         return out
-    lib = _native.cuda()
-    # the tcgen05 kernel's forms: its tiles hold 64 or 128 columns, 128 rows and whole pages, and TMA wants 16-byte boundaries
-    if q.dtype == torch.bfloat16 and dk in _TILE and dv in _TILE and page_size in _PAGES and hq // hkv <= 128 and q.stride(0) % 8 == 0 \
-            and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
-        with _native.on_device(dev):
-            cols = block_table.shape[1]
-            work = torch.empty(lib.gb_tree_attn_workspace(_i(b), _i(cols), _i(page_size), _i(max_nodes), _i(hq), _i(hkv), _i(dv)), dtype=torch.float32, device=dev)
-            rc = lib.gb_tree_attn(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _p(work), _p(cu_q), _p(kv_len), _p(block_table), _i(cols),
-                                  _i(page_size), _p(mask), _i(mask.shape[1]), _p(positions), _i(b), _l(slots), _i(t), _i(max_nodes), _i(hq), _i(hkv), _i(dk), _i(dv),
-                                  _i(window), _c(_native.status_ptr()), _c(_native.stream()))
-            _native.check(rc, "gb_tree_attn", n=1 if work.numel() <= 4 else 2)
-        return out
+    if slots == 0:
+        raise ValueError("an empty cache")
+    cols = block_table.shape[1]
+    qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    pos = positions.data_ptr() if positions is not None else None
     with _native.on_device(dev):
-        rc = lib.gb_tree_any(_p(q), _l(q.stride(0)), _p(k_cache), _p(v_cache), _p(out), _i(int(q.dtype == torch.float32)), _p(cu_q), _p(kv_len),
-                                        _p(block_table), _i(block_table.shape[1]), _i(page_size), _p(mask), _i(mask.shape[1]), _p(positions), _i(b), _l(slots),
-                                        _i(t), _i(hq), _i(hkv), _i(dk), _i(dv), _i(window), _c(_native.stream()))
-        _native.check(rc, "gb_tree_any")
+        # the tcgen05 kernel's forms: its tiles hold 64 or 128 columns, 128 rows and whole pages, and TMA wants 16-byte boundaries
+        if dtype is torch.bfloat16 and dk in _TILE and dv in _TILE and page_size in _PAGES and hq // hkv <= 128 and not (q_ts & 7 or (qp | kp | vp) & 15):
+            n = _native.entry("gb_tree_attn_workspace", "iiiiiii")(b, cols, page_size, max_nodes, hq, hkv, dv)
+            work = torch.empty(n, dtype=torch.float32, device=dev)
+            rc = _native.entry("gb_tree_attn", "plpppppppiipipiliiiiiiipp")(
+                qp, q_ts, kp, vp, out.data_ptr(), work.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), cols, page_size, mask.data_ptr(), words, pos,
+                b, slots, t, max_nodes, hq, hkv, dk, dv, window, _native.status_ptr(), _native.stream())
+            _native.check(rc, "gb_tree_attn", n=1 if n <= 4 else 2)
+        else:
+            rc = _native.entry("gb_tree_any", "plpppippp" + "iipipiliiiiiip")(
+                qp, q_ts, kp, vp, out.data_ptr(), int(dtype is torch.float32), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), cols, page_size,
+                mask.data_ptr(), words, pos, b, slots, t, hq, hkv, dk, dv, window, _native.stream())
+            _native.check(rc, "gb_tree_any")
     return out
 
 
@@ -135,31 +134,29 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
     ``ctx, ctx + 1, ...``, in place.  ``tokens`` / ``parents`` / ``sampled``: int32 ``[T]``; the lengths and tables are those of the verifying pass (``kv_len``
     includes the tree).  No caches: the walk alone."""
     dev, t, b = tokens.device, tokens.numel(), kv_len.numel()
-    check_int32(dev, tokens=tokens, parents=parents, sampled=sampled, cu_q=cu_q, kv_len=kv_len, block_table=block_table)
+    check_int32(dev, "tokens parents sampled cu_q kv_len block_table", tokens, parents, sampled, cu_q, kv_len, block_table)
     if parents.numel() != t or sampled.numel() != t:
         raise ValueError("tokens, parents and sampled name different numbers of nodes")
     if cu_q.numel() != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b or page_size < 1 or b > 65535:
         raise ValueError("cu_q, kv_len and block_table name different numbers of sequences")
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"trees of 1 to {MAX_NODES} nodes, not {max_nodes}")
-    slots = caches[0].shape[0] if len(caches) else 0
-    for c in caches:
-        if not c.is_contiguous() or c.device != dev or c.shape[0] != slots:
-            raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
+    # (two caches a layer: by maps over the list, a loop of Python steps took 45 us of them)
+    slots = len(caches[0]) if len(caches) else 0
+    on = dev.index if dev.type == "cuda" else -1
+    if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or set(map(len, caches)) - {slots}:
+        raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
     if dev.type != "cuda":
         return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)
     with _native.on_device(dev):
-        i32 = dict(dtype=torch.int32, device=dev)
-        got = Accepted(torch.empty(b, **i32), torch.empty(b, max_nodes, **i32), torch.empty(b, **i32), torch.empty(b, **i32))
-        live = [c for c in caches if c.numel()]
-        n = len(live)
-        ptrs = (ctypes.c_void_p * max(1, n))(*[c.data_ptr() for c in live])
-        rows = (ctypes.c_int * max(1, n))(*[c.numel() // slots * c.element_size() for c in live])
-        rc = _native.cuda().gb_tree_commit(ptrs, rows, _i(n), _l(slots), _p(tokens), _p(parents), _p(sampled), _p(cu_q), _p(kv_len), _p(block_table),
-                                           _i(block_table.shape[1]), _i(page_size), _i(b), _i(t), _i(max_nodes), _p(got.count), _p(got.path),
-                                           _p(got.next_token), _p(got.kv_len), _c(_native.stream()))
-        _native.check(rc, "gb_tree_commit", n=max(1, (n + 223) // 224) if b else 0)
-    return got
+        count, nxt, new, path = torch.empty(b * (3 + max_nodes), dtype=torch.int32, device=dev).split((b, b, b, b * max_nodes))
+        ptrs, sizes = array("Q", map(torch.Tensor.data_ptr, caches)), array("q", map(_nbytes, caches))
+        rc = _native.entry("gb_tree_commit", "ppilppppppiiiiippppp")(
+            ptrs.buffer_info()[0], sizes.buffer_info()[0], len(ptrs), slots, tokens.data_ptr(), parents.data_ptr(), sampled.data_ptr(), cu_q.data_ptr(),
+            kv_len.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, b, t, max_nodes, count.data_ptr(), path.data_ptr(), nxt.data_ptr(),
+            new.data_ptr(), _native.stream())
+        _native.check(rc, "gb_tree_commit", n=max(1, (len(ptrs) + 223) // 224) if b else 0)
+    return Accepted(count, path.view(b, max_nodes), nxt, new)
 
 
 def tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes) -> Accepted:
