@@ -153,7 +153,7 @@ def cmd_generate(args):
         return _generate_with_audio(args)
     llm = _load_llm(args)
     prompts = args.prompt or ["Hello"]
-    sp = SamplingParams(max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, seed=args.seed)
+    sp = SamplingParams(max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, seed=args.seed, min_p=args.min_p)
     enc = []
     for p in prompts:
         if args.ids:
@@ -167,9 +167,9 @@ def cmd_generate(args):
     if args.speculative > 0 and not hasattr(llm, "generate_speculative"):
         sys.exit("--speculative needs the continuous-batching engine: this model family is served one request at a time")
     if args.speculative > 0:
-        if args.temperature != 0.0:
-            sys.exit("--speculative verifies drafts against greedy choices: use it with --temperature 0")
-        outs, stats = llm.generate_speculative(enc, args.max_new_tokens, gamma=args.speculative)
+        from .serve.speculative import NgramTreeDrafter
+        drafter = NgramTreeDrafter(gamma=args.speculative, width=args.tree) if args.tree > 1 else None
+        outs, stats = llm.generate_speculative(enc, args.max_new_tokens, gamma=args.speculative, drafter=drafter, sp=sp)
     else:
         outs = llm.generate(enc, sp)
     dt = time.time() - t0
@@ -420,11 +420,13 @@ def main(argv=None):
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-k", type=int, default=0)
     g.add_argument("--top-p", type=float, default=1.0)
+    g.add_argument("--min-p", type=float, default=0.0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--audio", default="", help="16 kHz WAV clip for a gemma4 model; write <audio> in the prompt where it belongs")
     g.add_argument("--audio-model", default="", help="safetensors checkpoint holding the gemma4 audio tower")
     g.add_argument("--speculative", type=int, default=0, metavar="GAMMA",
-                   help="greedy speculative decoding with prompt-lookup drafts of up to GAMMA tokens, verified in one batched step")
+                   help="speculative decoding with prompt-lookup drafts of up to GAMMA tokens, verified in one batched step")
+    g.add_argument("--tree", type=int, default=1, metavar="WIDTH", help="with --speculative: trees of drafts, from the last WIDTH places where the context occurred")
     g.set_defaults(fn=cmd_generate)
     s = sub.add_parser("serve", help="HTTP server")
     _add_model_args(s)

@@ -32,7 +32,7 @@ from .. import _native
 from ..ops import attention as att
 from ..ops import elementwise as ew
 from ..ops import deltanet as dn
-from ..ops import gemm, latent, lightning, moe, qlinear, recurrent, sampling, stream
+from ..ops import gemm, latent, lightning, moe, paging, qlinear, recurrent, sampling, stream, tree
 from ..ops.mxfp8 import MxTensor
 from .config import RECURRENT, LayerRun, LayerSpec, ModelConfig, MoeSpec
 from .weights import LinearWeight, ModelWeights
@@ -206,6 +206,10 @@ class ForwardBatch:
     kv_lens: Optional[List[int]] = None
     # context-parallel prefill: the cache slots whose K / V rows this rank contributes to the per-layer all-gather (staging order)
     cp_send_slots: Optional[torch.Tensor] = None   # int64 [p_local * page_size]
+    # trees of drafted tokens (``build_tree``): what each node sees of its tree (ops.paging.batch_tables), the most nodes of a sequence, parents
+    tree_mask: Optional[torch.Tensor] = None       # int64 [T, words]
+    tree_nodes: int = 0
+    parents: Optional[torch.Tensor] = None         # int32 [T]
 
     @staticmethod
     def build(q_lens: Sequence[int], ctx_lens: Sequence[int], ids, block_table: torch.Tensor, page_size: int, hq: int, hkv: int,
@@ -246,6 +250,62 @@ class ForwardBatch:
             dev["block_table"] = block_table.to(device=device, dtype=torch.int32)
         return ForwardBatch(plans={}, q_lens=list(q_lens), kv_lens=[c + q for c, q in zip(ctx_lens, q_lens)], ids=ids_t, num_splits=num_splits, n_tokens=t,
                             is_decode=(b > 0 and all(q == 1 for q in q_lens)), **dev)
+
+
+    @staticmethod
+    def build_paged(q_lens: Sequence[int], ctx_lens: Sequence[int], ids: Sequence[int], pages: Sequence[Sequence[int]], page_size: int, hq: int, hkv: int, device,
+                    seq_slots: Optional[Sequence[int]] = None, rows: Optional[Sequence[int]] = None) -> "ForwardBatch":
+        """``build`` from the sequences' page lists.  On a GPU the lengths, lists and ids go there in one copy and the tables are made there
+        (``ops.paging.batch_tables``).  ``rows``: the rows of logits that are wanted (default: each sequence's last token)."""
+        if torch.device(device).type == "cpu":
+            bt = torch.zeros(len(pages), max((len(p) for p in pages), default=0), dtype=torch.int32)
+            for i, p in enumerate(pages):
+                bt[i, : len(p)] = torch.tensor(p, dtype=torch.int32)
+            fb = ForwardBatch.build(q_lens, ctx_lens, ids, bt, page_size, hq, hkv, device, seq_slots=seq_slots)
+            if rows is not None:
+                fb.logit_rows = torch.tensor(list(rows), dtype=torch.int64)
+            return fb
+        b = len(q_lens)
+        ql, ctx = att.whole_numbers(q_lens), att.whole_numbers(ctx_lens)
+        have = np.asarray([len(p) for p in pages], dtype=np.int64)
+        if ql.size != ctx.size or have.size != b or (ql < 0).any() or (ctx < 0).any():
+            raise ValueError("chunk lengths, context lengths and page lists name different sequences")
+        if ((ql > 0) & (ctx + ql > have * page_size)).any():
+            raise IndexError("a sequence has more tokens than its pages hold")
+        end = np.cumsum(ql)
+        want = np.asarray(rows, dtype=np.int64) if rows is not None else end[ql > 0] - 1
+        parts = dict(q=ql, ctx=ctx, ptr=np.concatenate([np.zeros(1, np.int64), np.cumsum(have)]), pages=np.asarray([x for p in pages for x in p], dtype=np.int64),
+                     ids=np.asarray(ids, dtype=np.int64), work=att.build_work(q_lens, hq, hkv).numpy(),
+                     seq_slots=np.asarray([int(x) for x in seq_slots] if seq_slots is not None else range(b), dtype=np.int64))
+        d = _to_device(want, parts, device)
+        t = paging.batch_tables(d["q"], d["ctx"], d["ptr"], d["pages"], page_size, int(end[-1]) if b else 0, int(have.max(initial=0)))
+        return ForwardBatch(ids=d["ids"], positions=t.positions, slots=t.slots, cu_q=t.cu_q, kv_len=t.kv_len, block_table=t.block_table, work=d["work"],
+                            logit_rows=d["logit_rows"], n_tokens=int(end[-1]) if b else 0, seq_slots=d["seq_slots"], is_decode=(b > 0 and bool((ql == 1).all())),
+                            plans={}, q_lens=list(q_lens), kv_lens=[c + q for c, q in zip(ctx_lens, q_lens)])
+
+    @staticmethod
+    def build_tree(ctx_lens: Sequence[int], tokens: Sequence[Sequence[int]], parents: Sequence[Sequence[int]], pages: Sequence[Sequence[int]], page_size: int,
+                   device) -> "ForwardBatch":
+        """A verification step: sequence i brings the tree ``tokens[i]`` (the first one is its last certain token) with ``parents[i]`` (-1 at the first) on top of
+        ``ctx_lens[i]`` cached positions.  Logits of every node are wanted."""
+        ql, ctx = np.asarray([len(x) for x in tokens], dtype=np.int64), att.whole_numbers(ctx_lens)
+        have = np.asarray([len(p) for p in pages], dtype=np.int64)
+        if any(len(p) != n for p, n in zip(parents, ql)) or ql.max(initial=1) > paging.MAX_NODES or ql.min(initial=1) < 1:
+            raise ValueError(f"trees of 1 to {paging.MAX_NODES} nodes with a parent each are needed")
+        if any(p[0] != -1 or any(not 0 <= x < i for i, x in enumerate(p) if i) for p in parents):
+            raise ValueError("a node's parent comes in front of it, and the first node has none")
+        if (ctx + ql > have * page_size).any():
+            raise IndexError("a sequence has more tokens than its pages hold")
+        t = int(ql.sum())
+        parts = dict(q=ql, ctx=ctx, ptr=np.concatenate([np.zeros(1, np.int64), np.cumsum(have)]), pages=np.asarray([x for p in pages for x in p], dtype=np.int64),
+                     ids=np.asarray([x for y in tokens for x in y], dtype=np.int64), parents=np.asarray([x for y in parents for x in y], dtype=np.int64),
+                     seq_slots=np.arange(len(tokens)))
+        d = _to_device(np.arange(t), parts, device)
+        most = int(ql.max(initial=1))
+        tab = paging.batch_tables(d["q"], d["ctx"], d["ptr"], d["pages"], page_size, t, int(have.max(initial=0)), d["parents"], most)
+        return ForwardBatch(ids=d["ids"], positions=tab.positions, slots=tab.slots, cu_q=tab.cu_q, kv_len=tab.kv_len, block_table=tab.block_table,
+                            work=torch.zeros(0, 4, dtype=torch.int32, device=d["ids"].device), logit_rows=d["logit_rows"], n_tokens=t, seq_slots=d["seq_slots"], plans={},
+                            q_lens=ql.tolist(), kv_lens=(ctx + ql).tolist(), tree_mask=tab.mask, tree_nodes=most, parents=d["parents"])
 
 
 def _to_device(rows: np.ndarray, parts: dict, device) -> dict:
@@ -429,6 +489,8 @@ class Transformer:
         # decode-sized batches: the projection is cut along K and the rope kernel sums the partials (not with an output gate,
         # whose columns are read again below)
         qkv = apply_linear(lw.wqkv, h, h_mx) if cfg.attn_output_gate else apply_linear_split(lw.wqkv, h, h_mx)
+        if fb.tree_mask is not None:
+            return self._attention_tree(li, lw, qkv, fb)
         if self.kv.quantized:
             return self._attention_q8(li, lw, qkv, fb)
         if getattr(self.par, "cp_world", 1) > 1:
@@ -449,6 +511,20 @@ class Transformer:
         a = att.attention(q, self.kv.k[li], self.kv.v[li], fb.cu_q, fb.kv_len, fb.block_table, self.kv.page_size, fb.work,
                           num_splits=fb.num_splits, causal=True, window=cfg.sliding_window, decode=fb.is_decode)
         a2 = a.reshape(a.shape[0], self.hq_local * cfg.head_dim)
+        if cfg.attn_output_gate:
+            g0 = (self.hq_local + 2 * self.hkv_local) * cfg.head_dim
+            dn.gate_mul(a2, qkv[:, g0: g0 + self.hq_local * cfg.head_dim])
+        return self.par.row_linear(lw.wo, a2)
+
+    def _attention_tree(self, li: int, lw, qkv, fb: ForwardBatch) -> torch.Tensor:
+        """Attention of a verification step: the nodes' K / V rows lie behind the context, and a node sees that and its ancestors."""
+        cfg, kv = self.cfg, self.kv
+        if kv.quantized or getattr(self.par, "cp_world", 1) > 1:
+            raise NotImplementedError("trees of drafted tokens: bf16 KV cache, no context parallelism")
+        q = ew.qk_norm_rope(qkv, fb.positions, fb.slots, lw.q_norm, lw.k_norm, kv.k[li], kv.v[li], self.hq_local, self.hkv_local, cfg.head_dim, cfg.rope_theta,
+                            cfg.rms_eps, self.q_scale, self.rope_dim, table=self.rope_table, positions3=fb.positions3, sections=cfg.mrope_sections)
+        a2 = tree.tree_attention(q, kv.k[li], kv.v[li], fb.cu_q, fb.kv_len, fb.block_table, kv.page_size, fb.tree_mask, fb.tree_nodes, window=cfg.sliding_window,
+                                 positions=fb.positions).reshape(q.shape[0], self.hq_local * cfg.head_dim)
         if cfg.attn_output_gate:
             g0 = (self.hq_local + 2 * self.hkv_local) * cfg.head_dim
             dn.gate_mul(a2, qkv[:, g0: g0 + self.hq_local * cfg.head_dim])
@@ -966,6 +1042,8 @@ class Transformer:
 
     def forward(self, fb: ForwardBatch) -> torch.Tensor:
         """Logits ``f32 [len(logit_rows), V_local]``."""
+        if fb.tree_mask is not None and (self.cfg.is_layered or self.cfg.has_recurrent_state):
+            raise NotImplementedError("trees of drafted tokens: every layer one of plain attention")
         x = self.forward_hidden(fb)
         return self.head(x, fb)
 

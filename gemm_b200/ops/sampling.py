@@ -87,6 +87,18 @@ def sample_ref(logits, temperature, top_k, top_p, seed, step):
     return torch.tensor(out, dtype=torch.int32)
 
 
+def uniform_numbers(seed: int, step: int, rows: int = 1) -> torch.Tensor:
+    """Numbers in [0, 1) for ``draw``: f32 ``[rows]`` on the host, a function of ``(seed, step, row)``: the generator that ``sample`` uses on the device."""
+    m, out = (1 << 64) - 1, []
+    for row in range(rows):
+        z = (seed + 0x9E3779B97F4A7C15 * (step + 1) + 0xBF58476D1CE4E5B9 * (row + 1)) & m
+        z = (z ^ z >> 30) * 0xBF58476D1CE4E5B9 & m
+        z = (z ^ z >> 27) * 0x94D049BB133111EB & m
+        z ^= z >> 31
+        out.append((z >> 40) / 16777216.0)
+    return torch.tensor(out, dtype=torch.float32)
+
+
 def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None, want_logprob: bool = False):
     """One token per row of ``logits [B, V]`` (f32 or bf16; rows may lie further apart than V) from given numbers ``uniform [B]`` (f32 in [0, 1)): int32 ``[B]``, with
     ``want_logprob`` also the f32 logarithm of the probability it was drawn with.  ``temperature``, ``top_k`` (0: no limit), ``top_p``, ``min_p``: a number, or a

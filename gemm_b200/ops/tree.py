@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import math
 from array import array
+from itertools import repeat
 from operator import attrgetter
 from typing import NamedTuple, Optional, Sequence
 
@@ -142,9 +143,9 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"trees of 1 to {MAX_NODES} nodes, not {max_nodes}")
     # (two caches a layer: by maps over the list, a loop of Python steps took 45 us of them)
-    slots = len(caches[0]) if len(caches) else 0
+    slots = caches[0].size(0) if len(caches) else 0
     on = dev.index if dev.type == "cuda" else -1
-    if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or set(map(len, caches)) - {slots}:
+    if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or set(map(torch.Tensor.size, caches, repeat(0))) - {slots}:
         raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
     if dev.type != "cuda":
         return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)

@@ -36,6 +36,7 @@ class SamplingParams:
     top_p: float = 1.0
     seed: int = 0
     stop_token_ids: Sequence[int] = ()
+    min_p: float = 0.0                # tokens less likely than this times the likeliest one are left out (drawn by ops.sampling.draw)
 
 
 class PageAllocator:
@@ -201,7 +202,14 @@ class Engine:
         return torch.stack(last_logits)
 
     # ------------------------------------------------------------------------------------------ decode
-    def _sample(self, logits: torch.Tensor, sp: SamplingParams, step: int, step_ctr: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def _sample(self, logits: torch.Tensor, sp: SamplingParams, step: int, step_ctr: Optional[torch.Tensor] = None,
+                uniform: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if sp.temperature > 0 and sp.min_p > 0:
+            if hasattr(self.par, "merge_sampled"):
+                raise NotImplementedError("min-p needs an unsharded LM head")
+            if uniform is None:
+                uniform = sampling.uniform_numbers(sp.seed, step, logits.shape[0]).to(logits.device)
+            return sampling.draw(logits, uniform, sp.temperature, sp.top_k, sp.top_p, sp.min_p)
         tok = sampling.sample(logits, sp.temperature, sp.top_k, sp.top_p, sp.seed, step, step_ctr) if sp.temperature > 0 else \
             sampling.argmax(logits, idx_offset=self.w.vocab_start)
         return self.par.merge_sampled(tok, logits) if hasattr(self.par, "merge_sampled") else tok
@@ -246,6 +254,8 @@ class Engine:
         # decode step number on the device: the sampler reads it and the bookkeeping kernel advances it, so graph replays and
         # eager steps draw the same random numbers
         st["step"] = torch.ones(1, dtype=torch.int64, device=self.device)       # step 0 sampled the first token after the prefill
+        # min-p: the numbers a step draws with, written before each step
+        st["uniform"] = sampling.uniform_numbers(sp.seed, 1, b).to(self.device) if sp.temperature > 0 and sp.min_p > 0 else None
         self._splits = splits
         self._graph = None
         self.step_count = 0
@@ -281,7 +291,7 @@ class Engine:
             tok = self.model.forward_greedy(fb)
         else:
             logits = self.model.forward(fb)
-            tok = self._sample(logits, self._sp, 0, st["step"])
+            tok = self._sample(logits, self._sp, 0, st["step"], st["uniform"])
         st["tokens"].copy_(tok)
         st["ids"].copy_(tok)
         ew.decode_advance(st["positions"], st["kv_len"], st["slots"], st["block_table"], self.page_size, step_ctr=st["step"],
@@ -290,6 +300,8 @@ class Engine:
     @torch.no_grad()
     def decode_step(self) -> torch.Tensor:
         """One token for every sequence; returns the device tensor of sampled ids (valid until the next step)."""
+        if self._static["uniform"] is not None and self.step_count:
+            self._static["uniform"].copy_(sampling.uniform_numbers(self._sp.seed, self.step_count + 1, self._static["ids"].numel()))
         with profiler.region("decode_step", "step", "engine"):
             if self._graph is not None:
                 self._graph.replay()

@@ -111,18 +111,12 @@ class LLM:
         """One engine step over the block manager's sequences ``seqs`` (state slots ``slots``): sequence i brings ``q_lens[i]`` tokens on top of
         ``ctx[i]`` cached positions.  ``rows``: the places among the step's tokens whose logits are wanted (default: each sequence's last)."""
         pages = [self.blocks.pages(s) for s in seqs]
-        bt = torch.zeros(len(seqs), max(len(p) for p in pages), dtype=torch.int32)
-        for i, p in enumerate(pages):
-            bt[i, : len(p)] = torch.tensor(p, dtype=torch.int32)
         # a sequence starts (or restarts after a recompute-preemption) from an empty recurrent state: unlike K/V, which the prefill
         # overwrites, the state that an earlier user of the slot (or the first pass) left would otherwise leak into it
         fresh = [sl for sl, c in zip(slots, ctx) if c == 0]
         if fresh:
             self.kv.reset_slots(fresh)
-        fb = ForwardBatch.build(q_lens, ctx, ids, bt, self.page_size, self.model.hq_local, self.model.hkv_local, self.device, seq_slots=slots)
-        if rows is not None:
-            fb.logit_rows = torch.tensor(list(rows), dtype=torch.int64, device=self.device)
-        return fb
+        return ForwardBatch.build_paged(q_lens, ctx, ids, pages, self.page_size, self.model.hq_local, self.model.hkv_local, self.device, seq_slots=slots, rows=rows)
 
     def has_work(self) -> bool:
         return self.sched.num_waiting > 0 or self.sched.num_running > 0
@@ -206,7 +200,11 @@ class LLM:
                     self.spec_accepted += n_keep
                 else:
                     j = row0[i]
-                    new = [int(sampling.sample(logits[j:j + 1], sp.temperature, sp.top_k, sp.top_p, sp.seed + it.req_id, len(r.out))[0])]
+                    if sp.min_p > 0 and sp.temperature > 0:
+                        u = sampling.uniform_numbers(sp.seed + it.req_id, len(r.out)).to(self.device)
+                        new = [int(sampling.draw(logits[j:j + 1], u, sp.temperature, sp.top_k, sp.top_p, sp.min_p)[0])]
+                    else:
+                        new = [int(sampling.sample(logits[j:j + 1], sp.temperature, sp.top_k, sp.top_p, sp.seed + it.req_id, len(r.out))[0])]
                 kept = []
                 for tok in new:
                     r.tokens.append(tok)
@@ -245,9 +243,10 @@ class LLM:
         return [q.out for q in reqs]
 
     def generate_speculative(self, prompts: Sequence, max_new_tokens: int = 64, gamma: int = 4, drafter=None,
-                             stop_token_ids: Sequence[int] = ()):
-        """Greedy generation with speculative decoding (``serve/speculative.py``): same tokens as greedy ``generate``, fewer
-        model steps when the drafts hit.  Uses the whole cache, so no request may be in flight.  Returns (outputs, statistics)."""
+                             stop_token_ids: Sequence[int] = (), sp: Optional[SamplingParams] = None):
+        """Generation with speculative decoding (``serve/speculative.py``): same tokens as without drafts, fewer model steps when they hit.  Greedy, or with the
+        temperature, top-k, top-p, min-p and seed of ``sp``; chains of drafts, or trees (``NgramTreeDrafter``).  Uses the whole cache, so no request may be in
+        flight.  Returns (outputs, statistics)."""
         from .speculative import NgramDrafter, SpeculativeDecoder
         if self.has_work():
             raise RuntimeError("speculative generation needs an idle engine")
@@ -255,7 +254,7 @@ class LLM:
             raise RuntimeError("speculative generation needs an empty cache")
         dec = SpeculativeDecoder(self.model, self.kv, self.page_size, self.num_pages, drafter or NgramDrafter(gamma=gamma))
         enc = [self.tokenizer.encode(p) if isinstance(p, str) else list(p) for p in prompts]
-        return dec.generate(enc, max_new_tokens, stop_token_ids), dec.stats
+        return dec.generate(enc, max_new_tokens, stop_token_ids, sp), dec.stats
 
     def stream(self, prompt, sp: Optional[SamplingParams] = None) -> Iterator[int]:
         """Yield the tokens of one request as they are produced (other queued requests keep being served)."""

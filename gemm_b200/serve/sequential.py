@@ -73,12 +73,15 @@ class SequentialLLM:
             kth = torch.topk(row, min(sp.top_k, row.numel())).values[-1]
             row = row.masked_fill(row < kth, float("-inf"))
         p = torch.softmax(row, dim=-1)
+        low = p < sp.min_p * p.max()
         if sp.top_p < 1.0:
             sp_, idx = torch.sort(p, descending=True)
             cut = (torch.cumsum(sp_, 0) - sp_) > sp.top_p
             sp_[cut] = 0.0
             p = torch.zeros_like(p).scatter_(0, idx, sp_)
             p = p / p.sum()
+        if sp.min_p > 0:
+            p = p.masked_fill(low, 0.0)                 # (multinomial takes weights that do not add up to one)
         g = torch.Generator(device="cpu").manual_seed(sp.seed * 1000003 + step)
         return int(torch.multinomial(p.cpu(), 1, generator=g))
 

@@ -208,7 +208,7 @@ def make_handler(engine: EngineThread, model_name: str):
                 stops = [i for i in (llm.tokenizer.eos_id, llm.tokenizer.eot_id) if i >= 0]
             sp = SamplingParams(max_new_tokens=int(req.get("max_tokens", 128)), temperature=float(req.get("temperature", 0.0)),
                                 top_k=int(req.get("top_k", 0)), top_p=float(req.get("top_p", 1.0)), seed=int(req.get("seed", 0)),
-                                stop_token_ids=tuple(stops))
+                                min_p=float(req.get("min_p", 0.0)), stop_token_ids=tuple(stops))
             stop_strings = req.get("stop") or []
             if isinstance(stop_strings, str):
                 stop_strings = [stop_strings]
