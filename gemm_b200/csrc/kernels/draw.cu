@@ -33,6 +33,7 @@ constexpr int kDrPairs = 256;              // candidates that are compared with 
 constexpr int kDrGroups = 4096;            // groups of logits whose maxima prune a row
 constexpr int kDrPrune = 1000;             // k' at most: a quarter of the groups, so that few logits beyond the k'-th lie above the bound
 constexpr int kDrMass = 44;                // fraction bits of a weight
+constexpr size_t kDrSmem = 202000;         // bytes of logits that a block holds at most
 
 struct DrawArgs {
   const void* logits;
@@ -158,6 +159,7 @@ draw_kernel(const DrawArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = a.ctas;
   const int row = blockIdx.x / C, rank = blockIdx.x - row * C;     // (the cluster is C blocks along x: rank is the block's place in it)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // here; what another block's shared memory gets in front of the first exchange waits for it
   if (tid == 0) { mbar_init(&s.bar, 1); s.abort_flag = 0; fence_barrier_init(); }
   if (tid < 32) s.table[tid] = exp2((double)tid * 0.03125);
   __syncthreads();
@@ -198,6 +200,7 @@ draw_kernel(const DrawArgs a) {
     if (tid < n - head - body) f(Key::value(x[head + body + tid]), head + body + tid);
   };
 
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces.  (fmaxf passes over NaN.)
   float mx = -INFINITY, low = INFINITY;
   {
@@ -1037,13 +1040,13 @@ static int draw_launch(DrawArgs a, cudaStream_t stream) {
   a.ctas = c;
   a.per = ((a.vocab + c - 1) / c + 15) / 16 * 16;
   const size_t smem = (size_t)a.per * sizeof(T) + 32;
-  if (smem > 202000) return fail("draw: the vocabulary does not fit the shared memory of eight blocks%s");
-  static size_t attr[64];
+  if (smem > kDrSmem) return fail("draw: the vocabulary does not fit the shared memory of eight blocks%s");
+  static bool attr[64];
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
-  if (dev > 63 || smem > attr[dev]) {
-    GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (dev < 64) attr[dev] = smem;
+  if (dev > 63 || !attr[dev]) {
+    GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDrSmem));
+    if (dev < 64) attr[dev] = true;
   }
   launch_k_cluster(draw_kernel<T>, (unsigned)(a.rows * c), kDrThreads, smem, stream, (unsigned)c, a);
   GB_CUDA_OK(cudaGetLastError());

@@ -107,7 +107,8 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
     In the order (logit descending, id ascending): the first ``top_k`` ids; of these the ids that have less than ``top_p`` of the probability in front of them (at
     least one); of these the ids with at least ``min_p`` times the largest probability.  The draw is the first id, in id order, at which the kept probability so
     far exceeds ``uniform`` of it all.  ``temperature <= 0``: the lowest id of the largest logit.  NaN counts as -inf; a row without any logit above -inf answers
-    id 0 with logarithm -inf.  Probabilities below 2^-45 of the largest count as zero."""
+    id 0 with logarithm -inf.  Probabilities below 2^-45 of the largest count as zero.  On a GPU a row has at most
+    1.6 MB of logits."""
     if logits.dim() != 2 or (logits.dtype is not torch.float32 and logits.dtype is not torch.bfloat16) or logits.shape[1] < 1:
         raise ValueError("logits: a tensor [B, V] in f32 or bf16 is needed")
     b, v = logits.shape
@@ -124,7 +125,7 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
                 raise ValueError(f"{name}: a contiguous {dt} tensor [{b}] beside the logits is needed")
             given.append((x, none))
         else:
-            given.append((None, none if x is None else type(none)(x)))
+            given.append((None, none if x is None else type(none)(x) if x is not top_k else max(-1, min(int(x), 2 ** 31 - 1))))
     if not logits.is_cuda:
         token, logprob = draw_ref(logits, uniform, *(x if x is not None else y for x, y in given))
         return (token, logprob) if want_logprob else token
