@@ -258,8 +258,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint64_t* g_full = bars + 28; uint64_t* g_empty = bars + 32;                                 // [kTaSegs] each
   uint32_t* tmem_slot = (uint32_t*)(bars + 36);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  int* s_odd = (int*)(tmem_slot + 2);                             // [8] tree nodes of the segment whose value rows are not finite, as bits
-  float* s_x = (float*)(bars + 42);                               // [2][128]: what the groups tell each other about a row
+  int* s_odd = (int*)(tmem_slot + 2);                             // [16] places of the segment whose value rows are not finite, as bits: tree nodes; context from the window's begin on
+  float* s_x = (float*)(bars + 46);                               // [2][128]: what the groups tell each other about a row
   TaSeg* s_seg = (TaSeg*)(s_x + 256);                           // [kTaSegs]; n_tiles = 0: no more
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -269,7 +269,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int i = 0; i < 10; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 1); }
     for (int i = 0; i < kTaSegs; ++i) { mbar_init(&g_full[i], 1); mbar_init(&g_empty[i], 4); }      // (a softmax thread and the warps 8, 9, 10 give a segment back)
     *abort_flag = 0;
-    for (int i = 0; i < 8; ++i) s_odd[i] = 0;
+    for (int i = 0; i < 16; ++i) s_odd[i] = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
   }
@@ -463,6 +463,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int tok = s.q.begin + min(node, s.q.nodes - 1);
       const unsigned long long* mrow = a.mask + (size_t)tok * a.words;
       const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first place of the context that the row sees
+      const int win0 = ctx - a.window + 1, win1 = a.window > 0 ? win0 + s.q.nodes - 1 : 0;         // places in front of win0 are out of every row's window, those in front of win1 out of some row's
       float m = -INFINITY, l = 0.f;
       bool first = true;
       for (int b = two ? 0 : g; b < n && ok; b += two ? 1 : 2) {
@@ -481,13 +482,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b));        // (a warp leaves as one)
         if (!ok) break;
         s_ph ^= 1;
-        if (tail && (!two || g == 0)) {
+        if ((tail || kv0 < win1) && (!two || g == 0)) {
           // Values of places that some row does not see must be finite: a weight of 0 times them is added.  Thread r looks at place r of the block; what is not
           // finite is taken out, noted, and put back at the end for the rows that see it.  (Behind the wait for S, which tells that the products in front are done:
           // in front of it the place's tile before this one may still be on its way, and its barrier two phases from the one waited for.)
           const uint32_t t = t0 + 2 * b + 1;
           ok = __all_sync(0xffffffffu, mbar_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b));
-          if (ok && kv0 + r >= min(ctx, len)) {
+          if (ok && (kv0 + r >= min(ctx, len) || kv0 + r < win1)) {
             uint8_t* row = ring + (t % slots) * kSlot + r * 128;
             bool odd = false;
 #pragma unroll 2
@@ -507,8 +508,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               if (put) *w = v;
               odd |= put;
             }
-            const int x = kv0 + r - ctx;
-            if (odd && kv0 + r < len && x >= 0 && x < 256) atomicOr(&s_odd[x >> 5], 1 << (x & 31));
+            const int x = kv0 + r >= ctx ? kv0 + r - ctx : kv0 + r - win0 + 256;         // (the window's begin is cut by fewer places than there are nodes)
+            if (odd && kv0 + r < len && x >= (kv0 + r >= ctx ? 0 : 256) && x < (kv0 + r >= ctx ? 256 : 512)) atomicOr(&s_odd[x >> 5], 1 << (x & 31));
           }
           fence_proxy_async_smem();
         }
@@ -555,7 +556,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       uint32_t any_odd = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) any_odd |= (uint32_t)s_odd[i];
+      for (int i = 0; i < 16; ++i) any_odd |= (uint32_t)s_odd[i];
       if (n > 0) {
         ok = mbar_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, k);
         if (both) ok = ok && mbar_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, k);
@@ -604,9 +605,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           bar_group(g);
         }
         if (any_odd && ok && live && fold == 0) {
-          for (int x = 0; x < min(256, a.words * 64); ++x) {
-            if (!((s_odd[x >> 5] >> (x & 31)) & 1) || !((mrow[x >> 6] >> (x & 63)) & 1)) continue;
-            const int at = ctx + x;
+          for (int x = 0; x < 512; ++x) {
+            if (!((s_odd[x >> 5] >> (x & 31)) & 1)) continue;
+            const int at = x < 256 ? ctx + x : win0 + x - 256;
+            if (x < 256 ? x >= a.words * 64 || !((mrow[x >> 6] >> (x & 63)) & 1) : at < lo) continue;
             const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
             if (slot < 0 || slot >= a.num_slots) continue;
             const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
@@ -670,7 +672,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (live && fold == 0 && !full && c0 == 0) a.part_lse[prow] = lse;
       if (any_odd) {
         bar256_and(true);
-        if (threadIdx.x < 8) s_odd[threadIdx.x] = 0;
+        if (threadIdx.x < 16) s_odd[threadIdx.x] = 0;
       }
       tc_fence_before();
       ok = ok && mbar_wait(&g_full[(k + 1) % kTaSegs], ((k + 1) / kTaSegs) & 1, abort_flag, a.status, 834, k + 1);

@@ -10,6 +10,8 @@
 #include "sm100.cuh"
 #include "host_common.h"
 #include <algorithm>
+#include <utility>
+#include <vector>
 
 namespace gb {
 
@@ -126,6 +128,14 @@ GB_API int gb_tree_commit(const void* const* caches, const long long* bytes, int
                           int* count, int* path, int* next_token, int* new_len, cudaStream_t stream) {
   if (n_seqs <= 0) return 0;
   if (n_seqs > 65535 || n_caches < 0 || page_size < 1 || max_pages < 0 || total_tokens < 0 || max_nodes < 1 || max_nodes > kTcNodes) return fail("tree_commit: bad sizes%s");
+  // a row moved twice, or by two blocks at once, would be read after it was written
+  try {
+    std::vector<std::pair<uintptr_t, long long>> at;
+    at.reserve(n_caches);
+    for (int i = 0; i < n_caches; ++i) if (bytes[i] > 0) at.emplace_back((uintptr_t)caches[i], bytes[i]);
+    std::sort(at.begin(), at.end());
+    for (size_t i = 1; i < at.size(); ++i) if (at[i - 1].first + at[i - 1].second > at[i].first) return fail("tree_commit: caches that overlap%s");
+  } catch (...) { return fail("tree_commit: out of memory%s"); }
   TreeCommitArgs a;
   int done = 0;
   do {

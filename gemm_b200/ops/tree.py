@@ -29,13 +29,16 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``k_cache [slots, Hkv, dk]`` / ``v_cache [slots, Hkv, dv]``.  Sequence s has the nodes ``cu_q[s] .. cu_q[s + 1]`` (at most ``max_nodes`` <= 256), cached at
     its last places.  A node sees the places in front of the tree (``window`` > 0: those less than ``window`` in front of its ``positions`` entry) and the
     nodes whose bits are set in its row of ``mask`` (int64 ``[T, words]``, its own bit among them as a rule).  A node that sees nothing gets zeros; rows behind
-    the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not finite."""
+    the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not
+    finite; a value that is not finite makes that feature of the nodes that see it not finite."""
     t, hq, dk = q.shape
     slots, hkv, dv = v_cache.shape
     dev, dtype = q.device, q.dtype
     b = kv_len.numel()
     q_ts, q_hs, q_es = q.stride()
-    if q_es != 1 or q_hs != dk or (t > 1 and q_ts < hq * dk):
+    if t <= 1:
+        q_ts = hq * dk
+    if q_es != 1 or (hq > 1 and q_hs != dk) or q_ts < hq * dk:
         raise ValueError("q: the heads of a token lie one after the other")
     if k_cache.shape != (slots, hkv, dk) or not (k_cache.is_contiguous() and v_cache.is_contiguous()) or v_cache.dtype is not dtype or k_cache.dtype is not dtype:
         raise ValueError("contiguous caches of the same slots, heads and type as the queries are needed")
@@ -133,7 +136,7 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
     """Accepts, from the root of every tree, the first child whose token (``tokens``) is the one drawn at its parent (``sampled``), as long as there is one, and
     moves the accepted nodes' rows of all ``caches`` (``[slots, ...]`` contiguous, any type, e.g. every layer's K and V) from the places ``ctx + node`` to
     ``ctx, ctx + 1, ...``, in place.  ``tokens`` / ``parents`` / ``sampled``: int32 ``[T]``; the lengths and tables are those of the verifying pass (``kv_len``
-    includes the tree).  No caches: the walk alone."""
+    includes the tree).  The caches do not overlap.  No caches: the walk alone."""
     dev, t, b = tokens.device, tokens.numel(), kv_len.numel()
     check_int32(dev, "tokens parents sampled cu_q kv_len block_table", tokens, parents, sampled, cu_q, kv_len, block_table)
     if parents.numel() != t or sampled.numel() != t:
@@ -142,12 +145,15 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
         raise ValueError("cu_q, kv_len and block_table name different numbers of sequences")
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"trees of 1 to {MAX_NODES} nodes, not {max_nodes}")
-    # (two caches a layer: by maps over the list, a loop of Python steps took 45 us of them)
+    # (two caches a layer: by maps over the list, a loop of Python steps took 45 us of 56)
     slots = caches[0].size(0) if len(caches) else 0
     on = dev.index if dev.type == "cuda" else -1
     if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or set(map(torch.Tensor.size, caches, repeat(0))) - {slots}:
         raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
     if dev.type != "cuda":
+        spans = sorted((c.data_ptr(), c.nbytes) for c in caches if c.nbytes)
+        if any(a + n > z for (a, n), (z, _) in zip(spans, spans[1:])):
+            raise ValueError("tree_commit: caches that overlap")
         return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)
     with _native.on_device(dev):
         count, nxt, new, path = torch.empty(b * (3 + max_nodes), dtype=torch.int32, device=dev).split((b, b, b, b * max_nodes))

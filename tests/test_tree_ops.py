@@ -271,6 +271,58 @@ def test_attention_kernel_masked_places(hq, hkv, n, d):
     assert torch.isfinite(got[n:, :, 4:]).all()
 
 
+def window_inputs(hq, hkv, n, d, window, ctx):
+    """Keys and values that are not finite in front of every row's window, and one infinite feature at a place that only the root of each tree sees."""
+    s = attention_inputs([n, 1, n], [ctx, ctx, ctx + 61], hq, hkv, d, d, 16, seed=n)
+    s["window"] = window
+    odd = s["v_cache"].clone()
+    for seq, c in enumerate((ctx, ctx, ctx + 61)):
+        place = torch.arange(max(0, c - window + 1))
+        slot = s["block_table"][seq].long()[place // 16] * 16 + place % 16
+        for cache in (s["k_cache"], s["v_cache"], odd):
+            cache[slot] = float("nan")
+        j = c - window + 1
+        odd[int(s["block_table"][seq, j // 16]) * 16 + j % 16, :, 3] = float("inf")
+    depth0 = torch.zeros(2 * n + 1, dtype=torch.bool)
+    depth0[[0, n, n + 1]] = True
+    return s, odd, depth0
+
+
+WINDOWS = [(4, 2, 3, 128, 50, 300), (16, 2, 70, 128, 130, 700), (8, 8, 12, 64, 100, 260), (32, 8, 20, 128, 257, 3000), (4, 1, 30, 64, 7, 130), (2, 1, 5, 96, 40, 130)]
+
+
+def check_window(run, hq, hkv, n, d, window, ctx):
+    s, odd, depth0 = window_inputs(hq, hkv, n, d, window, ctx)
+    got = run(s).cpu()
+    assert torch.isfinite(got).all()
+    close(got, s)
+    got = run({**s, "v_cache": odd}).cpu()
+    # What sees the infinite value is not finite: infinite, or NaN, since a row may be held as several sums over its places, and in those that leave the place out it
+    # is multiplied by a weight of zero (0 * inf = NaN) where all of the sequence's rows see it.
+    assert not torch.isfinite(got[depth0][:, :, 3]).any() and torch.isfinite(got[~depth0]).all() and torch.isfinite(got[:, :, 4:]).all()
+
+
+@pytest.mark.parametrize("hq,hkv,n,d,window,ctx", WINDOWS)
+def test_attention_plain_window(hq, hkv, n, d, window, ctx):
+    check_window(lambda s: tree.tree_attention(**s), hq, hkv, n, d, window, ctx)
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,n,d,window,ctx", WINDOWS)
+def test_attention_kernel_window(hq, hkv, n, d, window, ctx):
+    check_window(lambda s: tree.tree_attention(**on_gpu(s)), hq, hkv, n, d, window, ctx)
+
+
+@gpu
+def test_attention_kernel_single_rows():
+    """The strides of dimensions of size one do not matter."""
+    for nodes, hq, hkv in (([1], 4, 2), ([3], 1, 1)):
+        s = attention_inputs(nodes, [40], hq, hkv, 64, 64, 16)
+        c = on_gpu(s)
+        c["q"] = c["q"].as_strided(c["q"].shape, (8, 64, 1) if nodes == [1] else (64, 8, 1))
+        close(tree.tree_attention(**c), s)
+
+
 @gpu
 @pytest.mark.parametrize("nodes,hkv,ctx", [(8, 4, 4000), (40, 2, 1500)])
 def test_attention_kernel_long_pieces(nodes, hkv, ctx):
@@ -574,3 +626,77 @@ def test_commit_refusals():
                 dict(page_size=0), dict(block_table=s["block_table"][0]), dict(caches=[s["caches"][0], s["caches"][1][:3]]), dict(caches=[s["caches"][0].transpose(1, 2)])):
         with pytest.raises(ValueError):
             tree.tree_commit(**{**s, **bad})
+
+
+def test_commit_refuses_caches_that_overlap():
+    """A row moved twice would be read after it was written."""
+    s = commit_inputs([4, 2], [3, 0], 8, [((2, 8), torch.bfloat16)] * 2)
+    for caches in ([s["caches"][0]] * 2, [s["caches"][0], s["caches"][0].flatten()[: -8 * s["caches"][0].shape[0]].view(-1, 8)]):
+        with pytest.raises(ValueError, match="overlap"):
+            tree.tree_commit(**{**s, "caches": caches})
+
+
+@gpu
+def test_commit_kernel_refuses_caches_that_overlap():
+    s = commit_inputs([4, 2], [3, 0], 8, [((2, 8), torch.bfloat16)] * 2)
+    d = on_gpu({**s, "caches": None})
+    with pytest.raises(RuntimeError, match="overlap"):
+        tree.tree_commit(**{**d, "caches": [s["caches"][0].cuda()] * 2})
+    flat = s["caches"][0].cuda().flatten()                                     # neighbours in one buffer
+    half = flat.numel() // 2
+    want = tree.tree_commit(**{**s, "caches": [flat[:half].cpu().view(-1, 8), flat[half:].cpu().view(-1, 8)]})
+    for a, b in zip(tree.tree_commit(**{**d, "caches": [flat[:half].view(-1, 8), flat[half:].view(-1, 8)]}), want):
+        assert torch.equal(a.cpu(), b)
+
+
+# ------------------------------------------------------------------------------------------ a step
+def step_of(s):
+    """A verification step in its parts, from tensors alone."""
+    t = paging.batch_tables(s["q"], s["ctx"], s["ptr"], s["pages"], 16, s["parents"].numel(), 40, s["parents"], 12)
+    o = tree.tree_attention(s["rows"], s["k"], s["v"], t.cu_q, t.kv_len, t.block_table, 16, t.mask, 12, window=64, positions=t.positions, out=torch.zeros_like(s["rows"]))
+    logits = o.flatten(1)[:, :50] * 8
+    tok, lp = sampling.draw(logits, s["u"], s["temp"], 5, s["top_p"], 0.02, want_logprob=True)
+    return [t.slots, o, tok, lp] + list(tree.tree_commit([s["k"], s["v"]], s["tokens"], s["parents"], tok, t.cu_q, t.kv_len, t.block_table, 16, 12)) + [s["k"], s["v"]]
+
+
+def step_inputs(seed):
+    r, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    q, ctx = [r.randint(0, 12) for _ in range(7)], [r.randint(0, 600) for _ in range(7)]
+    pages = list(range(7 * 40))
+    r.shuffle(pages)
+    par = [p for n in q for p in (random_tree(n, r) if n else [])]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)                     # noqa: E731
+    cut = lambda v: (v + [-1] * 84)[:84]                                    # noqa: E731
+    need = [(a + b + 15) // 16 for a, b in zip(q, ctx)]
+    ptr = [0] + [int(x) for x in torch.tensor(need).cumsum(0)]
+    rnd = lambda *sh: torch.randn(*sh, generator=g).bfloat16()             # noqa: E731
+    return dict(q=i32(q), ctx=i32(ctx), ptr=i32(ptr), pages=i32(pages), parents=i32(cut(par)), tokens=i32([r.randrange(4) for _ in range(84)]), rows=rnd(84, 8, 64) / 4,
+                k=rnd(7 * 640, 2, 64), v=rnd(7 * 640, 2, 64), u=torch.rand(84, generator=g), temp=torch.rand(84, generator=g) * 2,
+                top_p=torch.rand(84, generator=g))
+
+
+@gpu
+def test_captured_steps():
+    """Two captured steps, replayed in turn with other lengths, trees and numbers, and one beside the other on two streams: what the eager calls answer, bit for bit."""
+    cases = [{k: x.cuda() for k, x in step_inputs(i).items()} for i in range(4)]
+    copy = lambda s: {k: x.clone() for k, x in s.items()}                   # noqa: E731
+    want = [[x.clone() for x in step_of(copy(s))] for s in cases]
+    static, graphs, outs = [copy(cases[0]), copy(cases[0])], [torch.cuda.CUDAGraph() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for s, graph in zip(static, graphs):
+        with torch.cuda.graph(graph):
+            outs.append(step_of(s))
+    for first, second in ((1, 2), (3, 0), (2, 2)):
+        for s, i in zip(static, (first, second)):
+            for k, x in s.items():
+                x.copy_(cases[i][k])
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, i in zip(outs, (first, second)):
+            for a, b in zip(got, want[i]):
+                assert torch.equal(a, b)
+    _native.assert_status_ok()
