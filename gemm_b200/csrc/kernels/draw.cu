@@ -66,12 +66,15 @@ struct alignas(16) DrawShared {
   float bound;                             // written by the first block into all
   int cand_n[8];                           // of every block, written by it into all
   int cand_in[8];
-  int cand_own;
+  int cand_own, cand_own_in;
+  int cut;                                 // of top-p: its step, the mass in front of the step, and the mass in front of which it keeps (written by the first block into all)
+  unsigned long long cut_before, cut_target;
   unsigned tau, last;                      // written by the first block into all: the cut
   unsigned long long block_mass[8];        // kept mass of every block, written by it into all
   union {
     float group[kDrGroups];                // first block: maxima of the groups
     uint2 cand[kDrCand];                   // first block: key and id; a share of the places for every block
+    unsigned long long chunk[kDrThreads];  // masses of the block's chunks of ids
     unsigned short list[kDrWarps][kDrList];
   };
 };
@@ -116,20 +119,19 @@ template <> struct DrawKey<__nv_bfloat16> {
   static __device__ __forceinline__ unsigned of(float v) { return DrawKey<float>::of(v) >> 16; }         // (the value is a bf16: nothing is lost, and the order stays)
 };
 
-// 2^t in units of 2^-44, for t <= 0; t = -46 and below (and NaN): 0.
-template <typename F>
-__device__ __forceinline__ unsigned long long dr_weight(double t, F entry) {
-  if (!(t > -46.0)) t = -47.0;                                    // (rounds to 0)
+// 2^(d scale / 32) in units of 2^-44, for -32000 < d scale <= 0.  table[j]: 2^(44 + j / 32).
+__device__ __forceinline__ unsigned long long dr_weight(double d, double scale, const double* table) {
   constexpr double kRound = 6755399441055744.0;                   // 1.5 * 2^52: the sum's low bits are the rounded number
-  const double m = fma(t, 32.0, kRound);
+  const double m = fma(d, scale, kRound);
   const int k = __double2loint(m);
-  const double r = t - (m - kRound) * 0.03125;                    // |r| <= 1/64
-  // 2^r = sum (r ln 2)^n / n!
-  constexpr double c1 = 0.69314718055994531, c2 = 0.24022650695910072, c3 = 0.05550410866482158, c4 = 0.009618129107628477, c5 = 0.0013333558146428443;
-  double p = fma(r, c5, c4);
-  p = fma(r, p, c3); p = fma(r, p, c2); p = fma(r, p, c1); p = fma(r, p, 1.0);
-  p *= entry(k & 31);
-  p = __hiloint2double(__double2hiint(p) + ((k >> 5) + kDrMass) * 1048576, __double2loint(p));     // times 2^(k >> 5), in units
+  const double r = fma(d, scale, kRound - m);                     // |r| <= 1/2
+  // 2^(r / 32) = sum (r ln 2 / 32)^n / n!, the fifth power by (20 r^3 / 4 - 5 r / 16) / 16 (its error: Chebyshev's polynomial, 8e-14 of the weight)
+  constexpr double c5 = 0.0013333558146428443 / 33554432, c4 = 0.009618129107628477 / 1048576, c3 = 0.05550410866482158 / 32768 + c5 * 0.3125,
+                   c2 = 0.24022650695910072 / 1024, c1 = 0.69314718055994531 / 32 - c5 * 0.01953125;
+  double p = fma(r, c4, c3);
+  p = fma(r, p, c2); p = fma(r, p, c1); p = fma(r, p, 1.0);
+  p *= table[k & 31];
+  p = __hiloint2double(__double2hiint(p) + (int)((unsigned)(k & ~31) << 15), __double2loint(p));   // times 2^(k >> 5)
   return (unsigned long long)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;    // 2^52: rounded to a whole number
 }
 
@@ -161,7 +163,7 @@ draw_kernel(const DrawArgs a) {
   const int row = blockIdx.x / C, rank = blockIdx.x - row * C;     // (the cluster is C blocks along x: rank is the block's place in it)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // here; what another block's shared memory gets in front of the first exchange waits for it
   if (tid == 0) { mbar_init(&s.bar, 1); s.abort_flag = 0; fence_barrier_init(); }
-  if (tid < 32) s.table[tid] = exp2((double)tid * 0.03125);
+  if (tid < 32) s.table[tid] = exp2(kDrMass + (double)tid * 0.03125);
   __syncthreads();
   pdl_wait();
   pdl_trigger();
@@ -189,8 +191,16 @@ draw_kernel(const DrawArgs a) {
 
   // f(value, index in the block) for the thread's share of the block's logits: 16 bytes at a time, and the ragged ends.  Step: threads between two of a thread's turns
   const int nv = body / kVec;
-  auto vec_at = [&](int j, float* v) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(x + head + j * kVec);
+  auto vec_raw = [&](int j) -> uint4 { return *reinterpret_cast<const uint4*>(x + head + j * kVec); };
+  auto vec_max = [&](const uint4& r) -> float {                    // the largest (NaN only where there is nothing else)
+    if constexpr (sizeof(T) == 4) return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    else {                                                         // (two to an instruction)
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+      const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(m.x, m.y);
+    }
+  };
+  auto vec_of = [&](const uint4& raw, float* v) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int e = 0; e < kVec; ++e) v[e] = sizeof(T) == 4 ? __uint_as_float(w[e & 3]) : __uint_as_float(e & 1 ? w[(e >> 1) & 3] & 0xffff0000u : w[(e >> 1) & 3] << 16);
@@ -204,25 +214,37 @@ draw_kernel(const DrawArgs a) {
   // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces.  (fmaxf passes over NaN.)
   float mx = -INFINITY, low = INFINITY;
   {
-    const int pieces = kDrGroups / kDrThreads / C;
-    const bool fine = 2 * nv < pieces * kDrThreads;                // few logits: groups of single ones rather than empty groups
-    for (int p = 0; p < pieces; ++p) {
-      float gm = -INFINITY;
-      if (fine) {
-        for (int i = p * kDrThreads + tid; i < n; i += pieces * kDrThreads) gm = fmaxf(gm, Key::value(x[i]));
-      } else {
-        if (p == 0) ends([&](float v, int) { gm = fmaxf(gm, v); });
-#pragma unroll 2
-        for (int j = p * kDrThreads + tid; j < nv; j += pieces * kDrThreads) {
-          float v[kVec];
-          vec_at(j, v);
+    constexpr int kPieces = kDrGroups / kDrThreads;
+    const int pieces = kPieces / C;
+    float gm[kPieces];                                             // eight running maxima, joined to as many as there are pieces
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) gm = fmaxf(gm, v[e]);
-        }
+    for (int p = 0; p < kPieces; ++p) gm[p] = -INFINITY;
+    if (2 * nv < pieces * kDrThreads) {                            // few logits: groups of single ones rather than empty groups
+      for (int i = tid; i < n; i += kPieces * kDrThreads) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) if (i + p * kDrThreads < n) gm[p] = fmaxf(gm[p], Key::value(x[i + p * kDrThreads]));
       }
-      dr_put32(&s.group[(rank * pieces + p) * kDrThreads + tid], 0, __float_as_uint(gm));
-      mx = fmaxf(mx, gm);
-      if (gm > -INFINITY) low = fminf(low, gm);
+    } else {
+      for (int j = tid; j < nv; j += kPieces * kDrThreads) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) if (j + p * kDrThreads < nv) gm[p] = fmaxf(gm[p], vec_max(vec_raw(j + p * kDrThreads)));
+      }
+      ends([&](float v, int) { gm[0] = fmaxf(gm[0], v); });
+    }
+#pragma unroll
+    for (int half = kPieces / 2; half > 0; half /= 2) {
+      if (pieces > half) break;
+#pragma unroll
+      for (int p = 0; p < half; ++p) gm[p] = fmaxf(gm[p], gm[p + half]);
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      if (p >= pieces) break;
+      float* to = &s.group[(rank * pieces + p) * kDrThreads + tid];
+      if (rank == 0) *to = gm[p];                                  // (a store through the cluster's network takes several times as long, to the own block too)
+      else dr_put32(to, 0, __float_as_uint(gm[p]));
+      mx = fmaxf(mx, gm[p]);
+      if (gm[p] > -INFINITY) low = fminf(low, gm[p]);
     }
   }
   mx = warp_max(mx);
@@ -259,15 +281,19 @@ draw_kernel(const DrawArgs a) {
     return;
   }
 
-  const double scale = 1.4426950408889634 / (double)temp, dmx = (double)mx;
-  auto weight = [&](float v) -> unsigned long long {
-    return v == mx ? 1ull << kDrMass : dr_weight(((double)v - dmx) * scale, [&](int j) { return s.table[j]; });
-  };
-  // the same where the whole warp asks: the table lies in the lanes (a shuffle has no bank conflicts)
-  const double lane_entry = s.table[lane];
-  auto weight_all = [&](float v) -> unsigned long long {
-    const unsigned long long w = dr_weight(((double)v - dmx) * scale, [&](int j) { return __shfl_sync(0xffffffffu, lane_entry, j); });
-    return v == mx ? 1ull << kDrMass : w;
+  // Logits of floor_x and below (and NaN) weigh nothing: 46.5 halvings or more.  Where the next logit below the maximum lies further down than 1000 halvings, the scale is one
+  // that takes it to 64 (the exponent stays in range).  Rows whose floor is no number take the cluster's path, which looks at every logit.
+  const double dmx = (double)mx;
+  const float floor_x = fmaxf(__fsub_rd(mx, 32.25f * temp), -FLT_MAX);
+  const bool plain = mx < INFINITY && floor_x > -FLT_MAX;
+  double scale = 1.4426950408889634 / (double)temp;
+  if (plain && (dmx - (double)floor_x) * scale > 1000.0) scale = 64.0 / (dmx - (double)floor_x);
+  const double scale32 = scale * 32.0;
+  auto weight = [&](float v) -> unsigned long long { return dr_weight((double)fmaxf(v, floor_x) - dmx, scale32, s.table); };
+  // and for any row: 0 from -46 on (and for NaN)
+  auto weight_any = [&](float v) -> unsigned long long {
+    const double t = ((double)v - dmx) * scale;
+    return v == mx ? 1ull << kDrMass : t > -46.0 ? dr_weight(t, 32.0, s.table) : 0ull;
   };
   auto bin_of = [&](float v) -> int { return min(kDrBins - 1, (int)fminf((mx - v) * 16.0f, 1e6f)); };       // monotone in v (mx = inf: all in the last bin)
   const unsigned long long min_w = min_p > 0.f ? (unsigned long long)ceil(fmin((double)min_p, 1.0) * (double)(1ull << kDrMass)) : 0ull;
@@ -276,7 +302,7 @@ draw_kernel(const DrawArgs a) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
   };
   auto logprob_of = [&](float v, unsigned long long all) -> float {
-    return (float)((v == mx ? 0.0 : ((double)v - dmx) * scale) * 0.69314718055994531 - log((double)all * (1.0 / (double)(1ull << kDrMass))));
+    return (v == mx ? 0.f : (float)(((double)v - dmx) * scale * 0.69314718055994531)) - logf((float)((double)all * (1.0 / (double)(1ull << kDrMass))));
   };
   auto spot_of = [&](unsigned long long all) -> unsigned long long {         // u below 0 or NaN: the first id; 1 and above: the last
     const double spot = (double)u * (double)all;
@@ -288,24 +314,34 @@ draw_kernel(const DrawArgs a) {
   };
 
   const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f;
-  // all values of the block with the whole warp in step: f(values, of how many, index of the first)
-  auto each_vec = [&](auto f) {
-    for (int b = warp * 32; b < nv; b += kDrThreads) {
-      const int j = b + lane;
-      float v[kVec];
-      vec_at(min(j, nv - 1), v);
+  // The block's ids in chunks, in id order: the head, the body by 32 vectors, the tail.  A warp's chunk: f(values, index of the first, chunk), with -inf where the lane has none.
+  const int chunks = (nv + 31) / 32 + 2;                           // at most 397
+  auto chunk_at = [&](int c, float* v) -> int {
+    if (c > 0 && c < chunks - 1) {
+      const int j = (c - 1) * 32 + lane;
+      vec_of(vec_raw(min(j, nv - 1)), v);
+      if (j >= nv) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = j < nv && v[e] == v[e] ? v[e] : -INFINITY;
-      f(v, head + j * kVec);
+        for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
+      }
+      return head + j * kVec;
     }
-    if (warp == 0) {                                               // the ragged ends: fewer than 16 in all
-      float v[kVec];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
-      int i = lane;
-      if (lane < head) v[0] = Key::value(x[i]);
-      else if (lane - head < n - head - body) { i = body + lane; v[0] = Key::value(x[i]); }
-      f(v, i);
+    for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;               // (the ends have fewer than kVec ids: one a lane)
+    const int i = c == 0 ? lane : head + body + lane;
+    if (c == 0 ? lane < head : i < n) v[0] = Key::value(x[i]);
+    return i;
+  };
+  auto each_vec = [&](auto f) {
+    for (int c = 1 + warp; c < chunks - 1; c += kDrWarps) {
+      float v[kVec];
+      const int i = chunk_at(c, v);
+      f(v, i, c);
+    }
+    if (warp < 2) {
+      float v[kVec];
+      const int c = warp == 0 ? 0 : chunks - 1, i = chunk_at(c, v);
+      f(v, i, c);
     }
   };
   auto sum = [&](unsigned long long v) -> unsigned long long {     // over the block
@@ -474,58 +510,97 @@ draw_kernel(const DrawArgs a) {
       }
   };
 
-  // The first id of this block at which the mass of what keeps(key, id) and min-p leave, with `front` in front of the block, exceeds r.  Steps of 512 x 32 ids: a
-  // warp's 1024 in turn, then the warp that holds the place looks closer.
-  auto locate = [&](unsigned long long front, unsigned long long r, unsigned long long all, auto keeps) {
-    auto mass_at = [&](int i) -> unsigned long long {              // (the whole warp)
-      const float v = i < n ? Key::value(x[i]) : -INFINITY;
-      const unsigned long long w = weight_all(v);
-      return i < n && w >= min_w && keeps(Key::of(v), (unsigned)(i0 + i)) ? w : 0ull;
-    };
-    const int run = (n + kDrThreads - 1) / kDrThreads * 32;        // a warp's run of ids
-    unsigned long long mine = 0;
-    for (int b = 0; b < run; b += 64) {
-      mine += mass_at(warp * run + b + lane);
-      if (b + 32 < run) mine += mass_at(warp * run + b + 32 + lane);
+  // Masses of the chunks, of what keeps(key, id) and min-p leave; returns the thread's chunk's.
+  auto weigh = [&](auto keeps) -> unsigned long long {
+    each_vec([&](const float* v, int i, int c) {
+      unsigned long long m = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const unsigned long long w = weight(v[e]);
+        m += (w >= min_w) & keeps(Key::of(v[e]), (unsigned)(i0 + i + e)) ? w : 0ull;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (lane == 0) s.chunk[c] = m;
+    });
+    __syncthreads();
+    return tid < chunks ? s.chunk[tid] : 0ull;
+  };
+  // The first id of this block at which the mass, `front` of it in front of the block and `mine` in the thread's chunk, exceeds r.
+  auto locate = [&](unsigned long long mine, unsigned long long front, unsigned long long r, unsigned long long all, auto keeps) {
+    dr_find(mine, r - front + 1, s);
+    if (warp != 0 || s.found_at < 0) return;
+    front += s.found_before;
+    float v[kVec];
+    const int i = chunk_at(s.found_at, v);
+    unsigned long long w[kVec], m = 0;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      w[e] = weight(v[e]);
+      w[e] = w[e] >= min_w && keeps(Key::of(v[e]), (unsigned)(i0 + i + e)) ? w[e] : 0ull;
+      m += w[e];
     }
+    unsigned long long incl = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) s.warp_mass[warp] = mine;
-    __syncthreads();
-    int w = 0;
-    for (; w < kDrWarps - 1 && r >= front + s.warp_mass[w]; ++w) front += s.warp_mass[w];
-    __syncthreads();
-    // the run again, a piece of it per warp
-    const int piece = (run / 32 + kDrWarps - 1) / kDrWarps * 32;
-    mine = 0;
-    for (int b = warp * piece; b < min(run, (warp + 1) * piece); b += 32) mine += mass_at(w * run + b + lane);
+    for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
+    const unsigned hit = __ballot_sync(0xffffffffu, r < front + incl);
+    if (hit == 0 || lane != __ffs(hit) - 1) return;
+    front += incl - m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) s.warp_mass[warp] = mine;
-    __syncthreads();
-    int p = 0;
-    for (; p < kDrWarps - 1 && r >= front + s.warp_mass[p]; ++p) front += s.warp_mass[p];
-    if (warp != 0) return;
-    for (int b = p * piece; b < min(run, (p + 1) * piece); b += 32) {
-      const int i = w * run + b + lane;
-      unsigned long long incl = mass_at(i);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
-      const unsigned hit = __ballot_sync(0xffffffffu, r < front + incl);
-      if (hit != 0) {
-        if (lane == __ffs(hit) - 1) {
-          a.out[row] = i0 + i;
-          if (a.logprob != nullptr) a.logprob[row] = logprob_of(Key::value(x[i]), all);
-        }
+    for (int e = 0; e < kVec; ++e) {
+      if (r < front + w[e]) {
+        a.out[row] = i0 + i + e;
+        if (a.logprob != nullptr) a.logprob[row] = logprob_of(v[e], all);
         return;
       }
-      front += __shfl_sync(0xffffffffu, incl, 31);
+      front += w[e];
     }
   };
 
+  // The block's candidates, into its own list: logits of `bound` and above that `wanted` takes; those of `special` are counted in cand_own_in as well.  Few vectors hold
+  // one, and few of their logits are one, so each thread goes on by itself.  Plain stores: the first block gets the list in one go.
+  const int cap = kDrCand / C;                                     // a block's places in the first block's list
+  auto collect = [&](float bound, int room, auto wanted, auto special) {
+    auto take = [&](unsigned m, int i) {                           // logits i + the bits of m
+      int q = atomicAdd(&s.cand_own, __popc(m)), n2 = 0;
+      for (; m != 0; m &= m - 1, ++q) {
+        const int at = i + __ffs(m) - 1;
+        const float v = Key::value(x[at]);
+        n2 += special(v);
+        if (q < room) s.cand[q] = make_uint2(Key::of(v), (unsigned)(i0 + at));
+      }
+      if (n2 != 0) atomicAdd(&s.cand_own_in, n2);
+    };
+#pragma unroll 2
+    for (int j = tid; j < nv; j += kDrThreads) {
+      const uint4 raw = vec_raw(j);
+      if (!(vec_max(raw) >= bound)) continue;
+      float v[kVec];
+      vec_of(raw, v);
+      unsigned m = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) m |= (v[e] >= bound && wanted(v[e])) ? 1u << e : 0u;
+      if (m != 0) take(m, head + j * kVec);
+    }
+    ends([&](float v, int i) { if (v >= bound && wanted(v)) take(1u, i); });
+  };
+  auto hand_over = [&](int many, int place) {                      // to the first block
+    if (rank == 0) return;
+    for (int q = tid; q < many; q += kDrThreads) dr_put64(&s.cand[place + q], 0, *reinterpret_cast<const unsigned long long*>(&s.cand[q]));
+  };
+  auto settle = [&](unsigned long long target) {                   // the first block finishes with the lists of all
+    int found = 0;
+    for (int c = 0; c < C; ++c) found += s.cand_n[c];
+    finish(found, target, [&](int q) -> uint2 {
+      int c = 0;
+      while (q >= s.cand_n[c]) q -= s.cand_n[c++];
+      return s.cand[c * cap + q];
+    });
+  };
+
   // ---- rows with a top-k: pruned.  With min-p alone the bound is known
-  if (has_k ? top_k <= kDrPrune : !has_p && min_w != 0) {
-    if (tid == 0) s.cand_own = 0;
+  if (plain && (has_k ? top_k <= kDrPrune : !has_p && min_w != 0)) {
+    if (tid == 0) { s.cand_own = 0; s.cand_own_in = 0; }
     float bound = fmaxf(mx + temp * logf(fminf(min_p, 1.0f)) - fmaf(fabsf(mx), 2.5e-7f, 1e-5f) - temp * 1e-5f, -FLT_MAX);
     if (!has_k) __syncthreads();
     if (has_k && rank == 0) {
@@ -547,57 +622,32 @@ draw_kernel(const DrawArgs a) {
       dr_cluster_sync();
       bound = s.bound;
     }
-    const int cap = kDrCand / C;                                   // places of a block
-    each_vec([&](const float* v, int i) {
-      float most = v[0];
-#pragma unroll
-      for (int e = 1; e < kVec; ++e) most = fmaxf(most, v[e]);
-      if (!__any_sync(0xffffffffu, most >= bound)) return;
-      int mine = 0;                                                // one addition to the block's count per warp and vector
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) mine += v[e] >= bound;
-      int incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += y; }
-      int at = 0;
-      if (lane == 31) at = atomicAdd(&s.cand_own, incl);
-      at = __shfl_sync(0xffffffffu, at, 31) + incl - mine;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (v[e] >= bound) {
-          if (at < cap) dr_put64(&s.cand[rank * cap + at], 0, (unsigned long long)(unsigned)(i0 + i + e) << 32 | Key::of(v[e]));
-          ++at;
-        }
-    });
+    collect(bound, cap, [](float) { return true; }, [](float) { return 0; });
     __syncthreads();
+    hand_over(min(s.cand_own, cap), rank * cap);
     if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
     dr_cluster_sync();
     bool settled = true;
     for (int c = 0; c < C; ++c) settled &= s.cand_n[c] <= cap;
     if (settled) {
       if (rank != 0) return;                                       // (nobody reads this block's shared memory any more)
-      int found = 0;
-      for (int c = 0; c < C; ++c) found += s.cand_n[c];
-      finish(found, 0, [&](int q) -> uint2 {
-        int c = 0;
-        while (q >= s.cand_n[c]) q -= s.cand_n[c++];
-        return s.cand[c * cap + q];
-      });
+      settle(0);
       return;
     }
   }
   // ---- rows with a top-p alone: one pass for all weights and their histogram, over steps that suit the row: to twice the depth of its lowest group, at most
   // 45 halvings.  The step of the cut is then known, with the mass in front of it.
   bool by_min_p = false;
-  if (has_p && !has_k) {
+  if (plain && has_p && !has_k) {
     const float depth = fminf(2.0f * (mx - low), 32.0f * temp), steps = kDrBins / depth;
-    auto step_of = [&](float v) -> int { return max(0, min(kDrBins - 1, (int)fminf((mx - v) * steps, 1e6f))); };      // monotone in v
-    s.count[0][tid] = 0; s.lo[0][tid] = 0; s.hi[0][tid] = 0;
+    auto step_of = [&](float v) -> int { return max(0, min(kDrBins - 1, (int)((mx - v) * steps))); };      // monotone in v
+    s.lo[0][tid] = 0; s.hi[0][tid] = 0;
+    if (tid == 0) { s.cand_own = 0; s.cand_own_in = 0; }
     __syncthreads();
-    each_vec([&](const float* v, int) {
+    each_vec([&](const float* v, int, int) {
       unsigned long long w[kVec];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) w[e] = weight_all(v[e]);
+      for (int e = 0; e < kVec; ++e) w[e] = weight(v[e]);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         if (w[e] == 0) continue;
@@ -605,99 +655,79 @@ draw_kernel(const DrawArgs a) {
         const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[0][b], l);
         const unsigned h = (unsigned)(w[e] >> 32) + (old + l < old ? 1u : 0u);
         if (h != 0) atomicAdd(&s.hi[0][b], h);
-        atomicAdd(&s.count[0][b], 1u);
       }
     });
     __syncthreads();
     dr_cluster_sync();
-    // The blocks' histograms, four steps of one block a turn (16-byte loads; single ones took 7500 cycles, these 3000): lanes 8 apart hold the same block.
-    unsigned long long at = 0;
-    unsigned n_at[2 * 4];
-    const int block = lane & 7;
-    unsigned long long part[2 * 4];
+    // The first block adds up the histograms, four steps of one block a turn (16-byte loads; lanes 8 apart hold the same block), and tells the step of the cut.
+    if (rank == 0) {
+      unsigned long long at;
+      if (C == 1) at = ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid];
+      else {
+        const int block = lane & 7;
+        unsigned long long part[2 * 4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int quad = (tid >> 3) + k * (kDrThreads / 8);
-      uint4 c4 = make_uint4(0, 0, 0, 0), l4 = c4, h4 = c4;
-      if (block < C) { c4 = dr_peer128(&s.count[0][quad * 4], block); l4 = dr_peer128(&s.lo[0][quad * 4], block); h4 = dr_peer128(&s.hi[0][quad * 4], block); }
-      n_at[k * 4] = c4.x; n_at[k * 4 + 1] = c4.y; n_at[k * 4 + 2] = c4.z; n_at[k * 4 + 3] = c4.w;
-      part[k * 4] = (unsigned long long)h4.x << 32; part[k * 4 + 1] = (unsigned long long)h4.y << 32; part[k * 4 + 2] = (unsigned long long)h4.z << 32;
-      part[k * 4 + 3] = (unsigned long long)h4.w << 32;
-      part[k * 4] += l4.x; part[k * 4 + 1] += l4.y; part[k * 4 + 2] += l4.z; part[k * 4 + 3] += l4.w;
+        for (int k = 0; k < 2; ++k) {
+          const int quad = (tid >> 3) + k * (kDrThreads / 8);
+          uint4 l4 = make_uint4(0, 0, 0, 0), h4 = l4;
+          if (block < C) { l4 = dr_peer128(&s.lo[0][quad * 4], block); h4 = dr_peer128(&s.hi[0][quad * 4], block); }
+          part[k * 4] = ((unsigned long long)h4.x << 32) + l4.x; part[k * 4 + 1] = ((unsigned long long)h4.y << 32) + l4.y;
+          part[k * 4 + 2] = ((unsigned long long)h4.z << 32) + l4.z; part[k * 4 + 3] = ((unsigned long long)h4.w << 32) + l4.w;
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int b = ((tid >> 3) + (k >> 2) * (kDrThreads / 8)) * 4 + (k & 3);
+          if (block == k) { s.lo[1][b] = (unsigned)part[k]; s.hi[1][b] = (unsigned)(part[k] >> 32); }
+        }
+        __syncthreads();
+        at = (unsigned long long)s.hi[1][tid] << 32 | s.lo[1][tid];
+      }
+      const unsigned long long goal = top_p_target(sum(at));
+      dr_find(at, goal, s);
+      if (tid < C) { dr_put32(&s.cut, tid, (uint32_t)s.found_at); dr_put64(&s.cut_before, tid, s.found_before); dr_put64(&s.cut_target, tid, goal); }
     }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                                  // (sums: in the other parity, which no other block reads)
-      const int b = ((tid >> 3) + (k >> 2) * (kDrThreads / 8)) * 4 + (k & 3);
-      if (block == k) { s.lo[1][b] = (unsigned)part[k]; s.hi[1][b] = (unsigned)(part[k] >> 32); }
-    }
-    __syncthreads();
-    at = (unsigned long long)s.hi[1][tid] << 32 | s.lo[1][tid];
-    const unsigned long long target = top_p_target(sum(at));
-    dr_find(at, target, s);
-    int cut = s.found_at;
-    const unsigned long long before = s.found_before;
+    dr_cluster_sync();
+    const unsigned long long target = s.cut_target, before = s.cut_before;
+    const int full_cut = s.cut;
     // min-p may cut higher up: what lies more than a step below its weight is kept by neither
     const float min_off = min_w != 0 ? -temp * logf(fminf(min_p, 1.0f)) : 0.f, slack = fmaf(fabsf(mx) + depth + min_off, 1e-6f, 1e-4f);
-    const int full_cut = cut, min_step = min_w != 0 ? step_of(mx - min_off - slack) + 1 : kDrBins;         // no logit of this step or below has the weight
-    const int all_step = min_w != 0 ? step_of(mx - min_off + slack) : kDrBins;                             // all logits above this step have it
-    if (cut > 0) cut = min(cut, min_step);
-    // how many of each block lie above the cut's step, and in it
-    if (tid < 8) { s.cand_n[tid] = 0; s.cand_in[tid] = 0; }
-    __syncthreads();
-    {
-      unsigned up = 0, in = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int b = ((tid >> 3) + (k >> 2) * (kDrThreads / 8)) * 4 + (k & 3);
-        if (b < cut) up += n_at[k];
-        if (b == cut) in += n_at[k];
-      }
-      up += __shfl_xor_sync(0xffffffffu, up, 8); up += __shfl_xor_sync(0xffffffffu, up, 16);
-      in += __shfl_xor_sync(0xffffffffu, in, 8); in += __shfl_xor_sync(0xffffffffu, in, 16);
-      if (lane < 8) {
-        if (up != 0) atomicAdd(&s.cand_n[block], (int)up);
-        if (in != 0) atomicAdd(&s.cand_in[block], (int)in);
-      }
-    }
-    __syncthreads();
-    int above = 0, in_cut = 0, my_above = 0, my_cut = 0;
-    for (int c = 0; c < C; ++c) {
-      if (c == rank) { my_above = above + in_cut; my_cut = in_cut; }
-      above += s.cand_n[c]; in_cut += s.cand_in[c];
-    }
-    const bool few = above + in_cut <= kDrCand, some = in_cut <= kDrCand && full_cut < all_step;      // (some: min-p leaves all that top-p leaves)
-    by_min_p = !few && min_step < full_cut && full_cut > 0;                    // min-p cuts first: nothing of top-p is left to do
-    if (cut >= 0 && cut < kDrBins - 1 && (few || some) && !by_min_p) {
-      // the candidates, or those of the cut's step, to the first block; each block keeps its own of the latter too
-      if (tid == 0) s.cand_own = 0;
-      __syncthreads();
-      const int base = few ? my_above : my_cut;
+    const int min_step = min_w != 0 ? step_of(mx - min_off - slack) + 1 : kDrBins;         // no logit of this step or below has the weight
+    const int all_step = min_w != 0 ? step_of(mx - min_off + slack) : kDrBins;             // all logits above this step have it
+    const int cut = full_cut > 0 ? min(full_cut, min_step) : full_cut;
+    if (cut >= 0 && cut < kDrBins - 1) {
+      // the candidates to the first block
       const float bound = fmaxf(mx - (cut + 1) / steps - fmaf(fabsf(mx) + depth, 1e-6f, 1e-4f), -FLT_MAX);       // (a little below the step: which step a logit is of is asked anew)
-      each_vec([&](const float* v, int i) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          if (!(v[e] >= bound)) continue;
-          const int b = step_of(v[e]);
-          if (b > cut || (!few && b < cut) || weight(v[e]) == 0) continue;
-          const int k = atomicAdd(&s.cand_own, 1);
-          const unsigned long long entry = (unsigned long long)(unsigned)(i0 + i + e) << 32 | Key::of(v[e]);
-          if (base + k < kDrCand) dr_put64(&s.cand[base + k], 0, entry);
-          if (!few && rank != 0 && k < kDrCand) s.cand[k] = make_uint2((unsigned)entry, (unsigned)(entry >> 32));
-        }
-      });
+      collect(bound, cap, [](float) { return true; }, [&](float v) { return (int)(step_of(v) == cut); });      // (with some of the next step: they lie behind the cut)
       __syncthreads();
-      const int own = min(s.cand_own, kDrCand);
+      hand_over(min(s.cand_own, cap), rank * cap);
+      if (tid < C) { dr_put32(&s.cand_n[rank], tid, s.cand_own); dr_put32(&s.cand_in[rank], tid, s.cand_own_in); }
       dr_cluster_sync();
+      bool few = true;
+      int in_cut = 0, my_cut = 0;
+      for (int c = 0; c < C; ++c) {
+        few &= s.cand_n[c] <= cap;
+        if (c == rank) my_cut = in_cut;
+        in_cut += s.cand_in[c];
+      }
       if (few) {
-        if (rank != 0) return;
-        finish(above + in_cut, target, [&](int q) { return s.cand[q]; });
+        if (rank == 0) settle(target);
         return;
       }
+      by_min_p = min_step < full_cut;                              // min-p cuts first: nothing of top-p is left to do
+      if (!by_min_p && in_cut <= kDrCand && full_cut < all_step) { // (the second: min-p leaves all that top-p leaves)
+      // too many: those of the cut's step, of which each block keeps its own too
+      if (tid == 0) s.cand_own = 0;
+      __syncthreads();
+      collect(bound, kDrCand, [&](float v) { return step_of(v) == cut; }, [](float) { return 0; });
+      __syncthreads();
+      const int own = min(s.cand_own, kDrCand);
+      hand_over(own, my_cut);
+      dr_cluster_sync();
       // Many above the cut: the first block finds the cut in its step, every block then knows its kept mass, and the block in which the draw falls goes through
       // its logits once more.
       if (rank == 0) {
@@ -755,7 +785,7 @@ draw_kernel(const DrawArgs a) {
       }
       dr_cluster_sync();
       const unsigned tau = s.tau, last = s.last;
-      auto keeps = [&](unsigned key, unsigned id) { return key > tau || (key == tau && id <= last); };
+      auto keeps = [&](unsigned key, unsigned id) -> bool { return (key > tau) | ((key == tau) & (id <= last)); };
       unsigned long long mine = tid < cut ? ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid] : 0ull;
       for (int q = tid; q < own; q += kDrThreads) {
         const uint2 e = s.cand[q];
@@ -768,25 +798,22 @@ draw_kernel(const DrawArgs a) {
       for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
       const unsigned long long r = spot_of(all);
       if (r < front || r >= front + mine) return;
-      locate(front, r, all, keeps);
+      locate(weigh(keeps), front, r, all, keeps);
       return;
+      }
     }
   }
   // ---- rows without a limit, or with min-p alone (too many for the first block): one pass for the blocks' masses
-  if (!has_k && (!has_p || by_min_p)) {
-    unsigned long long mine = 0;
-    each_vec([&](const float* v, int) {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) { const unsigned long long w = weight_all(v[e]); mine += w >= min_w ? w : 0ull; }
-    });
-    mine = sum(mine);
+  if (plain && !has_k && (!has_p || by_min_p)) {
+    auto keeps = [](unsigned, unsigned) { return true; };
+    const unsigned long long chunk = weigh(keeps), mine = sum(chunk);
     if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
     dr_cluster_sync();
     unsigned long long all = 0, front = 0;
     for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
     const unsigned long long r = spot_of(all);
     if (r < front || r >= front + mine) return;
-    locate(front, r, all, [&](unsigned, unsigned) { return true; });
+    locate(chunk, front, r, all, keeps);
     return;
   }
 
@@ -867,7 +894,7 @@ draw_kernel(const DrawArgs a) {
         const unsigned off = min(Key::of(e) - k0, range);
         in = in && bin_of(e) == bin && (bits >= 32 ? 0u : off >> bits) == prefix;
         if (!mass) put((off >> shift) & 255, in);
-        else if (in && Key::of(e) > tau) { const unsigned long long w = weight(e); if (w) put_mass((off >> shift) & 255, w); }
+        else if (in && Key::of(e) > tau) { const unsigned long long w = weight_any(e); if (w) put_mass((off >> shift) & 255, w); }
       });
       __syncthreads();
       dr_cluster_sync();
@@ -911,7 +938,7 @@ draw_kernel(const DrawArgs a) {
       const unsigned long long above = cut(false, (unsigned long long)top_k, 0, 0, -1);
       ties = (unsigned long long)top_k - above;
       const float vt = value_of(tau);
-      tie_mass = ties * weight(vt);
+      tie_mass = ties * weight_any(vt);
       tau_bin = bin_of(vt);
     }
     ++step;
@@ -919,7 +946,7 @@ draw_kernel(const DrawArgs a) {
   // ---- top-p of what is left
   if (has_p) {
     clear(true);
-    each([&](float e, bool in) { const unsigned long long w = weight_all(e); if (in && Key::of(e) > tau && w) put_mass(bin_of(e), w); });
+    each([&](float e, bool in) { const unsigned long long w = weight_any(e); if (in && Key::of(e) > tau && w) put_mass(bin_of(e), w); });
     __syncthreads();
     dr_cluster_sync();
     unsigned long long all = gather(tid, true);
@@ -934,18 +961,18 @@ draw_kernel(const DrawArgs a) {
     const unsigned old_tau = tau;
     const unsigned long long old_ties = ties;
     const unsigned long long above = cut(true, target, old_tau, tie_mass, tau_bin);
-    const unsigned long long wt = weight(value_of(tau));
+    const unsigned long long wt = weight_any(value_of(tau));
     ties = wt > 0 ? (target - above + wt - 1) / wt : 0;
     if (tau == old_tau) ties = min(ties, old_ties);
     ++step;
   }
   // ---- the draw, in id order: blocks, warps, sixteenths of a warp's ids, ids
-  unsigned long long wt = ties > 0 ? weight(value_of(tau)) : 0;
+  unsigned long long wt = ties > 0 ? weight_any(value_of(tau)) : 0;
   if (wt < min_w) wt = 0;
   auto kept = [&](float e, bool in, bool& tie) -> unsigned long long {       // (the whole warp)
     const unsigned k = Key::of(e);
     tie = in && k == tau;
-    const unsigned long long w = weight_all(e);
+    const unsigned long long w = weight_any(e);
     return in && k > tau && w >= min_w ? w : 0;
   };
   unsigned long long mass = 0;
