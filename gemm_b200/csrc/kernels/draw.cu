@@ -65,8 +65,8 @@ struct alignas(16) DrawShared {
   int abort_flag;
   float bound;                             // written by the first block into all
   int cand_n[8];                           // of every block, written by it into all
-  int cand_in[8];
-  int cand_own, cand_own_in;
+  int cand_own;
+  int many;                                // in the steps up to the cut, about
   int cut;                                 // of top-p: its step, the mass in front of the step, and the mass in front of which it keeps (written by the first block into all)
   unsigned long long cut_before, cut_target;
   unsigned tau, last;                      // written by the first block into all: the cut
@@ -212,6 +212,7 @@ draw_kernel(const DrawArgs a) {
 
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces.  (fmaxf passes over NaN.)
+  const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f, few_groups = has_k && top_k <= kDrThreads / 8;      // eight groups for each logit that top-k keeps
   float mx = -INFINITY, low = INFINITY;
   {
     constexpr int kPieces = kDrGroups / kDrThreads;
@@ -240,11 +241,24 @@ draw_kernel(const DrawArgs a) {
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       if (p >= pieces) break;
-      float* to = &s.group[(rank * pieces + p) * kDrThreads + tid];
-      if (rank == 0) *to = gm[p];                                  // (a store through the cluster's network takes several times as long, to the own block too)
-      else dr_put32(to, 0, __float_as_uint(gm[p]));
       mx = fmaxf(mx, gm[p]);
       if (gm[p] > -INFINITY) low = fminf(low, gm[p]);
+    }
+    auto put_group = [&](int at, float v) {                        // (a store through the cluster's network takes several times as long, to the own block too)
+      if (rank == 0) s.group[at] = v;
+      else dr_put32(&s.group[at], 0, __float_as_uint(v));
+    };
+    if (few_groups) {                                              // 512 in all: a thread's maxima in one, and those of C threads
+#pragma unroll
+      for (int p = 1; p < kPieces; ++p) if (p < pieces) gm[0] = fmaxf(gm[0], gm[p]);
+      for (int o = 1; o < C; o <<= 1) gm[0] = fmaxf(gm[0], __shfl_xor_sync(0xffffffffu, gm[0], o));
+      if ((tid & (C - 1)) == 0) put_group(rank * (kDrThreads / C) + tid / C, gm[0]);
+    } else if (has_k) {
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        if (p >= pieces) break;
+        put_group((rank * pieces + p) * kDrThreads + tid, gm[p]);
+      }
     }
   }
   mx = warp_max(mx);
@@ -313,7 +327,6 @@ draw_kernel(const DrawArgs a) {
     return goal >= (double)all ? all : goal < 1.0 ? 1ull : (unsigned long long)goal;
   };
 
-  const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f;
   // The block's ids in chunks, in id order: the head, the body by 32 vectors, the tail.  A warp's chunk: f(values, index of the first, chunk), with -inf where the lane has none.
   const int chunks = (nv + 31) / 32 + 2;                           // at most 397
   auto chunk_at = [&](int c, float* v) -> int {
@@ -510,14 +523,14 @@ draw_kernel(const DrawArgs a) {
       }
   };
 
-  // Masses of the chunks, of what keeps(key, id) and min-p leave; returns the thread's chunk's.
+  // Masses of the chunks, of what keeps(logit, id) and min-p leave; returns the thread's chunk's.
   auto weigh = [&](auto keeps) -> unsigned long long {
     each_vec([&](const float* v, int i, int c) {
       unsigned long long m = 0;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const unsigned long long w = weight(v[e]);
-        m += (w >= min_w) & keeps(Key::of(v[e]), (unsigned)(i0 + i + e)) ? w : 0ull;
+        m += (w >= min_w) & keeps(v[e], (unsigned)(i0 + i + e)) ? w : 0ull;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
@@ -537,7 +550,7 @@ draw_kernel(const DrawArgs a) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
       w[e] = weight(v[e]);
-      w[e] = w[e] >= min_w && keeps(Key::of(v[e]), (unsigned)(i0 + i + e)) ? w[e] : 0ull;
+      w[e] = w[e] >= min_w && keeps(v[e], (unsigned)(i0 + i + e)) ? w[e] : 0ull;
       m += w[e];
     }
     unsigned long long incl = m;
@@ -557,19 +570,17 @@ draw_kernel(const DrawArgs a) {
     }
   };
 
-  // The block's candidates, into its own list: logits of `bound` and above that `wanted` takes; those of `special` are counted in cand_own_in as well.  Few vectors hold
+  // The block's candidates, into its own list: logits of `bound` and above that `wanted` takes; Few vectors hold
   // one, and few of their logits are one, so each thread goes on by itself.  Plain stores: the first block gets the list in one go.
   const int cap = kDrCand / C;                                     // a block's places in the first block's list
-  auto collect = [&](float bound, int room, auto wanted, auto special) {
+  auto collect = [&](float bound, int room, auto wanted) {
     auto take = [&](unsigned m, int i) {                           // logits i + the bits of m
-      int q = atomicAdd(&s.cand_own, __popc(m)), n2 = 0;
+      int q = atomicAdd(&s.cand_own, __popc(m));
       for (; m != 0; m &= m - 1, ++q) {
         const int at = i + __ffs(m) - 1;
         const float v = Key::value(x[at]);
-        n2 += special(v);
         if (q < room) s.cand[q] = make_uint2(Key::of(v), (unsigned)(i0 + at));
       }
-      if (n2 != 0) atomicAdd(&s.cand_own_in, n2);
     };
 #pragma unroll 2
     for (int j = tid; j < nv; j += kDrThreads) {
@@ -600,14 +611,14 @@ draw_kernel(const DrawArgs a) {
 
   // ---- rows with a top-k: pruned.  With min-p alone the bound is known
   if (plain && (has_k ? top_k <= kDrPrune : !has_p && min_w != 0)) {
-    if (tid == 0) { s.cand_own = 0; s.cand_own_in = 0; }
+    if (tid == 0) s.cand_own = 0;
     float bound = fmaxf(mx + temp * logf(fminf(min_p, 1.0f)) - fmaf(fabsf(mx), 2.5e-7f, 1e-5f) - temp * 1e-5f, -FLT_MAX);
     if (!has_k) __syncthreads();
     if (has_k && rank == 0) {
       s.count[0][tid] = 0;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kDrGroups / kDrThreads; ++i) {
+      for (int i = 0; i < (few_groups ? 1 : kDrGroups / kDrThreads); ++i) {
         const float v = s.group[i * kDrThreads + tid];
         if (v > mx - kDrBins / 16.0f) atomicAdd(&s.count[0][bin_of(v)], 1u);
       }
@@ -622,7 +633,7 @@ draw_kernel(const DrawArgs a) {
       dr_cluster_sync();
       bound = s.bound;
     }
-    collect(bound, cap, [](float) { return true; }, [](float) { return 0; });
+    collect(bound, cap, [](float) { return true; });
     __syncthreads();
     hand_over(min(s.cand_own, cap), rank * cap);
     if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
@@ -642,7 +653,7 @@ draw_kernel(const DrawArgs a) {
     const float depth = fminf(2.0f * (mx - low), 32.0f * temp), steps = kDrBins / depth;
     auto step_of = [&](float v) -> int { return max(0, min(kDrBins - 1, (int)((mx - v) * steps))); };      // monotone in v
     s.lo[0][tid] = 0; s.hi[0][tid] = 0;
-    if (tid == 0) { s.cand_own = 0; s.cand_own_in = 0; }
+    if (tid == 0) s.cand_own = 0;
     __syncthreads();
     each_vec([&](const float* v, int, int) {
       unsigned long long w[kVec];
@@ -659,6 +670,10 @@ draw_kernel(const DrawArgs a) {
     });
     __syncthreads();
     dr_cluster_sync();
+    // min-p may cut higher up: what lies more than a step below its weight is kept by neither
+    const float min_off = min_w != 0 ? -temp * logf(fminf(min_p, 1.0f)) : 0.f, slack = fmaf(fabsf(mx) + depth + min_off, 1e-6f, 1e-4f);
+    const int min_step = min_w != 0 ? step_of(mx - min_off - slack) + 1 : kDrBins;         // no logit of this step or below has the weight
+    const int all_step = min_w != 0 ? step_of(mx - min_off + slack) : kDrBins;             // all logits above this step have it
     // The first block adds up the histograms, four steps of one block a turn (16-byte loads; lanes 8 apart hold the same block), and tells the step of the cut.
     if (rank == 0) {
       unsigned long long at;
@@ -689,45 +704,50 @@ draw_kernel(const DrawArgs a) {
       }
       const unsigned long long goal = top_p_target(sum(at));
       dr_find(at, goal, s);
-      if (tid < C) { dr_put32(&s.cut, tid, (uint32_t)s.found_at); dr_put64(&s.cut_before, tid, s.found_before); dr_put64(&s.cut_target, tid, goal); }
+      // About how many lie in the steps up to the cut: a step's mass by the weight in its middle (a step is a tenth of a halving or less).
+      const float halvings = (float)scale * depth * (1.0f / kDrBins);
+      const unsigned long long many = sum(tid <= min(s.found_at, min_step) ? (unsigned long long)((float)at * exp2f((tid + 0.5f) * halvings - kDrMass)) : 0ull);
+      if (tid < C) {
+        dr_put32(&s.many, tid, (uint32_t)min(many, 0x7fffffffull));
+        dr_put32(&s.cut, tid, (uint32_t)s.found_at); dr_put64(&s.cut_before, tid, s.found_before); dr_put64(&s.cut_target, tid, goal);
+      }
     }
     dr_cluster_sync();
     const unsigned long long target = s.cut_target, before = s.cut_before;
     const int full_cut = s.cut;
-    // min-p may cut higher up: what lies more than a step below its weight is kept by neither
-    const float min_off = min_w != 0 ? -temp * logf(fminf(min_p, 1.0f)) : 0.f, slack = fmaf(fabsf(mx) + depth + min_off, 1e-6f, 1e-4f);
-    const int min_step = min_w != 0 ? step_of(mx - min_off - slack) + 1 : kDrBins;         // no logit of this step or below has the weight
-    const int all_step = min_w != 0 ? step_of(mx - min_off + slack) : kDrBins;             // all logits above this step have it
     const int cut = full_cut > 0 ? min(full_cut, min_step) : full_cut;
     if (cut >= 0 && cut < kDrBins - 1) {
       // the candidates to the first block
       const float bound = fmaxf(mx - (cut + 1) / steps - fmaf(fabsf(mx) + depth, 1e-6f, 1e-4f), -FLT_MAX);       // (a little below the step: which step a logit is of is asked anew)
-      collect(bound, cap, [](float) { return true; }, [&](float v) { return (int)(step_of(v) == cut); });      // (with some of the next step: they lie behind the cut)
-      __syncthreads();
-      hand_over(min(s.cand_own, cap), rank * cap);
-      if (tid < C) { dr_put32(&s.cand_n[rank], tid, s.cand_own); dr_put32(&s.cand_in[rank], tid, s.cand_own_in); }
-      dr_cluster_sync();
-      bool few = true;
-      int in_cut = 0, my_cut = 0;
-      for (int c = 0; c < C; ++c) {
-        few &= s.cand_n[c] <= cap;
-        if (c == rank) my_cut = in_cut;
-        in_cut += s.cand_in[c];
-      }
+      bool few = s.many <= kDrCand + kDrCand / 8;                  // (many that are not too many after all take the other way)
       if (few) {
-        if (rank == 0) settle(target);
-        return;
+        collect(bound, cap, [](float) { return true; });           // (with some of the next step: they lie behind the cut)
+        __syncthreads();
+        hand_over(min(s.cand_own, cap), rank * cap);
+        if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
+        dr_cluster_sync();
+        for (int c = 0; c < C; ++c) few &= s.cand_n[c] <= cap;
+        if (few) {
+          if (rank == 0) settle(target);
+          return;
+        }
+        dr_cluster_sync();                                         // (cand_n is written again)
       }
       by_min_p = min_step < full_cut;                              // min-p cuts first: nothing of top-p is left to do
-      if (!by_min_p && in_cut <= kDrCand && full_cut < all_step) { // (the second: min-p leaves all that top-p leaves)
-      // too many: those of the cut's step, of which each block keeps its own too
-      if (tid == 0) s.cand_own = 0;
-      __syncthreads();
-      collect(bound, kDrCand, [&](float v) { return step_of(v) == cut; }, [](float) { return 0; });
-      __syncthreads();
-      const int own = min(s.cand_own, kDrCand);
-      hand_over(own, my_cut);
-      dr_cluster_sync();
+      bool settled = !by_min_p && full_cut < all_step;             // (the second: min-p leaves all that top-p leaves)
+      if (settled) {
+        // too many: those of the cut's step, of which each block keeps its own too
+        if (tid == 0) s.cand_own = 0;
+        __syncthreads();
+        collect(bound, cap, [&](float v) { return step_of(v) == cut; });
+        __syncthreads();
+        hand_over(min(s.cand_own, cap), rank * cap);
+        if (tid < C) dr_put32(&s.cand_n[rank], tid, s.cand_own);
+        dr_cluster_sync();
+        for (int c = 0; c < C; ++c) settled &= s.cand_n[c] <= cap;
+      }
+      if (settled) {
+      const int own = s.cand_own;
       // Many above the cut: the first block finds the cut in its step, every block then knows its kept mass, and the block in which the draw falls goes through
       // its logits once more.
       if (rank == 0) {
@@ -736,11 +756,12 @@ draw_kernel(const DrawArgs a) {
         unsigned long long w[kOwn];
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
-          const int q = k * kDrThreads + tid;
-          const uint2 e = q < in_cut ? s.cand[q] : make_uint2(0u, 0u);
+          const int q = k * kDrThreads + tid;                      // of the list: place q - c cap of block c
+          const bool in = (q & (cap - 1)) < s.cand_n[q / cap];
+          const uint2 e = in ? s.cand[q] : make_uint2(0u, 0u);
           key[k] = e.x; id[k] = e.y;
-          w[k] = q < in_cut ? weight(value_of(e.x)) : 0ull;
-          if (q < in_cut) { least = min(least, e.x); most = max(most, e.x); }
+          w[k] = in ? weight(value_of(e.x)) : 0ull;
+          if (in) { least = min(least, e.x); most = max(most, e.x); }
         }
         least = __reduce_min_sync(0xffffffffu, least);
         most = __reduce_max_sync(0xffffffffu, most);
@@ -754,6 +775,12 @@ draw_kernel(const DrawArgs a) {
         unsigned long long goal = target - before;
 #pragma unroll
         for (int by_id = 0; by_id < 2; ++by_id) {
+          if (by_id) {
+            unsigned long long same = 0;
+#pragma unroll
+            for (int k = 0; k < kOwn; ++k) same += key[k] == found[0];
+            if (sum(same) == 1) { found[1] = 0xffffffffu; break; }
+          }
           const unsigned first = by_id ? 0u : least, range = by_id ? (unsigned)a.vocab - 1 : most - least;
           unsigned prefix = 0;
           for (int bits = 32 - __clz(range); bits > 0;) {
@@ -785,11 +812,12 @@ draw_kernel(const DrawArgs a) {
       }
       dr_cluster_sync();
       const unsigned tau = s.tau, last = s.last;
-      auto keeps = [&](unsigned key, unsigned id) -> bool { return (key > tau) | ((key == tau) & (id <= last)); };
+      const float tau_x = value_of(tau);
+      auto keeps = [&](float v, unsigned id) -> bool { return (v > tau_x) | ((v == tau_x) & (id <= last)); };
       unsigned long long mine = tid < cut ? ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid] : 0ull;
       for (int q = tid; q < own; q += kDrThreads) {
         const uint2 e = s.cand[q];
-        if (keeps(e.x, e.y)) mine += weight(value_of(e.x));
+        if (keeps(value_of(e.x), e.y)) mine += weight(value_of(e.x));
       }
       mine = sum(mine);
       if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
@@ -805,7 +833,7 @@ draw_kernel(const DrawArgs a) {
   }
   // ---- rows without a limit, or with min-p alone (too many for the first block): one pass for the blocks' masses
   if (plain && !has_k && (!has_p || by_min_p)) {
-    auto keeps = [](unsigned, unsigned) { return true; };
+    auto keeps = [](float, unsigned) { return true; };
     const unsigned long long chunk = weigh(keeps), mine = sum(chunk);
     if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
     dr_cluster_sync();
