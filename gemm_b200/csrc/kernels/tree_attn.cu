@@ -24,7 +24,7 @@ namespace gb {
 constexpr int kTaThreads = 384;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads; 11: segments
 constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, one in which rows are joined and put in order, the rest is the ring
 constexpr int kTaSegs = 4;          // segments handed out ahead
-constexpr int kTaSmem = 1024 + kTaTiles * 32768 + 2048;
+constexpr int kTaSmem = kTaTiles * 32768 + 3072;      // (all there is)
 
 struct TreeAttnArgs {
   const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
@@ -91,10 +91,9 @@ __device__ __forceinline__ int ta_piece_of(long long at, long long total, int ac
 struct TaWalk {
   TaPiece p;
   TaSeq q;
-  int at, nth;
+  int nth;
   __device__ __forceinline__ bool next(const TreeAttnArgs& a, TaSeg& s) {
     while (p.left > 0) {
-      if (at != p.seq) { q.load(a, p.seq); at = p.seq; }
       const int kvh = p.item / q.pairs, tile = (p.item - kvh * q.pairs) * a.pair, n_tiles = min(a.pair, q.tiles - tile), w = a.whole ? 1 : n_tiles;
       const int cost = q.head + w * q.units;
       const int take = (int)min((long long)(cost - p.off), p.left);
@@ -108,7 +107,7 @@ struct TaWalk {
         p.off = 0;
         if (++p.item == q.items) {
           p.item = 0;
-          if (p.left > 0) do { ++p.seq; q.load(a, p.seq); at = p.seq; } while (q.items == 0 && p.seq + 1 < a.n_seqs);
+          if (p.left > 0) do { ++p.seq; q.load(a, p.seq); } while (q.items == 0 && p.seq + 1 < a.n_seqs);
         }
       }
       if (b1 == b0) continue;                                      // (the piece ends or begins beside the item's first or last block)
@@ -133,6 +132,16 @@ __device__ __forceinline__ bool bar256_and(bool pred) {
   return r != 0;
 }
 
+// A bounded wait: polls, and then the one that looks at the clock, which is not worth its place in the instruction cache at each wait.
+__device__ __noinline__ bool ta_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, KernelStatus* st, int where, int aux) {
+  return mbar_wait(bar, parity, abort_flag, st, where, aux);
+}
+__device__ __forceinline__ bool ta_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, KernelStatus* st, int where, int aux) {
+#pragma unroll 1
+  for (int it = 0; it < 256; ++it) if (mbar_try_wait(bar, parity)) return true;
+  return ta_wait_long(bar, parity, abort_flag, st, where, aux);
+}
+
 // Bits [at, at + 32) of a node's mask row (at may be negative: zeros in front).
 __device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int words, int at) {
   if (at <= -32 || at >= words * 64) return 0;
@@ -152,37 +161,37 @@ __device__ __forceinline__ uint64_t pair2(float lo, float hi) { uint64_t r; asm(
 __device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
-// 64 bytes of a row in two stores.
-__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-
 // One block's step of a softmax thread: NC = 128 / FOLD of the block's scores, from column `at` on.  Returns the factor that the sum and O were scaled by in `l`, `m`.
 template <int DV, int FOLD>
 __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first, bool edge, const uint32_t* see, float& m, float& l) {
   constexpr float kTau = 8.0f;         // O and the sum are rescaled only where a row's maximum has grown by more than 2^kTau
-  constexpr int NC = 128 / FOLD, CH = NC < 64 ? NC : 64;
+  constexpr int NC = 128 / FOLD;
   const uint32_t s_at = s_t + fold * NC;
-  float sv[CH];
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int c = 0; c < NC; c += CH) {
-#pragma unroll
-    for (int k = 0; k < CH; k += 32) tmem_ld_x32(s_at + c + k, reinterpret_cast<uint32_t*>(sv) + k);
+  float sv[32];
+  auto load = [&](int c) {                                         // scores of columns c to c + 31 of the lane's share
+    tmem_ld_x32(s_at + c, reinterpret_cast<uint32_t*>(sv));
     tc_wait_ld();
     if (edge) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) if (!((see[(c + i) >> 5] >> (i & 31)) & 1)) sv[i] = -INFINITY;
+      for (int i = 0; i < 32; ++i) if (!((see[c >> 5] >> i) & 1)) sv[i] = -INFINITY;
     }
+  };
+  // 32 columns at a time, in loops: unrolled they are 5% to 20% slower, as the SM's instruction cache does not hold the kernel then.  (The scores are read twice: all 128
+  // do not fit the registers.)
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < NC; c += 32) {
+    load(c);
+    float mx[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < CH; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
+    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
+    top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
   }
-  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
   float alpha = 1.0f;
   const bool grow = top > m + kTau || (m == -INFINITY && top > -INFINITY);
   if (grow) { alpha = fast_exp2(m - top); m = top; }
   if (!first && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < DV / 32; ++c) {
       uint32_t o[32];
       tmem_ld_x32(s_t + 128 + c * 32, o);
@@ -196,20 +205,12 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
   const uint64_t ref2 = pair2(-ref, -ref);
   uint64_t rs2[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};
   float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int c = 0; c < NC; c += 32) {
+    if (NC > 32) load(c);
+    uint32_t pk[16];
 #pragma unroll
-  for (int c = 0; c < NC; c += CH) {
-    if constexpr (NC > CH) {                                       // (all 128 at once do not fit the registers: read again)
-#pragma unroll
-      for (int k = 0; k < CH; k += 32) tmem_ld_x32(s_at + c + k, reinterpret_cast<uint32_t*>(sv) + k);
-      tc_wait_ld();
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) if (!((see[(c + i) >> 5] >> (i & 31)) & 1)) sv[i] = -INFINITY;
-      }
-    }
-    uint32_t pk[CH / 2];
-#pragma unroll
-    for (int i = 0; i < CH / 2; ++i) {
+    for (int i = 0; i < 16; ++i) {
       // (in pairs where a thread has all 128 columns: 3% on wide trees; with folded rows it costs as much)
       float p0, p1;
       if constexpr (FOLD == 1) {
@@ -222,8 +223,7 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
       }
       pk[i] = pack_bf16x2(p0, p1);
     }
-    if constexpr (FOLD == 4) tmem_st_x16(s_t + fold * 16, pk);
-    else tmem_st_x32(s_t + (fold * NC + c) / 2, pk);
+    tmem_st_x16(s_t + (fold * NC + c) / 2, pk);
   }
   if constexpr (FOLD > 1) {                                        // the other copies' places
     uint32_t z[NC / 2];
@@ -244,11 +244,18 @@ __device__ __forceinline__ void softmax_step(uint32_t s_t, int fold, bool first,
 template <int DK, int DV, int FOLD>
 __global__ void __launch_bounds__(kTaThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {                                   // (the swizzled tiles need it; the compiler is asked for it)
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      report_status(a.status, ST_BAD_ARG, 850);
+      if (a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
   constexpr uint32_t kQ = 256 * DK, kSlot = 256 * (DK > DV ? DK : DV), kStage = 32768;
   uint8_t* sQ = smem;                                             // pair x [128 rows] (64-column halves of 128 B, swizzled)
-  uint8_t* s_stage = smem + a.pair * kQ;                          // FOLD > 1: [2 groups][32 columns][96 lanes of the copies]; else [2 groups][128 rows] of 128 B
+  uint8_t* s_stage = smem + a.pair * kQ;                          // [2 groups][128 lanes] of 128 B
   uint8_t* ring = smem + a.pair * kQ + kStage;
   const int slots = min(10, (int)((kTaTiles * 32768 - a.pair * kQ - kStage) / kSlot));
   uint64_t* bars = (uint64_t*)(smem + kTaTiles * 32768);
@@ -259,8 +266,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint32_t* tmem_slot = (uint32_t*)(bars + 36);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   int* s_odd = (int*)(tmem_slot + 2);                             // [16] places of the segment whose value rows are not finite, as bits: tree nodes; context from the window's begin on
-  float* s_x = (float*)(bars + 46);                               // [2][128]: what the groups tell each other about a row
-  TaSeg* s_seg = (TaSeg*)(s_x + 256);                           // [kTaSegs]; n_tiles = 0: no more
+  float* s_m = (float*)(bars + 46);                               // [2][128] maxima and sums of the groups' lanes
+  float* s_l = s_m + 256;
+  unsigned short* s_row = (unsigned short*)(s_l + 256);           // [128] row of a tile: node << 8 | head of the group
+  TaSeg* s_seg = (TaSeg*)(s_row + 128);                         // [kTaSegs]; n_tiles = 0: no more
+  static_assert(46 * 8 + 2048 + 256 + kTaSegs * sizeof(TaSeg) <= 3072, "shared memory");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -273,6 +283,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     fence_barrier_init();
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
   }
+  if (threadIdx.x < 128) s_row[threadIdx.x] = (unsigned short)((int)threadIdx.x / a.G << 8 | (int)threadIdx.x % a.G);
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
@@ -285,7 +296,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // ---------------------------------------------------------------- segments: this block's piece of the line, handed to the other warps
     const int per = (a.n_seqs + 31) / 32, i0 = min(a.n_seqs, lane * per), i1 = min(a.n_seqs, i0 + per);
     TaWalk walk;
-    walk.at = -1; walk.nth = 0;
+    walk.nth = 0;
     long long mine = 0;
 #pragma unroll 4
     for (int i = i0; i < i1; ++i) { TaSeq q; q.load(a, i); mine += q.cost(a); }
@@ -309,7 +320,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       walk.p.seq = __shfl_sync(0xffffffffu, seq, src);
       in_seq = __shfl_sync(0xffffffffu, in_seq, src);
       walk.q.load(a, walk.p.seq);
-      walk.at = walk.p.seq;
       const TaSeq& q = walk.q;
       const int head_cost = a.whole ? q.pairs : q.pairs * q.head + q.tiles * q.units;          // a KV head's; all of its pairs but the last cost the same
       const int kvh = in_seq / head_cost, in_head = in_seq - kvh * head_cost, pair_cost = a.whole ? 1 : q.head + a.pair * q.units;
@@ -324,7 +334,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         TaSeg s;
         const bool more = walk.next(a, s);
         if (!more) s.n_tiles = 0;
-        if (!mbar_wait(&g_empty[i], ((k / kTaSegs) & 1) ^ 1, abort_flag, a.status, 840, k)) break;
+        if (!ta_wait(&g_empty[i], ((k / kTaSegs) & 1) ^ 1, abort_flag, a.status, 840, k)) break;
         s_seg[i] = s;
         mbar_arrive(&g_full[i]);
         if (!more) break;
@@ -339,7 +349,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = true;
     for (int k = 0; ok; ++k) {
       const int i = k % kTaSegs;
-      ok = __all_sync(0xffffffffu, mbar_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 801, k));
+      ok = __all_sync(0xffffffffu, ta_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 801, k));
       if (!ok || s_seg[i].n_tiles == 0) break;
       const int lo = s_seg[i].lo, n = s_seg[i].n, kvh = s_seg[i].kvh, len = s_seg[i].q.len;
       const int* bt = a.block_table + (size_t)s_seg[i].seq * a.max_pages;
@@ -352,7 +362,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (j + 1 < n && lane < ppb) page = bt[min((lo + j + 1) * ppb + lane, last_page)];      // (pages behind the end: the last one again; nothing of them counts)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          ok = ok && mbar_wait(&t_empty[slot], ph ^ 1, abort_flag, a.status, 800, j);
+          ok = ok && ta_wait(&t_empty[slot], ph ^ 1, abort_flag, a.status, 800, j);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const int D = kv ? DV : DK;
@@ -373,11 +383,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       uint32_t ph = 0;
       for (int k = 0;; ++k) {
         const int i = k % kTaSegs;
-        if (!mbar_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 811, k) || s_seg[i].n_tiles == 0) break;
+        if (!ta_wait(&g_full[i], (k / kTaSegs) & 1, abort_flag, a.status, 811, k) || s_seg[i].n_tiles == 0) break;
         const int n = s_seg[i].n, n_tiles = s_seg[i].n_tiles, kvh = s_seg[i].kvh, begin = s_seg[i].q.begin + s_seg[i].tile * tpt;
         mbar_arrive(&g_empty[i]);
         if (n <= 0) continue;
-        if (!mbar_wait(q_empty, ph ^ 1, abort_flag, a.status, 810, k)) break;
+        if (!ta_wait(q_empty, ph ^ 1, abort_flag, a.status, 810, k)) break;
         mbar_expect_tx(q_full, (uint32_t)(2 * DK * G * tpt) * FOLD * n_tiles);
         for (int t = 0; t < n_tiles * FOLD; ++t) {
           uint8_t* dst = FOLD > 1 ? sQ + t * (128 / FOLD) * 128 : sQ + t * kQ;      // a copy of the rows, or the second tile
@@ -400,46 +410,43 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       bool ok = true;
       for (int k = 0; ok; ++k) {
         const int sg = k % kTaSegs;
-        if (!mbar_wait(&g_full[sg], (k / kTaSegs) & 1, abort_flag, a.status, 824, k) || s_seg[sg].n_tiles == 0) break;
+        if (!ta_wait(&g_full[sg], (k / kTaSegs) & 1, abort_flag, a.status, 824, k) || s_seg[sg].n_tiles == 0) break;
         const bool two = s_seg[sg].n_tiles == 2;
         const int n = s_seg[sg].n, steps = two ? 2 * n : n;
         mbar_arrive(&g_empty[sg]);
         if (n <= 0) continue;
-        if (!mbar_wait(q_full, q_ph, abort_flag, a.status, 820, k)) break;
+        if (!ta_wait(q_full, q_ph, abort_flag, a.status, 820, k)) break;
         q_ph ^= 1;
-        // step i: group i & 1; KV block i, or i / 2 where the groups share the blocks
-        auto issue_s = [&](int i) -> bool {
-          const int p = i & 1;
-          if (!mbar_wait(&t_full[k_slot], k_ph, abort_flag, a.status, 821, i)) return false;
-          tc_fence_after();
-          const uint64_t qd = make_sdesc_sw128(q_addr + (two && p ? kQ : 0)), kd = make_sdesc_sw128(r_addr + k_slot * kSlot);
+        // Step i: group i & 1; KV block i, or i / 2 where the groups share the blocks.  S runs two steps ahead: S of step i + 2 overwrites P of step i, which the pipe, running
+        // this thread's MMAs in order, has read by then; and its arrival tells that O holds all of the group's earlier products.
+        for (int j = 0; j < steps + 2 && ok; ++j) {
+          const int p = j & 1;
+          if (j >= 2) {
+            const int i = j - 2;
+            if (!ta_wait(&p_ready[p], (p_ph >> p) & 1, abort_flag, a.status, 822, i)) { ok = false; break; }
+            p_ph ^= 1u << p;
+            if (!ta_wait(&t_full[v_slot], v_ph, abort_flag, a.status, 823, i)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t vd = make_sdesc_sw128_mn(r_addr + v_slot * kSlot, 16384);
 #pragma unroll
-          for (int ks = 0; ks < DK / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-            mma_f16_ss(tmem_base + p * 256, sdesc_at(qd, off), sdesc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+            for (int ks = 0; ks < 8; ++ks)                                     // (the group's first block of the segment: O starts from zero)
+              mma_f16_ts(tmem_base + p * 256 + 128, tmem_base + p * 256 + ks * 8, sdesc_at(vd, ks * 2048), idesc_o, (i >= 2 || ks > 0) ? 1u : 0u);
+            if (!two || p) { tc_commit(&t_empty[v_slot]); step_on(v_slot, v_ph); }
+            if (j >= steps) tc_commit(&o_full[p]);                             // the group's last block
           }
-          tc_commit(&s_full[p]);
-          if (!two || p) { tc_commit(&t_empty[k_slot]); step_on(k_slot, k_ph); }
-          if (i == steps - 1) tc_commit(q_empty);
-          return true;
-        };
-        ok = issue_s(0);
-        if (ok && steps > 1) ok = issue_s(1);
-        for (int i = 0; i < steps && ok; ++i) {
-          const int p = i & 1;
-          if (!mbar_wait(&p_ready[p], (p_ph >> p) & 1, abort_flag, a.status, 822, i)) { ok = false; break; }
-          p_ph ^= 1u << p;
-          if (!mbar_wait(&t_full[v_slot], v_ph, abort_flag, a.status, 823, i)) { ok = false; break; }
-          tc_fence_after();
-          const uint64_t vd = make_sdesc_sw128_mn(r_addr + v_slot * kSlot, 16384);
+          if (j < steps) {
+            if (!ta_wait(&t_full[k_slot], k_ph, abort_flag, a.status, 821, j)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t qd = make_sdesc_sw128(q_addr + (two && p ? kQ : 0)), kd = make_sdesc_sw128(r_addr + k_slot * kSlot);
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)                                       // (the group's first block of the segment: O starts from zero)
-            mma_f16_ts(tmem_base + p * 256 + 128, tmem_base + p * 256 + ks * 8, sdesc_at(vd, ks * 2048), idesc_o, (i >= 2 || ks > 0) ? 1u : 0u);
-          if (!two || p) { tc_commit(&t_empty[v_slot]); step_on(v_slot, v_ph); }
-          if (i + 2 >= steps) tc_commit(&o_full[p]);                           // the group's last block
-          // The pipe runs this thread's MMAs in order: S of step i + 2 overwrites P of step i only after it has been read, and its arrival tells that O
-          // holds all of the group's earlier products.
-          if (i + 2 < steps) ok = issue_s(i + 2);
+            for (int ks = 0; ks < DK / 16; ++ks) {
+              const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
+              mma_f16_ss(tmem_base + p * 256, sdesc_at(qd, off), sdesc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+            }
+            tc_commit(&s_full[p]);
+            if (!two || p) { tc_commit(&t_empty[k_slot]); step_on(k_slot, k_ph); }
+            if (j == steps - 1) tc_commit(q_empty);
+          }
         }
       }
     }
@@ -449,10 +456,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int r = threadIdx.x & 127, fold = r / (128 / FOLD), rr = r % (128 / FOLD);      // lane; copy of the rows; row (fold is the same for a warp)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem_base + g * 256 + lane_off;
-    const int t_local = rr / G, h_local = rr - t_local * G;
+    const int t_local = s_row[rr] >> 8;
     uint32_t s_ph = 0, o_ph0 = 0, o_ph1 = 0;
     uint32_t t0 = 0;                                                           // ring tiles in front of the segment
-    bool ok = bar256_and(mbar_wait(&g_full[0], 0, abort_flag, a.status, 834, 0));
+    bool ok = bar256_and(ta_wait(&g_full[0], 0, abort_flag, a.status, 834, 0));
     for (int k = 0; ok && s_seg[k % kTaSegs].n_tiles > 0; ++k) {
       const TaSeg& s = s_seg[k % kTaSegs];
       const bool two = FOLD == 1 && s.n_tiles == 2;
@@ -479,7 +486,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (tail) see[c] = (see[c] | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
           }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b));        // (a warp leaves as one)
+        ok = __all_sync(0xffffffffu, ta_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b));        // (a warp leaves as one)
         if (!ok) break;
         s_ph ^= 1;
         if ((tail || kv0 < win1) && (!two || g == 0)) {
@@ -487,11 +494,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // finite is taken out, noted, and put back at the end for the rows that see it.  (Behind the wait for S, which tells that the products in front are done:
           // in front of it the place's tile before this one may still be on its way, and its barrier two phases from the one waited for.)
           const uint32_t t = t0 + 2 * b + 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b));
+          ok = __all_sync(0xffffffffu, ta_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b));
           if (ok && (kv0 + r >= min(ctx, len) || kv0 + r < win1)) {
             uint8_t* row = ring + (t % slots) * kSlot + r * 128;
             bool odd = false;
-#pragma unroll 2
+#pragma unroll 1
             for (int c = 0; c < DV / 8; ++c) {
               uint4* w = reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
               uint4 v = *w;
@@ -527,7 +534,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int own = two ? g : 0;
       const bool both = !two && n > 1;                                         // accumulator 1 holds something of this group's rows too
       float w0, w1 = 0.f, lse;                                                 // factors of the lane's accumulators
-      s_x[g * 128 + r] = m;
+      s_m[g * 128 + r] = m;
+      s_l[g * 128 + r] = l;
       ok = bar256_and(ok);                                                     // all 256 threads leave together
       if (!ok) break;
       if (two) {
@@ -536,16 +544,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       } else {
         float ms[2 * FOLD], top = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < 2 * FOLD; ++x) { ms[x] = s_x[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr]; top = fmaxf(top, ms[x]); }
-        bar256_and(true);
-        s_x[g * 128 + r] = l;
-        bar256_and(true);
+        for (int x = 0; x < 2 * FOLD; ++x) { ms[x] = s_m[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr]; top = fmaxf(top, ms[x]); }
         const float ref = top == -INFINITY ? 0.f : top;
         float sum = 0.f, e0 = 0.f, e1 = 0.f;
 #pragma unroll
         for (int x = 0; x < 2 * FOLD; ++x) {                                   // (2^-inf = 0)
-          const float e = exp2f(ms[x] - ref);
-          sum += e * s_x[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr];
+          const float e = fast_exp2(ms[x] - ref);
+          sum += e * s_l[(x / FOLD) * 128 + (x % FOLD) * (128 / FOLD) + rr];
           if (x == fold) e0 = e;
           if (x == FOLD + fold) e1 = e;
         }
@@ -558,53 +563,42 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 16; ++i) any_odd |= (uint32_t)s_odd[i];
       if (n > 0) {
-        ok = mbar_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, k);
-        if (both) ok = ok && mbar_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, k);
+        ok = ta_wait(&o_full[own], own ? o_ph1 : o_ph0, abort_flag, a.status, 832, k);
+        if (both) ok = ok && ta_wait(&o_full[1], o_ph1, abort_flag, a.status, 833, k);
         o_ph0 ^= 1;
         if (two || n > 1) o_ph1 ^= 1;
       }
       tc_fence_after();
-      const int head = s.kvh * G + h_local;
-      const long prow = ((long)s.slot * a.pair + (two ? g : 0)) * 128 + rr;    // of the parts
+      const long prow = ((long)s.slot * a.pair + (two ? g : 0)) * 128;         // of the parts: the tile's first
       const bool full = s.full;
+      const int first_node = (s.tile + own) * tpt, n_live = min(tpt, s.q.nodes - first_node);
+      const long row0 = full ? (long)(s.q.begin + first_node) * a.hq + s.kvh * G : prow;
       constexpr int kC = DV / 32;
       const int c0 = !two && g == 1 ? kC / 2 : 0, c1 = !two && g == 0 ? kC / 2 : kC;
-      if constexpr (FOLD == 1) {
-        if (!two) bar256_and(true);                                            // (the other group has read the sums)
-        reinterpret_cast<int*>(s_x)[g * 128 + r] = !live ? -1 : full ? tok * a.hq + head : (int)prow;         // where the row goes
-      }
+      uint8_t* st = s_stage + g * 16384;
+#pragma unroll 1
       for (int c = c0; c < c1; ++c) {
         float o[32];
         __syncwarp();
-        if (ok && n > 0 && warp_live) {
-          uint32_t o0[32], o1[32];
-          tmem_ld_x32(tmem_base + lane_off + own * 256 + 128 + c * 32, o0);
-          if (both) tmem_ld_x32(tmem_base + lane_off + 256 + 128 + c * 32, o1);
+        const bool any = ok && n > 0 && warp_live;
+        if (any) {
+          tmem_ld_x32(tmem_base + lane_off + own * 256 + 128 + c * 32, reinterpret_cast<uint32_t*>(o));
+          tc_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = any ? o[i] * w0 : 0.f;
+        if (any && both) {
+          uint32_t o1[32];
+          tmem_ld_x32(tmem_base + lane_off + 256 + 128 + c * 32, o1);
           tc_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = both ? fmaf(__uint_as_float(o0[i]), w0, __uint_as_float(o1[i]) * w1) : __uint_as_float(o0[i]) * w0;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(o1[i]), w1, o[i]);
         }
-        if constexpr (FOLD > 1) {                                              // the copies' shares go to the first one's threads
-          float* st = (float*)s_stage + g * 32 * 96 + (r - 128 / FOLD);
-          if (fold > 0) {
+        // Through shared memory, where the copies of a row are added up; eight lanes then store a row's 32 columns.
 #pragma unroll
-            for (int i = 0; i < 32; ++i) st[i * 96] = o[i];
-          }
-          bar_group(g);
-          if (fold == 0) {
-#pragma unroll
-            for (int f = 1; f < FOLD; ++f) {
-              const float* sf = (const float*)s_stage + g * 32 * 96 + (f - 1) * (128 / FOLD) + rr;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] += sf[i * 96];
-            }
-          }
-          bar_group(g);
-        }
+        for (int v = 0; v < 8; ++v) *reinterpret_cast<float4*>(st + r * 128 + ((v ^ (r & 7)) << 4)) = make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
         if (any_odd && ok && live && fold == 0) {
+#pragma unroll 1
           for (int x = 0; x < 512; ++x) {
             if (!((s_odd[x >> 5] >> (x & 31)) & 1)) continue;
             const int at = x < 256 ? ctx + x : win0 + x - 256;
@@ -612,71 +606,39 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
             if (slot < 0 || slot >= a.num_slots) continue;
             const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) { const float v = __bfloat162float(vr[i]); if (!(fabsf(v) < INFINITY)) o[i] += v; }
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i) {
+              const float v = __bfloat162float(vr[i]);
+              if (!(fabsf(v) < INFINITY)) *reinterpret_cast<float*>(st + r * 128 + (((i >> 2) ^ (r & 7)) << 4) + (i & 3) * 4) += v;
+            }
           }
         }
-        if constexpr (FOLD > 1) {                                              // few rows: a thread stores its own
-          if (ok && live && fold == 0) {
-            if (full) {
-              __nv_bfloat16* dst = a.out + ((size_t)tok * a.hq + head) * DV + c * 32;
-              uint32_t w[16];
+        bar_group(g);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
-              store32(dst, w);
-              store32(dst + 16, w + 8);
-            } else {
-              float* dst = a.part_o + prow * DV + c * 32;
+        for (int it = 0; it < 8 / FOLD; ++it) {
+          const int row = it * 16 + (r >> 3), th = s_row[row];
+          const uint8_t* from = st + row * 128 + (((r ^ row) & 7) << 4);
+          float4 x = *reinterpret_cast<const float4*>(from);
 #pragma unroll
-              for (int v = 0; v < 4; ++v) store32(dst + v * 8, reinterpret_cast<const uint32_t*>(o) + v * 8);
-            }
+          for (int f = 1; f < FOLD; ++f) {
+            const float4 y = *reinterpret_cast<const float4*>(from + f * (128 / FOLD) * 128);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
           }
-        } else {
-          // Through shared memory, so that eight lanes store 128 bytes of a row (a lane per row: 32 lines a store, 4000 to 8000 cycles a segment; so: 1300).
-          // 128 bytes per row and turn: 32 columns of a part, or 64 of the output in two turns.
-          uint8_t* mine = s_stage + g * 16384 + r * 128;
-          const int half = full ? (c - c0) & 1 : 0;
-          if (full) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              *reinterpret_cast<uint4*>(mine + (((half * 4 + v) ^ (r & 7)) << 4)) =
-                  make_uint4(pack_bf16x2(o[v * 8], o[v * 8 + 1]), pack_bf16x2(o[v * 8 + 2], o[v * 8 + 3]), pack_bf16x2(o[v * 8 + 4], o[v * 8 + 5]),
-                             pack_bf16x2(o[v * 8 + 6], o[v * 8 + 7]));
-          } else {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<float4*>(mine + ((v ^ (r & 7)) << 4)) = make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
-          }
-          const bool last = c == c1 - 1;
-          if (!full || half == 1 || last) {
-            const int chunk = r & 7, cols = full && half == 0 ? 4 : 8;         // (DV = 64 and one tile: 32 columns a group)
-            bar_group(g);
-            int to[8];
-            uint4 v[8];
-#pragma unroll
-            for (int it = 0; it < 8; ++it) {
-              const int row = it * 16 + (r >> 3);
-              to[it] = reinterpret_cast<const int*>(s_x)[g * 128 + row];
-              v[it] = *reinterpret_cast<const uint4*>(s_stage + g * 16384 + row * 128 + ((chunk ^ (row & 7)) << 4));
-            }
-            if (ok && chunk < cols) {
-              char* base = full ? (char*)(a.out + (c - half) * 32 + chunk * 8) : (char*)(a.part_o + c * 32 + chunk * 4);
-              const size_t pitch = full ? DV * 2 : DV * 4;
-#pragma unroll
-              for (int it = 0; it < 8; ++it) if (to[it] >= 0) *reinterpret_cast<uint4*>(base + to[it] * pitch) = v[it];
-            }
-            bar_group(g);
-          }
+          if (!ok || (th >> 8) >= n_live) continue;
+          const int col = c * 32 + (r & 7) * 4;
+          if (full) *reinterpret_cast<uint2*>(a.out + (row0 + (long)(th >> 8) * a.hq + (th & 255)) * DV + col) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+          else *reinterpret_cast<float4*>(a.part_o + (row0 + row) * DV + col) = x;
         }
+        bar_group(g);
       }
-      if (live && fold == 0 && !full && c0 == 0) a.part_lse[prow] = lse;
+      if (live && fold == 0 && !full && c0 == 0) a.part_lse[prow + rr] = lse;
       if (any_odd) {
         bar256_and(true);
         if (threadIdx.x < 16) s_odd[threadIdx.x] = 0;
       }
       tc_fence_before();
-      ok = ok && mbar_wait(&g_full[(k + 1) % kTaSegs], ((k + 1) / kTaSegs) & 1, abort_flag, a.status, 834, k + 1);
-      ok = bar256_and(ok);                                                     // both accumulators, s_x and the segment are free again
+      ok = ok && ta_wait(&g_full[(k + 1) % kTaSegs], ((k + 1) / kTaSegs) & 1, abort_flag, a.status, 834, k + 1);
+      ok = bar256_and(ok);                                                     // both accumulators, s_m, s_l and the segment are free again
       if (threadIdx.x == 0) mbar_arrive(&g_empty[k % kTaSegs]);
     }
   }

@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import math
 from array import array
-from itertools import repeat
 from operator import attrgetter
 from typing import NamedTuple, Optional, Sequence
 
@@ -19,7 +18,7 @@ from .. import _native
 from .paging import MAX_NODES, check_int32
 
 _TILE, _PAGES = (64, 128), (8, 16, 32, 64, 128)
-_nbytes = attrgetter("nbytes")
+_nbytes, _shape = attrgetter("nbytes"), attrgetter("shape")
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor,
@@ -64,8 +63,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         out = torch.empty(t, hq, dv, dtype=dtype, device=dev)
     elif out.shape != (t, hq, dv) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out: a contiguous tensor [{t}, {hq}, {dv}] of the queries' type is needed")
-    elif out.data_ptr() % 32:
-        raise ValueError("out: a 32-byte boundary is needed")
+    elif out.data_ptr() % 16:
+        raise ValueError("out: a 16-byte boundary is needed")
     if dev.type != "cuda":
         return tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size, mask, window, positions, out)
     if t == 0 or b == 0:
@@ -146,9 +145,10 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"trees of 1 to {MAX_NODES} nodes, not {max_nodes}")
     # (two caches a layer: by maps over the list, a loop of Python steps took 45 us of 56)
-    slots = caches[0].size(0) if len(caches) else 0
+    shapes = set(map(_shape, caches))
+    slots = next((s[0] for s in shapes if s), 0)
     on = dev.index if dev.type == "cuda" else -1
-    if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or set(map(torch.Tensor.size, caches, repeat(0))) - {slots}:
+    if not all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.get_device, caches)) - {on} or any(not s or s[0] != slots for s in shapes):
         raise ValueError("contiguous caches of equal numbers of slots beside the tokens are needed")
     if dev.type != "cuda":
         spans = sorted((c.data_ptr(), c.nbytes) for c in caches if c.nbytes)
@@ -157,7 +157,9 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
         return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)
     with _native.on_device(dev):
         count, nxt, new, path = torch.empty(b * (3 + max_nodes), dtype=torch.int32, device=dev).split((b, b, b, b * max_nodes))
-        ptrs, sizes = array("Q", map(torch.Tensor.data_ptr, caches)), array("q", map(_nbytes, caches))
+        ptrs = array("Q", map(torch.Tensor.data_ptr, caches))
+        alike = len(shapes) == 1 and len(set(map(torch.Tensor.element_size, caches))) == 1
+        sizes = array("q", (caches[0].nbytes,)) * len(ptrs) if alike else array("q", map(_nbytes, caches))
         rc = _native.entry("gb_tree_commit", "ppilppppppiiiiippppp")(
             ptrs.buffer_info()[0], sizes.buffer_info()[0], len(ptrs), slots, tokens.data_ptr(), parents.data_ptr(), sampled.data_ptr(), cu_q.data_ptr(),
             kv_len.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, b, t, max_nodes, count.data_ptr(), path.data_ptr(), nxt.data_ptr(),

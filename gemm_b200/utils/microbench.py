@@ -26,6 +26,8 @@ Cases
                convolution and rotation, norms of Q and K, capped scores and sinks (plain attention), the stream's norms and sums
   zedirax      the kernels of Zedirax at the sizes of ``zedirax-30b-a3b`` beside the like kernels of the other models: minGRU (HGRN2), logarithmic distance
                bias (a table of biases, plain attention), the average over earlier layers (the stream's norms and sums), GELU epilogues
+  tree         a verification step with trees of drafts in its parts, 64 sequences x 2048 cached tokens, trees of 8 and of 64 nodes: the tables, the attention of the
+               nodes (and the causal kernel on as many tokens in chains), a draw per node with per-row parameters, acceptance and cache move over 48 layers
   spec_verify  whole-model step over 1, 2, 3 and 5 positions per sequence (speculative verification against plain decode);
                builds the full Qwen3-30B-A3B shape, not part of ``all``
 
@@ -770,10 +772,49 @@ def case_zedirax(args):
             del we
 
 
+def case_tree(args):
+    """The parts of a verification step with trees of drafts, and beside them the causal kernel and the sampler on as many tokens."""
+    from ..ops import paging, sampling, tree
+    hq, hkv, d, page, vocab, layers = args.hq, args.hkv, 128, args.page, 151936, 48
+    b, ctx = args.batch if args.batch > 0 else 64, args.ctx if args.ctx >= 0 else 2048
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")       # noqa: E731
+    for nodes in (8, 64):
+        per = (ctx + nodes + page - 1) // page
+        slots, t = b * per * page, b * nodes
+        lens, ctxs, ptr, ids = i32([nodes] * b), i32([ctx] * b), i32([i * per for i in range(b + 1)]), i32(list(range(b * per)))
+        parents = i32([-1] + [(i - 1) // 2 for i in range(1, nodes)]).repeat(b)
+        tables = lambda: paging.batch_tables(lens, ctxs, ptr, ids, page, t, per, parents, nodes)       # noqa: E731,B023
+        kw = dict(batch=b, nodes=nodes, ctx=ctx, hq=hq, hkv=hkv, page=page)
+        _run(f"tree_tables_{b}x{nodes}", tables, 0.0, 4.0 * (b * (3 + 2 * per) + t * 3) + 8 * t, args, **kw)
+        tab = tables()
+        q = (torch.randn(t, hq, d, device="cuda") * ew.softmax_scale_log2(d)).bfloat16()
+        k, v = (torch.randn(slots, hkv, d, device="cuda").bfloat16() for _ in range(2))
+        hbm = b * (ctx + nodes) * hkv * d * 4 + t * hq * d * 4
+        flops = 4.0 * t * hq * (ctx + nodes / 2) * d
+        _run(f"tree_attention_{b}x{nodes}", lambda: tree.tree_attention(q, k, v, tab.cu_q, tab.kv_len, tab.block_table, page, tab.mask, nodes), flops, hbm, args, **kw)   # noqa: B023
+        work = att.build_work([nodes] * b, hq, hkv, 1).to("cuda")
+        _run(f"causal_attention_{b}x{nodes}", lambda: att.attention(q, k, v, tab.cu_q, tab.kv_len, tab.block_table, page, work, causal=True), flops, hbm, args, **kw)     # noqa: B023
+        del k, v
+        logits = torch.randn(min(t, 1024), vocab, device="cuda") * 2.5
+        rows = logits.shape[0]
+        u, temp = torch.rand(rows, device="cuda"), torch.rand(rows, device="cuda") + 0.5
+        for name, top_k, top_p in (("top_k", 50, 0.95), ("top_p", 0, 0.95), ("all", 0, 1.0)):
+            _run(f"draw_{name}_{rows}x{vocab}", lambda: sampling.draw(logits, u, temp, top_k, top_p), 0.0, logits.numel() * 4, args)    # noqa: B023
+        _run(f"sampler_{rows}x{vocab}", lambda: sampling.sample(logits, 0.8, 50, 0.95, seed=1, step=3), 0.0, logits.numel() * 4, args)  # noqa: B023
+        del logits
+        caches = [torch.empty(slots, hkv, d, dtype=torch.bfloat16, device="cuda") for _ in range(2 * layers)]
+        tokens = i32([i % 7 for i in range(t)])
+        drawn = tokens.roll(-2)                                             # node 2 i + 2 is accepted behind node i here and there
+        n_moved = int((tree.tree_commit([], tokens, parents, drawn, tab.cu_q, tab.kv_len, tab.block_table, page, nodes).count - 1).sum())
+        _run(f"tree_commit_{b}x{nodes}", lambda: tree.tree_commit(caches, tokens, parents, drawn, tab.cu_q, tab.kv_len, tab.block_table, page, nodes), 0.0,   # noqa: B023
+             4.0 * n_moved * layers * hkv * d * 2, args, moved=n_moved, **kw)
+        del caches
+
+
 MODEL_CASES = {"spec_verify": case_spec_verify}      # build the whole benchmark model: not part of --case all
 CASES = {"gemm": case_gemm, "moe_decode": case_moe_decode, "moe_prefill": case_moe_prefill, "attn_decode": case_attn_decode,
          "attn_prefill": case_attn_prefill, "lm_head": case_lm_head, "quant": case_quant, "small": case_small, "layered": case_layered,
-         "famepel": case_famepel, "fidolix": case_fidolix, "zedirax": case_zedirax}
+         "famepel": case_famepel, "fidolix": case_fidolix, "zedirax": case_zedirax, "tree": case_tree}
 
 
 def main(argv=None):
