@@ -23,12 +23,17 @@ namespace gb {
 
 constexpr int kTaThreads = 384;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads; 11: segments
 constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, one in which rows are joined and put in order, the rest is the ring
+// Items of as many blocks or fewer are not cut (no parts to write and join).  64 sequences of 8 nodes on 500 places each: 24 us, cut 29; on 10 to 500: 24.4, cut 26.4; on 10 to
+// 1000 (8 blocks): 35.4, cut 33.6.  With a window most items have the same length: windows of 1000 in 10 blocks, 29 us, cut 34, if the items go round the SMs.
+constexpr int kTaWhole = 4, kTaWholeWindow = 12;
 constexpr int kTaSegs = 4;          // segments handed out ahead
 constexpr int kTaSmem = kTaTiles * 32768 + 3072;      // (all there is)
 
 struct TreeAttnArgs {
   const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
   int n_seqs, max_pages, page_size, words, window, hq, hkv, total_tokens;
+  int max_nodes;
+  int cap;                           // places that a row of the block table has room for
   int G, tpt;                        // query heads per KV head; nodes per tile
   int pair;                          // tiles per item: 1 or 2
   int fold;                          // copies of the rows in a tile: 1, 2 or 4 (pair = 1, and at most 128 / fold rows in any sequence)
@@ -48,10 +53,11 @@ struct TaSeq {
   __device__ __forceinline__ void load(const TreeAttnArgs& a, int s) {
     const int tpt = a.tpt;
     begin = min(max(a.cu_q[s], 0), a.total_tokens);
-    nodes = max(min(a.cu_q[s + 1], a.total_tokens) - begin, 0);
+    const int all = max(min(a.cu_q[s + 1], a.total_tokens) - begin, 0);
+    nodes = min(all, a.max_nodes);                     // (the bounds on the line and the workspace go by max_nodes)
     const int kv = a.kv_len[s];
-    len = max(0, (int)min((long long)kv, (long long)a.max_pages * a.page_size));
-    ctx = max(0, kv - nodes);
+    len = max(0, min(kv, a.cap));
+    ctx = max(0, kv - all);
     first = a.window > 0 ? max(0, ctx - a.window + 1) / 128 : 0;
     blocks = max(0, (len + 127) / 128 - first);
     units = a.whole ? 1 : max(1, blocks);
@@ -61,13 +67,15 @@ struct TaSeq {
     head = a.whole ? 0 : a.head;
   }
   // The line that is cut: an item takes `head` (its start and its end, in blocks of one tile) and, per block, one for each of its tiles.
-  __device__ __forceinline__ long long cost(const TreeAttnArgs& a) const { return a.whole ? items : (long long)a.hkv * (pairs * head + (long long)tiles * units); }
+  __device__ __forceinline__ int cost(const TreeAttnArgs& a) const { return a.whole ? items : a.hkv * (pairs * head + tiles * units); }
 };
 
-// The pieces: [c * total / active, (c + 1) * total / active) of the line.
+// The line is cut into `active` pieces that differ by one at most.  (The whole line is shorter than 2^31: the host sees to that.  64-bit divisions would cost more than all else here.)
 struct TaPiece {
-  long long total, pos, left;
-  int active, seq, item, off;             // off: place in the item
+  int total, active, each, more;          // each: length of a piece; the first `more` are longer by one
+  int pos, left, seq, item, off;          // off: place in the item
+  __device__ __forceinline__ int begin(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int piece_of(int at) const { return at < more * (each + 1) ? at / (each + 1) : more + (at - more * (each + 1)) / each; }
 };
 
 // The part of an item that a block works on.
@@ -80,14 +88,6 @@ struct TaSeg {
   int parts;                              // the item begins here and is cut: into so many parts
 };
 
-// Begin of piece c, and the piece that holds a place.  (64-bit division takes some hundred instructions: where 32 bits do, they are used.)
-__device__ __forceinline__ long long ta_begin(int c, long long total, int active) {
-  return total < (1 << 22) ? (long long)((unsigned)c * (unsigned)total / (unsigned)active) : c * total / active;             // (c <= 148)
-}
-__device__ __forceinline__ int ta_piece_of(long long at, long long total, int active) {
-  return total < (1 << 22) ? (int)(((unsigned)(at + 1) * (unsigned)active - 1) / (unsigned)total) : (int)(((at + 1) * active - 1) / total);
-}
-
 struct TaWalk {
   TaPiece p;
   TaSeq q;
@@ -96,11 +96,11 @@ struct TaWalk {
     while (p.left > 0) {
       const int kvh = p.item / q.pairs, tile = (p.item - kvh * q.pairs) * a.pair, n_tiles = min(a.pair, q.tiles - tile), w = a.whole ? 1 : n_tiles;
       const int cost = q.head + w * q.units;
-      const int take = (int)min((long long)(cost - p.off), p.left);
+      const int take = min(cost - p.off, p.left);
       // block b belongs to the piece that holds place head + b * w of the item
       auto block_at = [&](int o) { return o <= q.head ? 0 : (o - q.head + w - 1) >> (w - 1); };
       const int b0 = block_at(p.off), b1 = block_at(p.off + take);
-      const long long pos = p.pos - p.off;                         // the item's
+      const int pos = p.pos - p.off;                               // the item's
       s.q = q; s.seq = p.seq; s.item = p.item; s.kvh = kvh; s.tile = tile; s.n_tiles = n_tiles;
       p.left -= take; p.pos += take; p.off += take;
       if (p.off == cost) {
@@ -116,8 +116,8 @@ struct TaWalk {
       s.slot = 2 * (int)blockIdx.x + (nth++ == 0 ? 0 : 1);
       s.parts = 0;
       if (!s.full && b0 == 0) {
-        const long long last = pos + s.q.head + (long long)(s.q.units - 1) * w;      // the place of the item's last block; the piece that holds it is the last one that begins there or before
-        s.parts = ta_piece_of(last, p.total, p.active) - (int)blockIdx.x + 1;
+        const int last = pos + s.q.head + (s.q.units - 1) * w;     // the place of the item's last block; the piece that holds it is the last one that begins there or before
+        s.parts = p.piece_of(last) - (int)blockIdx.x + 1;
       }
       return true;
     }
@@ -297,35 +297,37 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int per = (a.n_seqs + 31) / 32, i0 = min(a.n_seqs, lane * per), i1 = min(a.n_seqs, i0 + per);
     TaWalk walk;
     walk.nth = 0;
-    long long mine = 0;
-#pragma unroll 4
+    int mine = 0;
+#pragma unroll 2
     for (int i = i0; i < i1; ++i) { TaSeq q; q.load(a, i); mine += q.cost(a); }
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
-    const long long total = __shfl_sync(0xffffffffu, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += x; }
+    TaPiece& p = walk.p;
+    p.total = __shfl_sync(0xffffffffu, incl, 31);
     // at least two blocks a piece: a part costs more to write and join than a block to work on (and every piece inside an item must get a block of it)
-    const int active = (int)min((long long)gridDim.x, a.whole ? total : max(total / (2 * a.pair), min(total, 1ll)));
-    walk.p.total = total; walk.p.active = active; walk.p.left = 0;
-    if ((int)blockIdx.x < active) {
-      const long long lo = ta_begin(blockIdx.x, total, active), excl = incl - mine;
-      int seq = 0, in_seq = 0;
-      const bool here = excl <= lo && lo < incl;
-      if (here) {
-        long long at = excl;
-        for (seq = i0;; ++seq) { walk.q.load(a, seq); const long long c = walk.q.cost(a); if (lo < at + c) break; at += c; }
-        in_seq = (int)(lo - at);
+    p.active = min((int)gridDim.x, a.whole ? p.total : max(p.total / (2 * a.pair), min(p.total, 1)));
+    p.left = 0;
+    if ((int)blockIdx.x < p.active) {
+      p.each = p.total / p.active; p.more = p.total - p.each * p.active;
+      const int lo = p.begin(blockIdx.x);
+      // the lane whose sequences hold the place, then the sequence
+      const int src = __ffs(__ballot_sync(0xffffffffu, incl > lo)) - 1;
+      int at = __shfl_sync(0xffffffffu, incl - mine, src);
+      p.seq = min(a.n_seqs, src * per);
+      while (true) {
+        walk.q.load(a, p.seq);
+        const int c = walk.q.cost(a);
+        if (lo < at + c) break;
+        at += c; ++p.seq;
       }
-      const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-      walk.p.seq = __shfl_sync(0xffffffffu, seq, src);
-      in_seq = __shfl_sync(0xffffffffu, in_seq, src);
-      walk.q.load(a, walk.p.seq);
+      const int in_seq = lo - at;
       const TaSeq& q = walk.q;
       const int head_cost = a.whole ? q.pairs : q.pairs * q.head + q.tiles * q.units;          // a KV head's; all of its pairs but the last cost the same
       const int kvh = in_seq / head_cost, in_head = in_seq - kvh * head_cost, pair_cost = a.whole ? 1 : q.head + a.pair * q.units;
       const int pair = min(in_head / pair_cost, q.pairs - 1);
-      walk.p.item = kvh * q.pairs + pair; walk.p.off = in_head - pair * pair_cost;
-      walk.p.pos = lo; walk.p.left = ta_begin(blockIdx.x + 1, total, active) - lo;
+      p.item = kvh * q.pairs + pair; p.off = in_head - pair * pair_cost;
+      p.pos = lo; p.left = p.begin(blockIdx.x + 1) - lo;
     }
     if (lane == 0) {
       if (a.part_of != nullptr) a.part_of[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -490,33 +492,38 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!ok) break;
         s_ph ^= 1;
         if ((tail || kv0 < win1) && (!two || g == 0)) {
-          // Values of places that some row does not see must be finite: a weight of 0 times them is added.  Thread r looks at place r of the block; what is not
+          // Values of places that some row does not see must be finite: a weight of 0 times them is added.  What is not
           // finite is taken out, noted, and put back at the end for the rows that see it.  (Behind the wait for S, which tells that the products in front are done:
           // in front of it the place's tile before this one may still be on its way, and its barrier two phases from the one waited for.)
           const uint32_t t = t0 + 2 * b + 1;
           ok = __all_sync(0xffffffffu, ta_wait(&t_full[t % slots], (t / slots) & 1, abort_flag, a.status, 830, b));
-          if (ok && (kv0 + r >= min(ctx, len) || kv0 + r < win1)) {
-            uint8_t* row = ring + (t % slots) * kSlot + r * 128;
-            bool odd = false;
+          // eight threads a row, 16 rows a turn
+          constexpr int kTurns = DV / 64;
 #pragma unroll 1
-            for (int c = 0; c < DV / 8; ++c) {
-              uint4* w = reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
-              uint4 v = *w;
+          for (int row = r >> 3; ok && row < 128; row += 16) {
+            const int at = kv0 + row;
+            if (!(at >= min(ctx, len) || at < win1)) continue;
+            const uint32_t in = at < len ? 0xffffffffu : 0u;
+            uint8_t* w = ring + (t % slots) * kSlot + row * 128 + (((r ^ row) & 7) << 4);
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < kTurns; ++c) {
+              uint4 v = *reinterpret_cast<uint4*>(w + c * 16384);
               uint32_t* x = reinterpret_cast<uint32_t*>(&v);
               bool put = false;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                uint32_t keep = kv0 + r < len ? 0xffffffffu : 0u;
+                uint32_t keep = in;
                 if ((x[e] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
                 if ((x[e] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
                 put |= keep != 0xffffffffu;
                 x[e] &= keep;
               }
-              if (put) *w = v;
+              if (put) *reinterpret_cast<uint4*>(w + c * 16384) = v;
               odd |= put;
             }
-            const int x = kv0 + r >= ctx ? kv0 + r - ctx : kv0 + r - win0 + 256;         // (the window's begin is cut by fewer places than there are nodes)
-            if (odd && kv0 + r < len && x >= (kv0 + r >= ctx ? 0 : 256) && x < (kv0 + r >= ctx ? 256 : 512)) atomicOr(&s_odd[x >> 5], 1 << (x & 31));
+            const int x = at >= ctx ? at - ctx : at - win0 + 256;              // (the window's begin is cut by fewer places than there are nodes)
+            if (odd && at < len && x >= (at >= ctx ? 0 : 256) && x < (at >= ctx ? 256 : 512)) atomicOr(&s_odd[x >> 5], 1 << (x & 31));
           }
           fence_proxy_async_smem();
         }
@@ -744,22 +751,25 @@ using namespace gb;
 
 // Blocks of the launch, how the rows lie in a tile, and whether the items stay whole: bounds by what the host knows (at most max_pages pages and max_nodes nodes a
 // sequence).
-static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int* pair, int* fold, int* whole) {
+static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int window, int* pair, int* fold, int* whole) {      // 0: too much work for 32-bit places
   const int G = hq / hkv;
   const long rows = (long)max_nodes * G;
   *fold = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
   const int tpt = 128 / *fold / G, tiles = (max_nodes + tpt - 1) / tpt;
   *pair = tiles > 1 ? 2 : 1;
-  const long blocks = std::max(1l, ((long)max_pages * page_size + 127) / 128), items = (long)n_seqs * hkv * ((tiles + *pair - 1) / *pair);
-  *whole = blocks <= 2;
+  long blocks = std::max(1l, ((long)max_pages * page_size + 127) / 128);
+  if (window > 0) blocks = std::min(blocks, ((long)window + max_nodes + 126) / 128 + 1);
+  const long items = (long)n_seqs * hkv * ((tiles + *pair - 1) / *pair);
+  *whole = blocks <= kTaWhole || (window > 0 && blocks <= kTaWholeWindow && 2 * items > sm_count());
+  if (items * *pair * (blocks + 8) > 1l << 30) return 0;
   return (int)std::max(1l, std::min((long)sm_count(), *whole ? items : (items * blocks + 1) / 2));
 }
 
-// Floats of the workspace that gb_tree_attn wants.
-GB_API int gb_tree_attn_workspace(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int dv) {
+// Floats of the workspace that gb_tree_attn wants; 0: not for gb_tree_attn.
+GB_API int gb_tree_attn_workspace(int n_seqs, int max_pages, int page_size, int max_nodes, int hq, int hkv, int dv, int window) {
   int pair, fold, whole;
-  const long grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &pair, &fold, &whole);
-  return whole ? 4 : (int)((grid + 1) / 2 * 8 + 2 * grid * pair * 128 * (dv + 1));          // (at most 148 * 2 * 2 * 128 rows)
+  const long grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, window, &pair, &fold, &whole);
+  return grid == 0 ? 0 : whole ? 4 : (int)((grid + 1) / 2 * 8 + 2 * grid * pair * 128 * (dv + 1));          // (at most 148 * 2 * 2 * 128 rows)
 }
 
 GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const void* v_cache, void* out, float* workspace, const int* cu_q, const int* kv_len,
@@ -773,11 +783,13 @@ GB_API int gb_tree_attn(const void* q, long q_ts, const void* k_cache, const voi
   if (window > 0 && positions == nullptr) return fail("tree_attn: a window needs the nodes' positions%s");
   TreeAttnArgs a;
   memset(&a, 0, sizeof(a));
-  const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, &a.pair, &a.fold, &a.whole);
+  const int grid = tree_attn_grid(n_seqs, max_pages, page_size, max_nodes, hq, hkv, window, &a.pair, &a.fold, &a.whole);
+  if (grid == 0) return fail("tree_attn: too much work for one call%s");
   a.cu_q = cu_q; a.kv_len = kv_len; a.block_table = block_table; a.mask = (const unsigned long long*)mask; a.positions = positions; a.n_seqs = n_seqs;
   a.max_pages = max_pages; a.page_size = page_size; a.words = words; a.window = window; a.hq = hq; a.hkv = hkv; a.total_tokens = tokens;
   a.head = a.pair == 2 ? 6 : 2;
   a.G = hq / hkv; a.tpt = 128 / a.fold / a.G;
+  a.max_nodes = max_nodes; a.cap = (int)std::min((long)max_pages * page_size, 0x7fffffffl);
   a.num_slots = num_slots; a.out = (__nv_bfloat16*)out; a.v_cache = (const __nv_bfloat16*)v_cache; a.status = (KernelStatus*)status;
   if (!a.whole) {
     a.part_of = (int4*)workspace;

@@ -76,8 +76,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     pos = positions.data_ptr() if positions is not None else None
     with _native.on_device(dev):
         # the tcgen05 kernel's forms: its tiles hold 64 or 128 columns, 128 rows and whole pages, and TMA wants 16-byte boundaries
+        n = 0
         if dtype is torch.bfloat16 and dk in _TILE and dv in _TILE and page_size in _PAGES and hq // hkv <= 128 and not (q_ts & 7 or (qp | kp | vp) & 15):
-            n = _native.entry("gb_tree_attn_workspace", "iiiiiii")(b, cols, page_size, max_nodes, hq, hkv, dv)
+            n = _native.entry("gb_tree_attn_workspace", "iiiiiiii")(b, cols, page_size, max_nodes, hq, hkv, dv, window)
+        if n > 0:
             work = torch.empty(n, dtype=torch.float32, device=dev)
             rc = _native.entry("gb_tree_attn", "plpppppppiipipiliiiiiiipp")(
                 qp, q_ts, kp, vp, out.data_ptr(), work.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), cols, page_size, mask.data_ptr(), words, pos,
