@@ -381,7 +381,8 @@ draw_kernel(const DrawArgs a) {
       unsigned long long w = q < found ? weight(value_of(e.x)) : 0ull;
       if (half == 0) pair[q] = make_uint4(e.x, e.y, (unsigned)w, (unsigned)(w >> 32));
       __syncthreads();
-      const int j0 = half ? (found + 1) / 2 : 0, j1 = half ? found : (found + 1) / 2;
+      // (warps without a candidate sit the loops out)
+      const int j0 = half ? (found + 1) / 2 : 0, j1 = (q & ~31) >= found ? j0 : half ? found : (found + 1) / 2;
       int place = 0;
       unsigned long long front = 0;
 #pragma unroll 4
