@@ -5,6 +5,8 @@
 // the one drawn at x, as long as there is one.  Accepted node number j goes from place ctx + path[j] to ctx + j.  Since path[j] >= j and the path ascends,
 // a thread that moves one column of a row in path order has read every row before it overwrites it: no staging.
 //
+// 64 trees of 64 nodes, 36 layers, 8 KV heads of 128: 63 MB move in 11.7 us, 5.4 TB/s; 4 trees, 28 layers: 3.3 us, the launch.
+//
 // One launch for all layers: a block handles one sequence and some of the caches, and makes the (short) walk for itself in one warp: a ballot per step, tokens
 // and parents in registers.  Blocks of the first column of the grid also write the results.
 #include "sm100.cuh"

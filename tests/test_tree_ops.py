@@ -243,6 +243,18 @@ def test_attention_kernel_f32(nodes, ctx, hq, hkv, dk, dv, page, window):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nodes,ctx,hq,hkv,dk,dv,page,window", [
+    ([7, 2], [100, 3], 6, 2, 320, 300, 16, 0), ([5, 0, 9, 1, 2, 1, 1], [70, 3, 0, 500, 31, 32, 33], 9, 3, 40, 256, 8, 0), ([1] * 40, list(range(40)), 3, 3, 256, 80, 12, 9),
+    ([256, 3], [10, 700], 5, 1, 16, 24, 32, 300)])
+def test_attention_kernel_other_heads(nodes, ctx, hq, hkv, dk, dv, page, window, dtype):
+    """Tiles of rows that span sequences and tokens, heads wider than a tile's, pages of any size."""
+    s = attention_inputs(nodes, ctx, hq, hkv, dk, dv, page, dtype, seed=dk)
+    s["window"] = window
+    close(tree.tree_attention(**on_gpu(s)), s)
+
+
+@gpu
 @pytest.mark.parametrize("hq,hkv,n,d", [(4, 2, 3, 128), (16, 2, 70, 128), (8, 8, 12, 64), (2, 1, 5, 96)])
 def test_attention_kernel_masked_places(hq, hkv, n, d):
     """Arbitrary masks, empty rows among them; keys and values that are not finite at nodes that some rows do not see; the lowest value of the type."""
