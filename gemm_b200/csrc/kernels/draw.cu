@@ -30,14 +30,14 @@
 
 namespace gb {
 
-constexpr int kDrThreads = 512, kDrWarps = 16;
-constexpr int kDrBins = 512;               // steps of 1/16 below the maximum; the last one takes all that lies further down
 constexpr int kDrList = 256;               // candidates a warp lists
 constexpr int kDrCand = 2048;              // candidates of a row in the first block
 constexpr int kDrPairs = 256;              // candidates that are compared with one another
-constexpr int kDrGroups = 4096;            // groups of logits whose maxima prune a row
-constexpr int kDrPrune = 1000;             // k' at most: a quarter of the groups, so that few logits beyond the k'-th lie above the bound
+constexpr int kDrPrune = 1000;             // k' at most: a half of the groups or less, so that few logits beyond the k'-th lie above the bound
 constexpr int kDrMass = 44;                // fraction bits of a weight
+// Rows of as many logits or fewer take half the threads, if there are more of them than fill the GPU: 30000 f32 rows of 1000 602 us, with 512 threads 914; 12000 bf16 rows of
+// 2500 527 and 479; 8000 f32 rows of 4000 323 and 324.
+constexpr int kDrShort = 2048;
 constexpr size_t kDrSmem = 202000;         // bytes of logits that a block holds at most
 
 struct DrawArgs {
@@ -51,7 +51,11 @@ struct DrawArgs {
   KernelStatus* status;
 };
 
+// Blocks have 512 threads, or 256 where rows are many and short.  As many steps of 1/16 below the maximum make the histogram (the last one takes all that lies further
+// down), and eight times as many groups of logits have their maxima taken.
+template <int kDrThreads>
 struct alignas(16) DrawShared {
+  static constexpr int kDrWarps = kDrThreads / 32, kDrBins = kDrThreads, kDrGroups = 8 * kDrThreads;
   unsigned count[2][kDrBins];              // histogram, by step parity
   unsigned lo[2][kDrBins], hi[2][kDrBins]; // its masses in two words
   double table[32];
@@ -140,8 +144,9 @@ __device__ __forceinline__ unsigned long long dr_weight(double d, double scale, 
   return (unsigned long long)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;    // 2^52: rounded to a whole number
 }
 
-// Exclusive position of `target` in the running sum of the 512 threads' values: the thread with before < target <= before + v stores itself.
-__device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long target, DrawShared& s) {
+// Exclusive position of `target` in the running sum of the threads' values: the thread with before < target <= before + v stores itself.
+template <typename S>
+__device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long target, S& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned long long incl = v;
 #pragma unroll
@@ -149,7 +154,7 @@ __device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long
   if (lane == 31) s.scan[warp] = incl;
   if (threadIdx.x == 0) { s.found_at = -1; s.found_before = 0; }
   __syncthreads();
-  unsigned long long front = lane < warp ? s.scan[lane] : 0ull;    // (16 warps: the lanes fetch, and add up)
+  unsigned long long front = lane < warp ? s.scan[lane] : 0ull;    // (16 warps at most: the lanes fetch, and add up)
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) front += __shfl_xor_sync(0xffffffffu, front, o);
   incl += __shfl_sync(0xffffffffu, front, 0);
@@ -157,11 +162,13 @@ __device__ __forceinline__ void dr_find(unsigned long long v, unsigned long long
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDrThreads, 2)
+template <typename T, int kDrThreads>
+__global__ void __launch_bounds__(kDrThreads, 1024 / kDrThreads)
 draw_kernel(const DrawArgs a) {
+  constexpr int kDrWarps = kDrThreads / 32, kDrBins = kDrThreads, kDrGroups = 8 * kDrThreads, kDrBits = kDrThreads == 512 ? 9 : 8;
+  static_assert(1 << kDrBits == kDrThreads, "a digit of the searches for each thread");
   extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ DrawShared s;
+  __shared__ DrawShared<kDrThreads> s;
   using Key = DrawKey<T>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = a.ctas;
@@ -216,7 +223,7 @@ draw_kernel(const DrawArgs a) {
   };
 
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in kDrGroups / (512 C) pieces.  (fmaxf passes over NaN.)
+  // ---- maximum, and the maxima of the groups: a thread's share of the block's logits in 8 / C pieces.  (fmaxf passes over NaN.)
   const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.f, few_groups = has_k && top_k <= kDrThreads / 8;      // eight groups for each logit that top-k keeps
   float mx = -INFINITY, low = INFINITY;
   {
@@ -253,7 +260,7 @@ draw_kernel(const DrawArgs a) {
       if (rank == 0) s.group[at] = v;
       else dr_put32(&s.group[at], 0, __float_as_uint(v));
     };
-    if (few_groups) {                                              // 512 in all: a thread's maxima in one, and those of C threads
+    if (few_groups) {                                              // one for each thread of a block in all: a thread's maxima in one, and those of C threads
 #pragma unroll
       for (int p = 1; p < kPieces; ++p) if (p < pieces) gm[0] = fmaxf(gm[0], gm[p]);
       for (int o = 1; o < C; o <<= 1) gm[0] = fmaxf(gm[0], __shfl_xor_sync(0xffffffffu, gm[0], o));
@@ -369,7 +376,7 @@ draw_kernel(const DrawArgs a) {
     __syncthreads();
     v = s.scan[lane & (kDrWarps - 1)];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = kDrWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
     return v;
   };
@@ -381,13 +388,14 @@ draw_kernel(const DrawArgs a) {
     if (found <= kDrPairs) {
       // Few: every candidate against every other one.  Its rank, the mass in front of it, and the kept mass at lower ids are plain sums.
       uint4* pair = reinterpret_cast<uint4*>(&s.lo[0][0]);         // key, id, mass (8 KB: lo and hi lie one behind the other)
+      constexpr int kHalves = kDrThreads / kDrPairs;               // two threads to a candidate, or one
       const int q = tid & (kDrPairs - 1), half = tid / kDrPairs;
       const uint2 e = q < found ? cand_at(q) : make_uint2(0u, 0u);
       unsigned long long w = q < found ? weight(value_of(e.x)) : 0ull;
       if (half == 0) pair[q] = make_uint4(e.x, e.y, (unsigned)w, (unsigned)(w >> 32));
       __syncthreads();
       // (warps without a candidate sit the loops out)
-      const int j0 = half ? (found + 1) / 2 : 0, j1 = (q & ~31) >= found ? j0 : half ? found : (found + 1) / 2;
+      const int j0 = half ? (found + 1) / 2 : 0, j1 = (q & ~31) >= found ? j0 : half || kHalves == 1 ? found : (found + 1) / 2;
       int place = 0;
       unsigned long long front = 0;
 #pragma unroll 4
@@ -399,9 +407,11 @@ draw_kernel(const DrawArgs a) {
       }
       unsigned long long* other = reinterpret_cast<unsigned long long*>(&s.count[0][0]);      // [kDrPairs], then the places
       int* other_place = (int*)(other + kDrPairs);
-      if (half) { other[q] = front; other_place[q] = place; }
-      __syncthreads();
-      if (!half) { front += other[q]; place += other_place[q]; }
+      if (kHalves > 1) {
+        if (half) { other[q] = front; other_place[q] = place; }
+        __syncthreads();
+        if (!half) { front += other[q]; place += other_place[q]; }
+      }
       bool keep = !half && q < found && (!cut_k || place < top_k);
       if (has_p) {
         const unsigned long long goal = target != 0 ? target : top_p_target(sum(keep ? w : 0ull));
@@ -418,10 +428,12 @@ draw_kernel(const DrawArgs a) {
         const uint4 o = pair[j];
         below += o.y < e.y ? (unsigned long long)o.w << 32 | o.z : 0ull;
       }
-      if (half) other[q] = below;
-      __syncthreads();
+      if (kHalves > 1) {
+        if (half) other[q] = below;
+        __syncthreads();
+      }
       if (!half && w != 0) {
-        below += other[q];
+        if (kHalves > 1) below += other[q];
         if (below <= r && r < below + w) {
           a.out[row] = (int)e.y;
           if (a.logprob != nullptr) a.logprob[row] = logprob_of(value_of(e.x), all);
@@ -453,7 +465,7 @@ draw_kernel(const DrawArgs a) {
       unsigned prefix = 0;
       before = 0;
       for (int bits = 32 - __clz(range); bits > 0;) {
-        const int shift = max(0, bits - 9);
+        const int shift = max(0, bits - kDrBits);
         s.count[0][tid] = 0;
         if (mass) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
         __syncthreads();
@@ -462,7 +474,7 @@ draw_kernel(const DrawArgs a) {
           const unsigned long long v = val(k);
           const unsigned off = min(of(k) - base, range);
           if (v == 0 || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
-          const int d = (off >> shift) & 511;
+          const int d = (off >> shift) & (kDrThreads - 1);
           if (!mass) atomicAdd(&s.count[0][d], 1u);
           else {
             const unsigned l = (unsigned)v, old = atomicAdd(&s.lo[0][d], l);
@@ -471,11 +483,11 @@ draw_kernel(const DrawArgs a) {
           }
         }
         __syncthreads();
-        const int d = up ? tid : 511 - tid;
+        const int d = up ? tid : kDrThreads - 1 - tid;
         const unsigned long long v = mass ? ((unsigned long long)s.hi[0][d] << 32) + s.lo[0][d] : s.count[0][d];
         dr_find(v, goal - before, s);
         const int hit = s.found_at < 0 ? 0 : s.found_at;
-        prefix = prefix << (bits - shift) | (unsigned)(up ? hit : 511 - hit);
+        prefix = prefix << (bits - shift) | (unsigned)(up ? hit : kDrThreads - 1 - hit);
         before += s.found_before;
         bits = shift;
         __syncthreads();
@@ -790,7 +802,7 @@ draw_kernel(const DrawArgs a) {
           const unsigned first = by_id ? 0u : least, range = by_id ? (unsigned)a.vocab - 1 : most - least;
           unsigned prefix = 0;
           for (int bits = 32 - __clz(range); bits > 0;) {
-            const int shift = max(0, bits - 9);
+            const int shift = max(0, bits - kDrBits);
             __syncthreads();
             s.lo[1][tid] = 0; s.hi[1][tid] = 0;
             __syncthreads();
@@ -798,16 +810,16 @@ draw_kernel(const DrawArgs a) {
             for (int k = 0; k < kOwn; ++k) {
               const unsigned off = min((by_id ? id[k] : key[k]) - first, range);
               if (w[k] == 0 || (by_id && key[k] != found[0]) || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
-              const int d = (off >> shift) & 511;
+              const int d = (off >> shift) & (kDrThreads - 1);
               const unsigned l = (unsigned)w[k], old = atomicAdd(&s.lo[1][d], l);
               const unsigned h = (unsigned)(w[k] >> 32) + (old + l < old ? 1u : 0u);
               if (h != 0) atomicAdd(&s.hi[1][d], h);
             }
             __syncthreads();
-            const int d = by_id ? tid : 511 - tid;
+            const int d = by_id ? tid : kDrThreads - 1 - tid;
             dr_find(((unsigned long long)s.hi[1][d] << 32) + s.lo[1][d], goal, s);
             const int hit = s.found_at < 0 ? 0 : s.found_at;
-            prefix = prefix << (bits - shift) | (unsigned)(by_id ? hit : 511 - hit);
+            prefix = prefix << (bits - shift) | (unsigned)(by_id ? hit : kDrThreads - 1 - hit);
             goal -= s.found_before;
             bits = shift;
           }
@@ -1093,7 +1105,7 @@ draw_kernel(const DrawArgs a) {
   dr_cluster_sync();                                               // nobody leaves while another one reads its shared memory
 }
 
-template <typename T>
+template <typename T, int kDrThreads>
 static int draw_launch(DrawArgs a, cudaStream_t stream) {
   // Blocks per row: as few as hold it with two blocks to an SM (the steps of a cluster cost every block of it: 1500 bf16 rows of 32003 in one block each 219 us, in eight 257, at the
   // time of the choice); few rows take as many as there is room for.
@@ -1107,12 +1119,17 @@ static int draw_launch(DrawArgs a, cudaStream_t stream) {
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
   if (dev > 63 || !attr[dev]) {
-    GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDrSmem));
+    GB_CUDA_OK(cudaFuncSetAttribute(draw_kernel<T, kDrThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDrSmem));
     if (dev < 64) attr[dev] = true;
   }
-  launch_k_cluster(draw_kernel<T>, (unsigned)(a.rows * c), kDrThreads, smem, stream, (unsigned)c, a);
+  launch_k_cluster(draw_kernel<T, kDrThreads>, (unsigned)(a.rows * c), kDrThreads, smem, stream, (unsigned)c, a);
   GB_CUDA_OK(cudaGetLastError());
   return 0;
+}
+
+template <typename T>
+static int draw_for(const DrawArgs& a, cudaStream_t stream) {
+  return a.vocab <= kDrShort && a.rows > 2 * sm_count() ? draw_launch<T, 256>(a, stream) : draw_launch<T, 512>(a, stream);
 }
 
 }  // namespace gb
@@ -1130,5 +1147,5 @@ GB_API int gb_draw(const void* logits, long ld, int dtype, int rows, int vocab, 
   a.logits = logits; a.ld = ld; a.rows = rows; a.vocab = vocab; a.u = u; a.temperature = temperature; a.temperature_all = temperature_all;
   a.top_k = top_k; a.top_k_all = top_k_all; a.top_p = top_p; a.top_p_all = top_p_all; a.min_p = min_p; a.min_p_all = min_p_all; a.out = out;
   a.logprob = logprob; a.status = (KernelStatus*)status;
-  return dtype == 0 ? draw_launch<float>(a, stream) : draw_launch<__nv_bfloat16>(a, stream);
+  return dtype == 0 ? draw_for<float>(a, stream) : draw_for<__nv_bfloat16>(a, stream);
 }

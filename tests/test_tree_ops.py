@@ -522,6 +522,17 @@ def test_draw_kernel(kind, v, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 37, 1009, 2048])
+@pytest.mark.parametrize("kind", KINDS)
+def test_draw_kernel_many_short_rows(kind, v, dtype):
+    s = draw_rows(700, v, dtype, v, kind)
+    got = sampling.draw(**on_gpu(s), want_logprob=True)
+    _native.assert_status_ok()
+    same_draws(got, s)
+
+
+@gpu
 def test_draw_kernel_borders_and_strides():
     """Numbers of 0 and 1 and beyond; rows that begin at odd places; one row; no rows; the largest vocabulary."""
     s = draw_rows(50, 5001, torch.bfloat16, 9, "normal")
