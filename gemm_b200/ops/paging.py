@@ -57,19 +57,17 @@ def batch_tables(q_lens: torch.Tensor, ctx_lens: torch.Tensor, page_ptr: torch.T
         return batch_tables_ref(q_lens, ctx_lens, page_ptr, pages, page_size, total_tokens, max_pages, parents, max_nodes)
     with _native.on_device(dev):
         # one buffer for all that is int32, every table on a 16-byte boundary
-        x1 = (b + 4) & -4
-        x2, rows = x1 + ((b + 3) & -4), (total_tokens + 3) & -4
-        x3, x4 = x2 + rows, x2 + 2 * rows
-        buf = torch.empty(x4 + b * max_pages, dtype=torch.int32, device=dev)
-        cu, kv, pos, slots, table = (buf.as_strided(size, step, at) for size, step, at in (((b + 1,), (1,), 0), ((b,), (1,), x1), ((total_tokens,), (1,), x2),
-                                                                                           ((total_tokens,), (1,), x3), ((b, max_pages), (max_pages, 1), x4)))
-        mask = torch.empty(total_tokens, words, dtype=torch.int64, device=dev) if words else None
+        gap, rows = -total_tokens & 3, b * max_pages
+        x1, x2 = -(b + 1) & 3, -b & 3
+        cu, _, kv, _, pos, _, slots, _, table = q_lens.new_empty(2 * (b + total_tokens + gap) + 1 + x1 + x2 + rows).split_with_sizes(
+            (b + 1, x1, b, x2, total_tokens, gap, total_tokens, gap, rows))
+        mask = q_lens.new_empty(total_tokens, words, dtype=torch.int64) if words else None
         rc = _native.entry("gb_batch_tables", "ppppiiiiipippppppp")(
             q_lens.data_ptr(), ctx_lens.data_ptr(), page_ptr.data_ptr(), pages.data_ptr(), pages.numel(), b, page_size, total_tokens, max_pages,
             parents.data_ptr() if words else None, max_nodes, cu.data_ptr(), kv.data_ptr(), pos.data_ptr(), slots.data_ptr(), table.data_ptr(),
             mask.data_ptr() if words else None, _native.stream())
         _native.check(rc, "gb_batch_tables")
-    return BatchTables(cu, kv, pos, slots, table, mask)
+    return BatchTables(cu, kv, pos, slots, table.view(b, max_pages), mask)
 
 
 def batch_tables_ref(q_lens, ctx_lens, page_ptr, pages, page_size, total_tokens, max_pages, parents=None, max_nodes=0) -> BatchTables:

@@ -131,8 +131,8 @@ def draw(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=Non
         return (token, logprob) if want_logprob else token
     (t, t0), (k, k0), (p, p0), (m, m0) = given
     with _native.on_device(dev):
-        out = torch.empty(b, dtype=torch.int32, device=dev)
-        logprob = torch.empty(b, dtype=torch.float32, device=dev) if want_logprob else None
+        out = uniform.new_empty(b, dtype=torch.int32)
+        logprob = uniform.new_empty(b) if want_logprob else None
         ptr = lambda x: x.data_ptr() if x is not None else None                # noqa: E731
         rc = _native.entry("gb_draw", "pliiipp" + "fpipfpf" + "pppp")(
             logits.data_ptr(), logits.stride(0) if b > 1 else v, 0 if logits.dtype is torch.float32 else 1, b, v, uniform.data_ptr(), ptr(t), t0, ptr(k), k0, ptr(p),

@@ -60,7 +60,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         if positions.numel() != t:
             raise ValueError("positions: one for each node")
     if out is None:
-        out = torch.empty(t, hq, dv, dtype=dtype, device=dev)
+        out = q.new_empty(t, hq, dv)
     elif out.shape != (t, hq, dv) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out: a contiguous tensor [{t}, {hq}, {dv}] of the queries' type is needed")
     elif out.data_ptr() % 16:
@@ -80,7 +80,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         if dtype is torch.bfloat16 and dk in _TILE and dv in _TILE and page_size in _PAGES and hq // hkv <= 128 and not (q_ts & 7 or (qp | kp | vp) & 15):
             n = _native.entry("gb_tree_attn_workspace", "iiiiiiii")(b, cols, page_size, max_nodes, hq, hkv, dv, window)
         if n > 0:
-            work = torch.empty(n, dtype=torch.float32, device=dev)
+            work = q.new_empty(n, dtype=torch.float32)
             rc = _native.entry("gb_tree_attn", "plpppppppiipipiliiiiiiipp")(
                 qp, q_ts, kp, vp, out.data_ptr(), work.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), cols, page_size, mask.data_ptr(), words, pos,
                 b, slots, t, max_nodes, hq, hkv, dk, dv, window, _native.status_ptr(), _native.stream())
@@ -158,7 +158,7 @@ def tree_commit(caches: Sequence[torch.Tensor], tokens: torch.Tensor, parents: t
             raise ValueError("tree_commit: caches that overlap")
         return tree_commit_ref(caches, tokens, parents, sampled, cu_q, kv_len, block_table, page_size, max_nodes)
     with _native.on_device(dev):
-        count, nxt, new, path = torch.empty(b * (3 + max_nodes), dtype=torch.int32, device=dev).split((b, b, b, b * max_nodes))
+        count, nxt, new, path = kv_len.new_empty(b * (3 + max_nodes)).split_with_sizes((b, b, b, b * max_nodes))
         ptrs = array("Q", map(torch.Tensor.data_ptr, caches))
         alike = len(shapes) == 1 and len(set(map(torch.Tensor.element_size, caches))) == 1
         sizes = array("q", (caches[0].nbytes,)) * len(ptrs) if alike else array("q", map(_nbytes, caches))
