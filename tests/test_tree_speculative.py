@@ -210,3 +210,37 @@ def test_engine_min_p_on_gpu():
     a = Engine(w, 2, 64, page_size=16).generate(prompts, sp, use_graph=True)
     b = Engine(w, 2, 64, page_size=16).generate(prompts, sp, use_graph=False)
     assert a == b and len(set(a[0])) > 3
+
+
+def windowed(drafter, device):
+    cfg = dataclasses.replace(get_config("tiny-dense"), sliding_window=10)
+    w = synthetic_weights(cfg, "bf16", device="cpu", seed=3)
+    kv = KvCache.allocate(cfg, 96, 16, device)
+    return cfg, w, SpeculativeDecoder(Transformer(w if device == "cpu" else w.to(device), kv), kv, 16, 96, drafter)
+
+
+def test_trees_with_a_sliding_window():
+    """Branches of several depths, each with a window of its own."""
+    torch.manual_seed(2)
+    cfg, _, plain = windowed(None, "cpu")
+    prompts = [torch.randint(0, cfg.vocab, (n,)).tolist() for n in (5, 33)]
+    ref = plain.generate(prompts, 16)
+    assert ref != decoder("tiny-dense", None)[1].generate(prompts, 16)
+    dec = windowed(KnowingTrees([p + o for p, o in zip(prompts, ref)], gamma=6), "cpu")[2]
+    assert dec.generate(prompts, 16) == ref and dec.stats.tokens_per_step > 8
+
+
+@gpu
+def test_trees_with_a_sliding_window_on_gpu():
+    torch.manual_seed(2)
+    cfg, w, plain = windowed(None, "cuda")
+    prompts = [torch.randint(0, cfg.vocab, (n,)).tolist() for n in (5, 33)]
+    dec = windowed(KnowingTrees([p + o for p, o in zip(prompts, plain.generate(prompts, 16))], gamma=6), "cuda")[2]
+    out = dec.generate(prompts, 16)
+    _native.assert_status_ok()
+    for p, o in zip(prompts, out):
+        logits = reference.reference_logits(w, torch.tensor(list(p) + list(o))[:-1]).float()
+        for j, tok in enumerate(o):
+            row = logits[len(p) - 1 + j]
+            assert row[tok] >= row.max() - 0.3 * row.std()
+    assert dec.stats.tokens_per_step > 2.0
