@@ -765,87 +765,87 @@ draw_kernel(const DrawArgs a) {
         for (int c = 0; c < C; ++c) settled &= s.cand_n[c] <= cap;
       }
       if (settled) {
-      const int own = s.cand_own;
-      // Many above the cut: the first block finds the cut in its step, every block then knows its kept mass, and the block in which the draw falls goes through
-      // its logits once more.
-      if (rank == 0) {
-        constexpr int kOwn = kDrCand / kDrThreads;
-        unsigned key[kOwn], id[kOwn], least = 0xffffffffu, most = 0;
-        unsigned long long w[kOwn];
+        const int own = s.cand_own;
+        // Many above the cut: the first block finds the cut in its step, every block then knows its kept mass, and the block in which the draw falls goes through
+        // its logits once more.
+        if (rank == 0) {
+          constexpr int kOwn = kDrCand / kDrThreads;
+          unsigned key[kOwn], id[kOwn], least = 0xffffffffu, most = 0;
+          unsigned long long w[kOwn];
 #pragma unroll
-        for (int k = 0; k < kOwn; ++k) {
-          const int q = k * kDrThreads + tid;                      // of the list: place q - c cap of block c
-          const bool in = (q & (cap - 1)) < s.cand_n[q / cap];
-          const uint2 e = in ? s.cand[q] : make_uint2(0u, 0u);
-          key[k] = e.x; id[k] = e.y;
-          w[k] = in ? weight(value_of(e.x)) : 0ull;
-          if (in) { least = min(least, e.x); most = max(most, e.x); }
-        }
-        least = __reduce_min_sync(0xffffffffu, least);
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (tid == 0) { s.first_max = -1; s.tau = 0; }
-        __syncthreads();
-        if (lane == 0) { atomicMin((unsigned*)&s.first_max, least); atomicMax(&s.tau, most); }
-        __syncthreads();
-        least = (unsigned)s.first_max; most = s.tau;
-        // the key at which the mass reaches the target, and, of equal keys, the id
-        unsigned found[2] = {0, 0};
-        unsigned long long goal = target - before;
-#pragma unroll
-        for (int by_id = 0; by_id < 2; ++by_id) {
-          if (by_id) {
-            unsigned long long same = 0;
-#pragma unroll
-            for (int k = 0; k < kOwn; ++k) same += key[k] == found[0];
-            if (sum(same) == 1) { found[1] = 0xffffffffu; break; }
+          for (int k = 0; k < kOwn; ++k) {
+            const int q = k * kDrThreads + tid;                      // of the list: place q - c cap of block c
+            const bool in = (q & (cap - 1)) < s.cand_n[q / cap];
+            const uint2 e = in ? s.cand[q] : make_uint2(0u, 0u);
+            key[k] = e.x; id[k] = e.y;
+            w[k] = in ? weight(value_of(e.x)) : 0ull;
+            if (in) { least = min(least, e.x); most = max(most, e.x); }
           }
-          const unsigned first = by_id ? 0u : least, range = by_id ? (unsigned)a.vocab - 1 : most - least;
-          unsigned prefix = 0;
-          for (int bits = 32 - __clz(range); bits > 0;) {
-            const int shift = max(0, bits - kDrBits);
-            __syncthreads();
-            s.lo[1][tid] = 0; s.hi[1][tid] = 0;
-            __syncthreads();
+          least = __reduce_min_sync(0xffffffffu, least);
+          most = __reduce_max_sync(0xffffffffu, most);
+          if (tid == 0) { s.first_max = -1; s.tau = 0; }
+          __syncthreads();
+          if (lane == 0) { atomicMin((unsigned*)&s.first_max, least); atomicMax(&s.tau, most); }
+          __syncthreads();
+          least = (unsigned)s.first_max; most = s.tau;
+          // the key at which the mass reaches the target, and, of equal keys, the id
+          unsigned found[2] = {0, 0};
+          unsigned long long goal = target - before;
 #pragma unroll
-            for (int k = 0; k < kOwn; ++k) {
-              const unsigned off = min((by_id ? id[k] : key[k]) - first, range);
-              if (w[k] == 0 || (by_id && key[k] != found[0]) || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
-              const int d = (off >> shift) & (kDrThreads - 1);
-              const unsigned l = (unsigned)w[k], old = atomicAdd(&s.lo[1][d], l);
-              const unsigned h = (unsigned)(w[k] >> 32) + (old + l < old ? 1u : 0u);
-              if (h != 0) atomicAdd(&s.hi[1][d], h);
+          for (int by_id = 0; by_id < 2; ++by_id) {
+            if (by_id) {
+              unsigned long long same = 0;
+#pragma unroll
+              for (int k = 0; k < kOwn; ++k) same += key[k] == found[0];
+              if (sum(same) == 1) { found[1] = 0xffffffffu; break; }
             }
-            __syncthreads();
-            const int d = by_id ? tid : kDrThreads - 1 - tid;
-            dr_find(((unsigned long long)s.hi[1][d] << 32) + s.lo[1][d], goal, s);
-            const int hit = s.found_at < 0 ? 0 : s.found_at;
-            prefix = prefix << (bits - shift) | (unsigned)(by_id ? hit : kDrThreads - 1 - hit);
-            goal -= s.found_before;
-            bits = shift;
+            const unsigned first = by_id ? 0u : least, range = by_id ? (unsigned)a.vocab - 1 : most - least;
+            unsigned prefix = 0;
+            for (int bits = 32 - __clz(range); bits > 0;) {
+              const int shift = max(0, bits - kDrBits);
+              __syncthreads();
+              s.lo[1][tid] = 0; s.hi[1][tid] = 0;
+              __syncthreads();
+#pragma unroll
+              for (int k = 0; k < kOwn; ++k) {
+                const unsigned off = min((by_id ? id[k] : key[k]) - first, range);
+                if (w[k] == 0 || (by_id && key[k] != found[0]) || (bits >= 32 ? 0u : off >> bits) != prefix) continue;
+                const int d = (off >> shift) & (kDrThreads - 1);
+                const unsigned l = (unsigned)w[k], old = atomicAdd(&s.lo[1][d], l);
+                const unsigned h = (unsigned)(w[k] >> 32) + (old + l < old ? 1u : 0u);
+                if (h != 0) atomicAdd(&s.hi[1][d], h);
+              }
+              __syncthreads();
+              const int d = by_id ? tid : kDrThreads - 1 - tid;
+              dr_find(((unsigned long long)s.hi[1][d] << 32) + s.lo[1][d], goal, s);
+              const int hit = s.found_at < 0 ? 0 : s.found_at;
+              prefix = prefix << (bits - shift) | (unsigned)(by_id ? hit : kDrThreads - 1 - hit);
+              goal -= s.found_before;
+              bits = shift;
+            }
+            found[by_id] = first + prefix;
           }
-          found[by_id] = first + prefix;
+          __syncthreads();
+          if (tid < C) { dr_put32(&s.tau, tid, found[0]); dr_put32(&s.last, tid, found[1]); }
         }
-        __syncthreads();
-        if (tid < C) { dr_put32(&s.tau, tid, found[0]); dr_put32(&s.last, tid, found[1]); }
-      }
-      dr_cluster_sync();
-      const unsigned tau = s.tau, last = s.last;
-      const float tau_x = value_of(tau);
-      auto keeps = [&](float v, unsigned id) -> bool { return (v > tau_x) | ((v == tau_x) & (id <= last)); };
-      unsigned long long mine = tid < cut ? ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid] : 0ull;
-      for (int q = tid; q < own; q += kDrThreads) {
-        const uint2 e = s.cand[q];
-        if (keeps(value_of(e.x), e.y)) mine += weight(value_of(e.x));
-      }
-      mine = sum(mine);
-      if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
-      dr_cluster_sync();
-      unsigned long long all = 0, front = 0;
-      for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
-      const unsigned long long r = spot_of(all);
-      if (r < front || r >= front + mine) return;
-      locate(weigh(keeps), front, r, all, keeps);
-      return;
+        dr_cluster_sync();
+        const unsigned tau = s.tau, last = s.last;
+        const float tau_x = value_of(tau);
+        auto keeps = [&](float v, unsigned id) -> bool { return (v > tau_x) | ((v == tau_x) & (id <= last)); };
+        unsigned long long mine = tid < cut ? ((unsigned long long)s.hi[0][tid] << 32) + s.lo[0][tid] : 0ull;
+        for (int q = tid; q < own; q += kDrThreads) {
+          const uint2 e = s.cand[q];
+          if (keeps(value_of(e.x), e.y)) mine += weight(value_of(e.x));
+        }
+        mine = sum(mine);
+        if (tid < C) dr_put64(&s.block_mass[rank], tid, mine);
+        dr_cluster_sync();
+        unsigned long long all = 0, front = 0;
+        for (int c = 0; c < C; ++c) { if (c < rank) front += s.block_mass[c]; all += s.block_mass[c]; }
+        const unsigned long long r = spot_of(all);
+        if (r < front || r >= front + mine) return;
+        locate(weigh(keeps), front, r, all, keeps);
+        return;
       }
     }
   }

@@ -32,7 +32,8 @@ constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two 
 // 1000 (8 blocks): 35.4, cut 33.6.  With a window most items have the same length: windows of 1000 in 10 blocks, 29 us, cut 34, if the items go round the SMs.
 constexpr int kTaWhole = 4, kTaWholeWindow = 12;
 constexpr int kTaSegs = 4;          // segments handed out ahead
-constexpr int kTaSmem = kTaTiles * 32768 + 3072;      // (all there is)
+constexpr int kTaSide = 3 * 1024;   // bytes beside the tiles
+constexpr int kTaSmem = kTaTiles * 32768 + kTaSide;      // (all there is)
 
 struct TreeAttnArgs {
   const int* cu_q; const int* kv_len; const int* block_table; const unsigned long long* mask; const int* positions;
@@ -275,7 +276,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   float* s_l = s_m + 256;
   unsigned short* s_row = (unsigned short*)(s_l + 256);           // [128] row of a tile: node << 8 | head of the group
   TaSeg* s_seg = (TaSeg*)(s_row + 128);                         // [kTaSegs]; n_tiles = 0: no more
-  static_assert(46 * 8 + 2048 + 256 + kTaSegs * sizeof(TaSeg) <= 3072, "shared memory");
+  static_assert(46 * 8 + 2048 + 256 + kTaSegs * sizeof(TaSeg) <= kTaSide, "shared memory");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
