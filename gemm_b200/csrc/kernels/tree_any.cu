@@ -1,8 +1,8 @@
 // Attention of drafted tree nodes over a paged KV cache, for any head sizes and element types: the path of f32 caches and of head sizes the tcgen05 kernel
 // (tree_attn.cu) is not built for.
 //
-// Node i of a sequence with context ctx and n nodes (cached at places ctx .. ctx + n - 1) sees the places j < ctx (with a window: position - j < window, where
-// the node's position is ctx + its depth) and the nodes whose bit is set in its mask.  o = sum_j 2^(q . k_j - m) v_j / sum_j 2^(q . k_j - m); nothing seen: 0.
+// Node i of a sequence with context ctx and n nodes (cached at places ctx .. ctx + n - 1) sees the places j < ctx and the nodes whose bit is set in its mask; with a
+// window, those less than it in front of the node's position (ctx + its depth; a place of the context has its number for position).  o = sum_j 2^(q . k_j - m) v_j / sum_j 2^(q . k_j - m); nothing seen: 0.
 // Q arrives multiplied by scale * log2(e); scores, weights and sums are f32.  A key that is not seen takes no part, whatever its rows hold.
 //
 // Heads of up to 256 columns: a block has 16 rows of a KV head ((node, head) pairs, in the order of the tokens), four to a warp, and goes over the keys 32 at a time, K and V through
@@ -28,6 +28,9 @@ __device__ __forceinline__ float ldt(const __nv_bfloat16* p) { return __bfloat16
 __device__ __forceinline__ void stt(float* p, float v) { *p = v; }
 __device__ __forceinline__ void stt(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 
+// Whether a node lies in a window that begins at position `from` (nodes have positions from ctx on).
+__device__ __forceinline__ bool tree_near(const TreeAnyArgs& a, int token, int ctx, int from) { return from <= ctx || (token < a.tokens && a.positions[token] >= from); }
+
 template <typename T>
 __global__ void __launch_bounds__(128)
 tree_any_kernel(const TreeAnyArgs a) {
@@ -49,7 +52,7 @@ tree_any_kernel(const TreeAnyArgs a) {
   float* q = s_q + warp * a.dk;
   for (int c = lane; c < a.dk; c += 32) q[c] = ldt((const T*)a.q + (size_t)t * a.q_ts + (size_t)h * a.dk + c);
   __syncwarp();
-  const int first = a.window > 0 ? min(ctx, max(0, a.positions[t] - a.window + 1)) : 0;
+  const int from = a.window > 0 ? max(0, a.positions[t] - a.window + 1) : 0, first = min(ctx, from);      // from: the first position in the window
   const int* bt = a.block_table + (size_t)seq * a.max_pages;
   float m = -INFINITY, l = 0.f, acc[NV];
 #pragma unroll
@@ -59,7 +62,7 @@ tree_any_kernel(const TreeAnyArgs a) {
     bool live = j < len;
     if (live && j >= ctx) {
       const int x = j - ctx;
-      live = x < a.words * 64 && ((a.mask[(size_t)t * a.words + (x >> 6)] >> (x & 63)) & 1);
+      live = x < a.words * 64 && ((a.mask[(size_t)t * a.words + (x >> 6)] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, from);
     }
     long slot = 0;
     float sc = -INFINITY;
@@ -123,13 +126,13 @@ tree_tile_kernel(const TreeAnyArgs a) {
     const int t0 = (int)(at / G);
     int lo = 0, hi = a.n_seqs;
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.cu_q[mid] <= t0) lo = mid; else hi = mid; }
-    const int seq = lo, n_nodes = a.cu_q[seq + 1] - a.cu_q[seq];
+    const int seq = lo, begin = a.cu_q[seq], n_nodes = a.cu_q[seq + 1] - begin;
     const long to = min(r1, (long)max(a.cu_q[seq + 1], t0 + 1) * G);
     const int len = min(a.kv_len[seq], (int)min((long)a.max_pages * a.page_size, 0x7fffffffl)), ctx = max(0, a.kv_len[seq] - n_nodes);
     const int* bt = a.block_table + (size_t)seq * a.max_pages;
     if (threadIdx.x < kTyRows) {
       const long r = r0 + threadIdx.x;
-      s_lo[threadIdx.x] = a.window > 0 && r >= at && r < to ? min(ctx, max(0, a.positions[r / G] - a.window + 1)) : a.window > 0 ? ctx : 0;
+      s_lo[threadIdx.x] = a.window > 0 && r >= at && r < to ? max(0, a.positions[r / G] - a.window + 1) : a.window > 0 ? ctx : 0;
     }
     __syncthreads();
     int first = ctx;
@@ -182,10 +185,11 @@ tree_tile_kernel(const TreeAnyArgs a) {
       float p[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        bool live = mine[k] && j < len && j >= from[k];
-        if (live && j >= ctx) {
+        bool live = mine[k] && j < len;
+        if (live && j < ctx) live = j >= from[k];
+        else if (live) {
           const int x = j - ctx;
-          live = x < a.words * 64 && ((mask[k][x >> 6] >> (x & 63)) & 1);
+          live = x < a.words * 64 && ((mask[k][x >> 6] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, from[k]);
         }
         seen[k] = __ballot_sync(0xffffffffu, live);
         const float mn = fmaxf(m[k], warp_max(live ? s[k] : -INFINITY)), ref = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m[k] - ref);

@@ -157,6 +157,15 @@ __device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int
   if (sh > 32 && w + 1 < words) v |= row[w + 1] << (64 - sh);
   return (uint32_t)v;
 }
+// Of the bits of 32 tree nodes those with a position of `lo` or more (positions: of the first of them; `n` have one).  Trees are seldom as deep as a window: not inlined.
+__device__ __noinline__ uint32_t near_bits(uint32_t bits, const int* positions, int n, int lo) {
+#pragma unroll 1
+  for (uint32_t m = bits; m; m &= m - 1) {
+    const int i = __ffs(m) - 1;
+    if (i >= n || positions[i] < lo) bits &= ~(1u << i);
+  }
+  return bits;
+}
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
 // 128 threads of softmax group g.
@@ -477,7 +486,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int tok = s.q.begin + min(node, s.q.nodes - 1);
       const unsigned long long* mrow = a.mask + (size_t)tok * a.words;
-      const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first place of the context that the row sees
+      const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first position that the row sees
       const int win0 = ctx - a.window + 1, win1 = a.window > 0 ? win0 + s.q.nodes - 1 : 0;         // places in front of win0 are out of every row's window, those in front of win1 out of some row's
       float m = -INFINITY, l = 0.f;
       bool first = true;
@@ -491,7 +500,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int c = 0; c < 4 / FOLD; ++c) {
             const int k0 = kv0 + (fold * (4 / FOLD) + c) * 32;
             see[c] = low_bits(ctx - k0) & ~low_bits(lo - k0);
-            if (tail) see[c] = (see[c] | mask_bits(mrow, a.words, k0 - ctx)) & low_bits(len - k0);
+            if (tail) {
+              uint32_t nodes = mask_bits(mrow, a.words, k0 - ctx);
+              if (lo > ctx && nodes) nodes = near_bits(nodes, a.positions + s.q.begin + k0 - ctx, s.q.nodes - (k0 - ctx), lo);
+              see[c] = (see[c] | nodes) & low_bits(len - k0);
+            }
           }
         }
         ok = __all_sync(0xffffffffu, ta_wait(&s_full[g], s_ph, abort_flag, a.status, 831, b));        // (a warp leaves as one)
@@ -615,7 +628,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int x = 0; x < 512; ++x) {
             if (!((s_odd[x >> 5] >> (x & 31)) & 1)) continue;
             const int at = x < 256 ? ctx + x : win0 + x - 256;
-            if (x < 256 ? x >= a.words * 64 || !((mrow[x >> 6] >> (x & 63)) & 1) : at < lo) continue;
+            if (x < 256 ? x >= a.words * 64 || !((mrow[x >> 6] >> (x & 63)) & 1) || (lo > ctx && (x >= s.q.nodes || a.positions[s.q.begin + x] < lo)) : at < lo) continue;
             const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
             if (slot < 0 || slot >= a.num_slots) continue;
             const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;

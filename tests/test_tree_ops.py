@@ -325,6 +325,61 @@ def test_attention_kernel_window(hq, hkv, n, d, window, ctx):
     check_window(lambda s: tree.tree_attention(**on_gpu(s)), hq, hkv, n, d, window, ctx)
 
 
+def deep_inputs(n, hq, hkv, dk, dv, page, window, dtype=torch.bfloat16):
+    """Trees deeper than the window: a chain, a tree whose branches reach past the window at several depths, and a wide one that does not."""
+    s = attention_inputs([n, n, n], [0, 200, 3], hq, hkv, dk, dv, page, dtype, seed=n + window)
+    r = random.Random(n)
+    masks, pos = [], []
+    for ctx, par in ((0, list(range(-1, n - 1))), (200, [-1] + [max(0, i - r.randint(1, 3)) for i in range(1, n)]), (3, random_tree(n, r, wide=True))):
+        m, d = masks_of(par, s["mask"].shape[1])
+        masks.append(m)
+        pos += [ctx + x for x in d]
+    s.update(mask=torch.cat(masks), positions=torch.tensor(pos, dtype=torch.int32), window=window)
+    return s
+
+
+def by_definition(s):
+    """A node sees the places of the context and the nodes of its mask that are less than ``window`` in front of it, one after the other, in 64 bits."""
+    q, k, v = (s[x].double() for x in ("q", "k_cache", "v_cache"))
+    g, page, out = q.shape[1] // k.shape[1], s["page_size"], torch.zeros(q.shape[0], q.shape[1], v.shape[2], dtype=torch.float64)
+    for seq in range(s["kv_len"].numel()):
+        a, z = int(s["cu_q"][seq]), int(s["cu_q"][seq + 1])
+        ctx, pos = int(s["kv_len"][seq]) - (z - a), s["positions"].tolist()
+        for i in range(a, z):
+            seen = [j for j in range(ctx) if pos[i] - j < s["window"]]
+            seen += [ctx + j for j in range(z - a) if int(s["mask"][i, j // 64]) >> (j % 64) & 1 and pos[i] - pos[a + j] < s["window"]]
+            slot = torch.tensor([int(s["block_table"][seq, j // page]) * page + j % page for j in seen], dtype=torch.long)
+            for h in range(q.shape[1]):
+                w = torch.softmax(k[slot, h // g] @ q[i, h] * math.log(2.0), 0)
+                out[i, h] = w @ v[slot, h // g]
+    return out
+
+
+DEEP = [(9, 4, 2, 128, 128, 16, 4), (30, 8, 2, 64, 64, 16, 10), (100, 4, 1, 128, 64, 32, 70), (140, 2, 2, 64, 128, 64, 33), (12, 6, 3, 80, 72, 16, 1), (70, 2, 1, 320, 300, 48, 20)]
+
+
+@pytest.mark.parametrize("n,hq,hkv,dk,dv,page,window", DEEP)
+def test_attention_plain_window_inside_the_tree(n, hq, hkv, dk, dv, page, window):
+    s = deep_inputs(n, hq, hkv, dk, dv, page, window, torch.float32)
+    assert torch.allclose(tree.tree_attention(**s).double(), by_definition(s), rtol=0, atol=2e-5)      # (sums of a few hundred f32 products, weights that add up to one)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hkv,dk,dv,page,window", DEEP)
+def test_attention_kernel_window_inside_the_tree(n, hq, hkv, dk, dv, page, window, dtype):
+    """Ancestors out of the window count no more than the context out of it: neither finite ones nor those that are no numbers."""
+    s = deep_inputs(n, hq, hkv, dk, dv, page, window, dtype)
+    got = tree.tree_attention(**on_gpu(s))
+    _native.assert_status_ok()
+    close(got, s)
+    # the chain's root: its infinite feature reaches the nodes less than a window behind it, and no others
+    slot = int(s["block_table"][0, 0]) * page
+    s["v_cache"][slot, :, 3] = float("inf")
+    got = tree.tree_attention(**on_gpu(s)).cpu()
+    assert not torch.isfinite(got[:window, :, 3]).any() and torch.isfinite(got[window:]).all() and torch.isfinite(got[:, :, 4:]).all()
+
+
 @gpu
 def test_attention_kernel_single_rows():
     """The strides of dimensions of size one do not matter."""

@@ -244,3 +244,43 @@ def test_trees_with_a_sliding_window_on_gpu():
             row = logits[len(p) - 1 + j]
             assert row[tok] >= row.max() - 0.3 * row.std()
     assert dec.stats.tokens_per_step > 2.0
+
+
+@pytest.mark.parametrize("window,gamma", [(1, 3), (4, 9), (10, 12)])
+@pytest.mark.parametrize("sp", [SamplingParams(), SamplingParams(temperature=0.8, top_k=40, top_p=0.9, seed=5)])
+def test_trees_deeper_than_the_window(window, gamma, sp):
+    """Drafts that reach past the window, as a tree and as a sampled chain: the tokens of decoding without drafts, all drafts accepted."""
+    def make(drafter):
+        cfg = dataclasses.replace(get_config("tiny-dense"), sliding_window=window)
+        kv = KvCache.allocate(cfg, 96, 16, "cpu")
+        return SpeculativeDecoder(Transformer(synthetic_weights(cfg, "bf16", device="cpu", seed=3), kv), kv, 16, 96, drafter)
+    torch.manual_seed(2)
+    prompts = [torch.randint(0, 512, (n,)).tolist() for n in (5, 33)]
+    ref = make(None).generate(prompts, 16, sp=sp)
+    known = [p + o for p, o in zip(prompts, ref)]
+    dec = make(KnowingTrees(known, gamma=gamma))
+    assert dec.generate(prompts, 16, sp=sp) == ref and dec.stats.verify_steps == -(-15 // (gamma + 1))
+    chain = CallableDrafter(lambda t: next((f[len(t): len(t) + gamma] for f in known if list(t) == f[: len(t)]), [7, 7]), gamma=gamma)
+    assert make(chain).generate(prompts, 16, sp=sp) == ref
+
+
+@gpu
+def test_trees_deeper_than_the_window_on_gpu():
+    """Every token is a legitimate greedy choice of the fp32 oracle, with branches of three windows' length."""
+    torch.manual_seed(2)
+    cfg = dataclasses.replace(get_config("tiny-dense"), sliding_window=4)
+    w = synthetic_weights(cfg, "bf16", device="cpu", seed=3).to("cuda")
+
+    def make(drafter):
+        kv = KvCache.allocate(cfg, 96, 16, "cuda")
+        return SpeculativeDecoder(Transformer(w, kv), kv, 16, 96, drafter)
+    prompts = [torch.randint(0, cfg.vocab, (n,)).tolist() for n in (5, 33)]
+    dec = make(KnowingTrees([p + o for p, o in zip(prompts, make(None).generate(prompts, 24))], gamma=12))
+    out = dec.generate(prompts, 24)
+    _native.assert_status_ok()
+    for p, o in zip(prompts, out):
+        logits = reference.reference_logits(w, torch.tensor(list(p) + list(o))[:-1]).float()
+        for j, tok in enumerate(o):
+            row = logits[len(p) - 1 + j]
+            assert row[tok] >= row.max() - 0.3 * row.std()
+    assert dec.stats.tokens_per_step > 4.0
