@@ -957,6 +957,8 @@ class Transformer:
                        x: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Residual stream after layers ``[first_layer, last_layer)`` (pipeline stages pass ``x`` in)."""
         cfg, w = self.cfg, self.w
+        if fb.tree_mask is not None and (cfg.is_layered or cfg.has_recurrent_state):
+            raise NotImplementedError("trees of drafted tokens: every layer one of plain attention")
         last_layer = len(self.runs) if last_layer is None else last_layer
         if x is None and self.stream_f32:
             x = stream.embed(fb.ids, w.embed, cfg.embed_scale) if fb.embeds is None else fb.embeds.float()
@@ -1042,8 +1044,6 @@ class Transformer:
 
     def forward(self, fb: ForwardBatch) -> torch.Tensor:
         """Logits ``f32 [len(logit_rows), V_local]``."""
-        if fb.tree_mask is not None and (self.cfg.is_layered or self.cfg.has_recurrent_state):
-            raise NotImplementedError("trees of drafted tokens: every layer one of plain attention")
         x = self.forward_hidden(fb)
         return self.head(x, fb)
 

@@ -284,3 +284,15 @@ def test_trees_deeper_than_the_window_on_gpu():
             row = logits[len(p) - 1 + j]
             assert row[tok] >= row.max() - 0.3 * row.std()
     assert dec.stats.tokens_per_step > 4.0
+
+
+@pytest.mark.parametrize("name", ["tiny-qwen35", "tiny-fidolix"])
+def test_every_forward_refuses_trees_on_other_models(name):
+    """Recurrent layers would take siblings for a chain."""
+    cfg = get_config(name)
+    kv = KvCache.allocate(cfg, 16, 16, "cpu")
+    m = Transformer(synthetic_weights(cfg, "bf16", device="cpu", seed=3), kv)
+    fb = ForwardBatch.build_tree([0], [[1, 2, 3]], [[-1, 0, 0]], [[0]], 16, "cpu")
+    for call in (m.forward, m.forward_greedy, m.forward_hidden, lambda b: m.forward_hidden(b, 0, 1)):
+        with pytest.raises(NotImplementedError):
+            call(fb)
