@@ -28,8 +28,11 @@ __device__ __forceinline__ float ldt(const __nv_bfloat16* p) { return __bfloat16
 __device__ __forceinline__ void stt(float* p, float v) { *p = v; }
 __device__ __forceinline__ void stt(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 
-// Whether a node lies in a window that begins at position `from` (nodes have positions from ctx on).
-__device__ __forceinline__ bool tree_near(const TreeAnyArgs& a, int token, int ctx, int from) { return from <= ctx || (token < a.tokens && a.positions[token] >= from); }
+// First position in the window of a node (nodes have positions ctx to ctx + nodes - 1), and whether another node lies in a window that begins at position `from`.
+__device__ __forceinline__ int tree_from(const TreeAnyArgs& a, long token, int ctx, int nodes) { return max(0, min(max(a.positions[token], ctx), ctx + nodes - 1) - a.window + 1); }
+__device__ __forceinline__ bool tree_near(const TreeAnyArgs& a, int token, int ctx, int nodes, int from) {
+  return from <= ctx || (token < a.tokens && min(a.positions[token], ctx + nodes - 1) >= from);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(128)
@@ -52,7 +55,7 @@ tree_any_kernel(const TreeAnyArgs a) {
   float* q = s_q + warp * a.dk;
   for (int c = lane; c < a.dk; c += 32) q[c] = ldt((const T*)a.q + (size_t)t * a.q_ts + (size_t)h * a.dk + c);
   __syncwarp();
-  const int from = a.window > 0 ? max(0, a.positions[t] - a.window + 1) : 0, first = min(ctx, from);      // from: the first position in the window
+  const int from = a.window > 0 ? tree_from(a, t, ctx, n_nodes) : 0, first = min(ctx, from);      // from: the first position in the window
   const int* bt = a.block_table + (size_t)seq * a.max_pages;
   float m = -INFINITY, l = 0.f, acc[NV];
 #pragma unroll
@@ -62,7 +65,7 @@ tree_any_kernel(const TreeAnyArgs a) {
     bool live = j < len;
     if (live && j >= ctx) {
       const int x = j - ctx;
-      live = x < a.words * 64 && ((a.mask[(size_t)t * a.words + (x >> 6)] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, from);
+      live = x < a.words * 64 && ((a.mask[(size_t)t * a.words + (x >> 6)] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, n_nodes, from);
     }
     long slot = 0;
     float sc = -INFINITY;
@@ -132,7 +135,7 @@ tree_tile_kernel(const TreeAnyArgs a) {
     const int* bt = a.block_table + (size_t)seq * a.max_pages;
     if (threadIdx.x < kTyRows) {
       const long r = r0 + threadIdx.x;
-      s_lo[threadIdx.x] = a.window > 0 && r >= at && r < to ? max(0, a.positions[r / G] - a.window + 1) : a.window > 0 ? ctx : 0;
+      s_lo[threadIdx.x] = a.window > 0 && r >= at && r < to ? tree_from(a, r / G, ctx, n_nodes) : a.window > 0 ? ctx : 0;
     }
     __syncthreads();
     int first = ctx;
@@ -189,7 +192,7 @@ tree_tile_kernel(const TreeAnyArgs a) {
         if (live && j < ctx) live = j >= from[k];
         else if (live) {
           const int x = j - ctx;
-          live = x < a.words * 64 && ((mask[k][x >> 6] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, from[k]);
+          live = x < a.words * 64 && ((mask[k][x >> 6] >> (x & 63)) & 1) && tree_near(a, begin + x, ctx, n_nodes, from[k]);
         }
         seen[k] = __ballot_sync(0xffffffffu, live);
         const float mn = fmaxf(m[k], warp_max(live ? s[k] : -INFINITY)), ref = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m[k] - ref);

@@ -157,12 +157,12 @@ __device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int
   if (sh > 32 && w + 1 < words) v |= row[w + 1] << (64 - sh);
   return (uint32_t)v;
 }
-// Of the bits of 32 tree nodes those with a position of `lo` or more (positions: of the first of them; `n` have one).  Trees are seldom as deep as a window: not inlined.
-__device__ __noinline__ uint32_t near_bits(uint32_t bits, const int* positions, int n, int lo) {
+// Of the bits of 32 tree nodes those with a position of `lo` or more (positions: of the first of them; `n` have one, of `last` at most).  Trees are seldom as deep as a window: not inlined.
+__device__ __noinline__ uint32_t near_bits(uint32_t bits, const int* positions, int n, int lo, int last) {
 #pragma unroll 1
   for (uint32_t m = bits; m; m &= m - 1) {
     const int i = __ffs(m) - 1;
-    if (i >= n || positions[i] < lo) bits &= ~(1u << i);
+    if (i >= n || min(positions[i], last) < lo) bits &= ~(1u << i);
   }
   return bits;
 }
@@ -486,7 +486,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int tok = s.q.begin + min(node, s.q.nodes - 1);
       const unsigned long long* mrow = a.mask + (size_t)tok * a.words;
-      const int lo = a.window > 0 ? a.positions[tok] - a.window + 1 : 0;      // first position that the row sees
+      const int last_pos = ctx + s.q.nodes - 1;                                // nodes have positions ctx to this
+      const int lo = a.window > 0 ? min(max(a.positions[tok], ctx), last_pos) - a.window + 1 : 0;      // first position that the row sees
       const int win0 = ctx - a.window + 1, win1 = a.window > 0 ? win0 + s.q.nodes - 1 : 0;         // places in front of win0 are out of every row's window, those in front of win1 out of some row's
       float m = -INFINITY, l = 0.f;
       bool first = true;
@@ -502,7 +503,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             see[c] = low_bits(ctx - k0) & ~low_bits(lo - k0);
             if (tail) {
               uint32_t nodes = mask_bits(mrow, a.words, k0 - ctx);
-              if (lo > ctx && nodes) nodes = near_bits(nodes, a.positions + s.q.begin + k0 - ctx, s.q.nodes - (k0 - ctx), lo);
+              if (lo > ctx && nodes) nodes = near_bits(nodes, a.positions + s.q.begin + k0 - ctx, s.q.nodes - (k0 - ctx), lo, last_pos);
               see[c] = (see[c] | nodes) & low_bits(len - k0);
             }
           }
@@ -628,7 +629,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int x = 0; x < 512; ++x) {
             if (!((s_odd[x >> 5] >> (x & 31)) & 1)) continue;
             const int at = x < 256 ? ctx + x : win0 + x - 256;
-            if (x < 256 ? x >= a.words * 64 || !((mrow[x >> 6] >> (x & 63)) & 1) || (lo > ctx && (x >= s.q.nodes || a.positions[s.q.begin + x] < lo)) : at < lo) continue;
+            if (x < 256 ? x >= a.words * 64 || !((mrow[x >> 6] >> (x & 63)) & 1) || (lo > ctx && (x >= s.q.nodes || min(a.positions[s.q.begin + x], last_pos) < lo)) : at < lo) continue;
             const long slot = (long)a.block_table[(size_t)s.seq * a.max_pages + at / a.page_size] * a.page_size + at % a.page_size;
             if (slot < 0 || slot >= a.num_slots) continue;
             const __nv_bfloat16* vr = a.v_cache + ((size_t)slot * a.hkv + s.kvh) * DV + c * 32;

@@ -28,7 +28,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``k_cache [slots, Hkv, dk]`` / ``v_cache [slots, Hkv, dv]``.  Sequence s has the nodes ``cu_q[s] .. cu_q[s + 1]`` (at most ``max_nodes`` <= 256), cached at
     its last places.  A node sees the places in front of the tree and the nodes whose bits are set in its row of ``mask`` (int64 ``[T, words]``, its own bit among
     them as a rule); with ``window`` > 0, of both those that are less than ``window`` in front of its ``positions`` entry (a place of the context by its number, a
-    node by its own entry).  A node that sees nothing gets zeros; rows behind the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not
+    node by its own entry; ``ctx + depth`` as ``ops.paging.batch_tables`` makes them: an entry outside ``ctx .. ctx + nodes - 1`` counts as the nearest of these).  A node that sees nothing gets zeros; rows behind the last sequence stay as they were in ``out``.  Keys that a node does not see never count, even if their rows are not
     finite; a value that is not finite makes that feature of the nodes that see it not finite."""
     t, hq, dk = q.shape
     slots, hkv, dv = v_cache.shape
@@ -112,7 +112,7 @@ def tree_attention_ref(q, k_cache, v_cache, cu_q, kv_len, block_table, page_size
         bits = mask[a:z][:, (off >> 6).clamp(0, mask.shape[1] - 1)] >> (off & 63) & 1
         see = (off < 0) | ((bits == 1) & (off < 64 * mask.shape[1]))
         if window > 0:
-            pos = positions[a:z].long()
+            pos = positions[a:z].long().clamp(ctx, ctx + z - a - 1)
             see &= torch.where(off < 0, place, pos[off.clamp(0, z - a - 1)]) > pos[:, None] - window
         k = k_cache[slot].to(wide).repeat_interleave(g, dim=1)
         v = v_cache[slot].to(wide).repeat_interleave(g, dim=1)

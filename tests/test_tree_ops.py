@@ -380,6 +380,39 @@ def test_attention_kernel_window_inside_the_tree(n, hq, hkv, dk, dv, page, windo
     assert not torch.isfinite(got[:window, :, 3]).any() and torch.isfinite(got[window:]).all() and torch.isfinite(got[:, :, 4:]).all()
 
 
+def stray_positions(dk, dtype):
+    """Positions in front of the context and behind the last node's, and the same as the operator takes them: the nearest that a node can have."""
+    n, ctx, window = 40, (0, 300, 1000), 20
+    s = attention_inputs([n, n, n], list(ctx), 4, 2, dk, dk, 16, dtype, seed=3)
+    g = torch.Generator().manual_seed(4)
+    s["window"] = window
+    s["positions"] = s["positions"] + torch.randint(-200, 200, (3 * n,), generator=g, dtype=torch.int32)
+    s["positions"][::7], s["positions"][1::7] = -2 ** 31, 2 ** 31 - 1
+    first = torch.tensor(ctx).repeat_interleave(n)
+    return s, {**s, "positions": s["positions"].long().clamp(first, first + n - 1).int()}
+
+
+def test_attention_plain_stray_positions():
+    s, taken = stray_positions(64, torch.float32)
+    got = tree.tree_attention(**s)
+    assert torch.equal(got, tree.tree_attention(**taken)) and torch.allclose(got.double(), by_definition(taken), rtol=0, atol=2e-5)
+
+
+@gpu
+@pytest.mark.parametrize("dk,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32), (320, torch.float32)])
+def test_attention_kernel_stray_positions(dk, dtype):
+    """Both kernels answer alike, and what no row sees stays out, even where it is no number."""
+    s, taken = stray_positions(dk, dtype)
+    for seq, ctx in enumerate((0, 300, 1000)):
+        place = torch.arange(max(0, ctx - 20 + 1))                         # in front of every window
+        slot = s["block_table"][seq].long()[place // 16] * 16 + place % 16
+        for x in ("k_cache", "v_cache"):
+            s[x][slot] = float("nan")
+    got = tree.tree_attention(**on_gpu(s))
+    _native.assert_status_ok()
+    close(got, taken)
+
+
 @gpu
 def test_attention_kernel_single_rows():
     """The strides of dimensions of size one do not matter."""
