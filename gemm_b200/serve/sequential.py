@@ -73,7 +73,7 @@ class SequentialLLM:
             kth = torch.topk(row, min(sp.top_k, row.numel())).values[-1]
             row = row.masked_fill(row < kth, float("-inf"))
         p = torch.softmax(row, dim=-1)
-        low = p < sp.min_p * p.max()
+        low = p < min(sp.min_p, 1.0) * p.max()
         if sp.top_p < 1.0:
             sp_, idx = torch.sort(p, descending=True)
             cut = (torch.cumsum(sp_, 0) - sp_) > sp.top_p

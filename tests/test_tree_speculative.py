@@ -296,3 +296,13 @@ def test_every_forward_refuses_trees_on_other_models(name):
     for call in (m.forward, m.forward_greedy, m.forward_hidden, lambda b: m.forward_hidden(b, 0, 1)):
         with pytest.raises(NotImplementedError):
             call(fb)
+
+
+def test_sequential_min_p_above_one():
+    """A min-p above 1 counts as 1, as in ``sampling.draw``: the likeliest token alone."""
+    from gemm_b200.serve.sequential import SequentialLLM
+    x = torch.randn(1, 50, generator=torch.Generator().manual_seed(0))
+    for min_p in (1.0, 1.5, 40.0):
+        for top_p in (1.0, 0.5):
+            sp = SamplingParams(temperature=0.7, top_p=top_p, min_p=min_p)
+            assert SequentialLLM._pick(None, x, sp, 0) == int(x.argmax()) == int(sampling.draw(x, torch.tensor([0.5]), 0.7, 0, top_p, min_p)[0])
