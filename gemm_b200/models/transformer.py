@@ -256,14 +256,15 @@ class ForwardBatch:
     def build_paged(q_lens: Sequence[int], ctx_lens: Sequence[int], ids: Sequence[int], pages: Sequence[Sequence[int]], page_size: int, hq: int, hkv: int, device,
                     seq_slots: Optional[Sequence[int]] = None, rows: Optional[Sequence[int]] = None) -> "ForwardBatch":
         """``build`` from the sequences' page lists.  On a GPU the lengths, lists and ids go there in one copy and the tables are made there
-        (``ops.paging.batch_tables``).  ``rows``: the rows of logits that are wanted (default: each sequence's last token)."""
-        if torch.device(device).type == "cpu":
+        (``ops.paging.batch_tables``; more sequences than that takes are assembled on the host).  ``rows``: the rows of logits that are wanted (default: each sequence's
+        last token)."""
+        if torch.device(device).type == "cpu" or len(q_lens) > paging.MAX_SEQS:
             bt = torch.zeros(len(pages), max((len(p) for p in pages), default=0), dtype=torch.int32)
             for i, p in enumerate(pages):
                 bt[i, : len(p)] = torch.tensor(p, dtype=torch.int32)
             fb = ForwardBatch.build(q_lens, ctx_lens, ids, bt, page_size, hq, hkv, device, seq_slots=seq_slots)
             if rows is not None:
-                fb.logit_rows = torch.tensor(list(rows), dtype=torch.int64)
+                fb.logit_rows = torch.tensor(list(rows), dtype=torch.int64, device=device)
             return fb
         b = len(q_lens)
         ql, ctx = att.whole_numbers(q_lens), att.whole_numbers(ctx_lens)

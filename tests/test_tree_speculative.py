@@ -9,7 +9,7 @@ from gemm_b200.models import reference
 from gemm_b200.models.config import get_config
 from gemm_b200.models.transformer import ForwardBatch, KvCache, Transformer
 from gemm_b200.models.weights import synthetic_weights
-from gemm_b200.ops import sampling, tree
+from gemm_b200.ops import paging, sampling, tree
 from gemm_b200.serve.engine import Engine, SamplingParams
 from gemm_b200.serve.llm import LLM
 from gemm_b200.serve.speculative import CallableDrafter, NgramTreeDrafter, SpeculativeDecoder
@@ -306,3 +306,24 @@ def test_sequential_min_p_above_one():
         for top_p in (1.0, 0.5):
             sp = SamplingParams(temperature=0.7, top_p=top_p, min_p=min_p)
             assert SequentialLLM._pick(None, x, sp, 0) == int(x.argmax()) == int(sampling.draw(x, torch.tensor([0.5]), 0.7, 0, top_p, min_p)[0])
+
+
+@gpu
+def test_build_paged_of_more_sequences_than_the_table_kernel_takes():
+    """A step of any number of sequences is assembled, as ``build`` does it."""
+    n = paging.MAX_SEQS + 300
+    q, ctx = [1 + i % 3 for i in range(n)], [i % 40 for i in range(n)]
+    have = [(a + b + 15) // 16 for a, b in zip(q, ctx)]
+    at = [0] + torch.tensor(have).cumsum(0).tolist()
+    pages = [list(range(at[i], at[i + 1])) for i in range(n)]
+    bt = torch.zeros(n, max(have), dtype=torch.int32)
+    for i, p in enumerate(pages):
+        bt[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
+    want = ForwardBatch.build(q, ctx, list(range(sum(q))), bt, 16, 8, 2, "cuda")
+    for count in (paging.MAX_SEQS, n):
+        got = ForwardBatch.build_paged(q[:count], ctx[:count], list(range(sum(q[:count]))), pages[:count], 16, 8, 2, "cuda", rows=[3, 0])
+        t = sum(q[:count])
+        for name, x in (("ids", t), ("positions", t), ("slots", t), ("cu_q", count + 1), ("kv_len", count), ("block_table", count), ("seq_slots", count)):
+            a, b = getattr(got, name), getattr(want, name)[:x]
+            assert torch.equal(a, b) and a.dtype == b.dtype, name
+        assert got.logit_rows.tolist() == [3, 0] and got.logit_rows.is_cuda and got.n_tokens == t
