@@ -151,6 +151,8 @@ def cmd_generate(args):
         if not (_is_gemma4(args.model) and args.audio_model):
             sys.exit("--audio needs a gemma4 GGUF as --model and --audio-model <checkpoint with the audio tower>")
         return _generate_with_audio(args)
+    if args.tree > 1 and args.speculative <= 0:
+        sys.exit("--tree shapes the drafts of --speculative: give that too")
     llm = _load_llm(args)
     prompts = args.prompt or ["Hello"]
     sp = SamplingParams(max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, seed=args.seed, min_p=args.min_p)
@@ -168,8 +170,11 @@ def cmd_generate(args):
         sys.exit("--speculative needs the continuous-batching engine: this model family is served one request at a time")
     if args.speculative > 0:
         from .serve.speculative import NgramTreeDrafter
-        drafter = NgramTreeDrafter(gamma=args.speculative, width=args.tree) if args.tree > 1 else None
-        outs, stats = llm.generate_speculative(enc, args.max_new_tokens, gamma=args.speculative, drafter=drafter, sp=sp)
+        try:
+            drafter = NgramTreeDrafter(gamma=args.speculative, width=args.tree) if args.tree > 1 else None
+            outs, stats = llm.generate_speculative(enc, args.max_new_tokens, gamma=args.speculative, drafter=drafter, sp=sp)
+        except ValueError as e:                         # (models and drafts that cannot be verified in one step)
+            sys.exit(f"--speculative: {e}")
     else:
         outs = llm.generate(enc, sp)
     dt = time.time() - t0

@@ -88,6 +88,16 @@ def test_generate_speculative_flag_gives_the_greedy_tokens(capsys):
     assert summary["verify_steps"] <= 9 and "draft_acceptance" in summary
 
 
+@pytest.mark.parametrize("model,flags,says", [
+    ("tiny-dense", ["--tree", "3"], "--speculative"), ("tiny-fidolix", ["--speculative", "2", "--tree", "2"], "recurrent"), ("tiny-qwen35", ["--speculative", "2"], "recurrent"),
+    ("tiny-dense", ["--speculative", "3", "--tree", "300"], "256")])
+def test_generate_says_what_speculation_cannot_do(model, flags, says):
+    """A message instead of a traceback, and no flag that is passed over."""
+    with pytest.raises(SystemExit) as e:
+        main(["generate", "--model", f"synthetic:{model}", "--device", "cpu", "--ids", "--prompt", "1 2 3 1 2", "--max-new-tokens", "3", "--pages", "16", "--page-size", "16"] + flags)
+    assert isinstance(e.value.code, str) and says in e.value.code
+
+
 def test_speculative_speedup_model():
     from gemm_b200.utils.estimate import speculative_speedup
     r = speculative_speedup(1.0, 4, 1.38)
