@@ -5,8 +5,8 @@
 //
 // All three filters cut that order at one place, so what is kept is {key > tau} and the first m ids with key = tau.  No sort: tau comes from radix searches.
 //
-// Masses are whole numbers: w_i is rounded to a multiple of 2^-44 (the rounding moves a border of the draw by 2^-45 of the largest weight; 2^18 of them stay
-// below 2^63).  Sums are then exact in any order: the atomics of the histograms, the split over blocks and the order of the warps change nothing, and the
+// Masses are whole numbers: w_i is rounded to a multiple of 2^-44 (the rounding moves a border of the draw by 2^-45 of the largest weight).  A row has fewer than 2^20
+// ids (eight blocks' shared memory holds no more), so a mass is below 2^64, and every sum is unsigned.  Sums are then exact in any order: the atomics of the histograms, the split over blocks and the order of the warps change nothing, and the
 // draw agrees with one in 64-bit floats except where u falls within some 1e-12 of a border (32-bit sums over a vocabulary: a row in a thousand).
 // 2^t: table of 2^(j/32) and a polynomial for the rest (P. T. P. Tang, "Table-driven implementation of the exponential function", 1989), in 64-bit floats.
 //
@@ -39,6 +39,7 @@ constexpr int kDrMass = 44;                // fraction bits of a weight
 // 2500 527 and 479; 8000 f32 rows of 4000 323 and 324.
 constexpr int kDrShort = 2048;
 constexpr size_t kDrSmem = 202000;         // bytes of logits that a block holds at most
+static_assert(8 * kDrSmem / sizeof(__nv_bfloat16) < 1ull << (64 - kDrMass), "the mass of a row, at most 2^kDrMass for each id, fits 64 bits");
 
 struct DrawArgs {
   const void* logits;

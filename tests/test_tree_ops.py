@@ -639,6 +639,22 @@ def test_draw_kernel_borders_and_strides():
 
 
 @gpu
+def test_draw_kernel_largest_masses():
+    """Rows of as many ids as there is room for, all or nearly all equal: masses beyond 2^63."""
+    v = 800_000
+    r = random.Random(0)
+    x = torch.full((12, v), 1.5)
+    x[6:, torch.randint(0, v, (1000,), generator=torch.Generator().manual_seed(1))] = 1.0
+    f = lambda vs: torch.tensor(vs, dtype=torch.float32)                   # noqa: E731
+    s = dict(logits=x.bfloat16(), uniform=f([r.random() for _ in range(12)]), temperature=f([1.0] * 6 + [0.7, 1e9] * 3), top_k=torch.tensor([0, 0, 0, 700_000, 799_999, 0] * 2, dtype=torch.int32),
+             top_p=f([1.0, 0.9, 0.99999, 1.0, 0.95, 0.3] * 2), min_p=f([0.0, 0.0, 0.5, 0.0, 0.0, 1.0] * 2))
+    s["uniform"][0] = 1 - 2 ** -24
+    got = sampling.draw(**on_gpu(s), want_logprob=True)
+    _native.assert_status_ok()
+    same_draws(got, s)
+
+
+@gpu
 def test_draw_kernel_frequencies():
     """Evenly spaced numbers meet every kept id as often as its probability says, to one number."""
     g = torch.Generator().manual_seed(0)
