@@ -655,6 +655,23 @@ def test_draw_kernel_largest_masses():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [3, 60])
+def test_draw_kernel_likely_tokens_side_by_side(rows, dtype):
+    """The likely tokens at neighbouring ids: one block of a row's cluster holds all candidates, more than its share of the places."""
+    s = draw_rows(rows, 151936, dtype, rows, "normal")
+    r = random.Random(rows)
+    for row in s["logits"]:
+        at = r.choice([0, 70_000, 150_000])
+        row[at:at + 1500] += 12
+    s["top_k"] = torch.tensor([r.choice([0, 200, 300, 700, 1000, 1400]) for _ in range(rows)], dtype=torch.int32)
+    s["temperature"].fill_(1.1)
+    got = sampling.draw(**on_gpu(s), want_logprob=True)
+    _native.assert_status_ok()
+    same_draws(got, s)
+
+
+@gpu
 def test_draw_kernel_frequencies():
     """Evenly spaced numbers meet every kept id as often as its probability says, to one number."""
     g = torch.Generator().manual_seed(0)
