@@ -29,7 +29,9 @@ namespace gb {
 constexpr int kTaThreads = 384;     // warps 0-3, 4-7: softmax groups; 8: K / V loads; 9: MMA; 10: Q loads; 11: segments
 constexpr int kTaTiles = 7;         // 32 KB tiles of shared memory: one or two of Q, one in which rows are joined and put in order, the rest is the ring
 // Items of as many blocks or fewer are not cut (no parts to write and join).  64 sequences of 8 nodes on 500 places each: 24 us, cut 29; on 10 to 500: 24.4, cut 26.4; on 10 to
-// 1000 (8 blocks): 35.4, cut 33.6.  With a window most items have the same length: windows of 1000 in 10 blocks, 29 us, cut 34, if the items go round the SMs.
+// 1000 (8 blocks): 35.4, cut 33.6.  With a window most items have the same length, and whole ones are faster where the last round of the SMs leaves half of them idle at most.
+// Whole / cut in us, windows of 1000, 12 nodes, heads of 128, on 148 SMs: 80 items 23 / 24, 144 24 / 31, 150 41 / 32, 200 42 / 38, 294 44 / 48, 304 59 / 51, 400 61 / 61, 592 79 / 83,
+// 800 114 / 108, 1024 135 to 140 / 137; heads of 64: 144 20 / 24, 150 33 / 25, 294 38 / 41, 304 50 / 44; windows of 512, heads of 128: 144 20 / 24, 150 29 / 25, 294 36 / 40, 400 50 / 47, 800 94 / 80, 1024 109 / 103.
 constexpr int kTaWhole = 4, kTaWholeWindow = 12;
 constexpr int kTaSegs = 4;          // segments handed out ahead
 constexpr int kTaSide = 3 * 1024;   // bytes beside the tiles
@@ -780,7 +782,8 @@ static int tree_attn_grid(int n_seqs, int max_pages, int page_size, int max_node
   long blocks = std::max(1l, ((long)max_pages * page_size + 127) / 128);
   if (window > 0) blocks = std::min(blocks, ((long)window + max_nodes + 126) / 128 + 1);
   const long items = (long)n_seqs * hkv * ((tiles + *pair - 1) / *pair);
-  *whole = blocks <= kTaWhole || (window > 0 && blocks <= kTaWholeWindow && 2 * items > sm_count());
+  const long idle = sm_count() - 1 - (items + sm_count() - 1) % sm_count();      // SMs without an item in the last round
+  *whole = blocks <= kTaWhole || (window > 0 && blocks <= kTaWholeWindow && 2 * idle <= sm_count());
   if (items * *pair * (blocks + 8) > 1l << 30) return 0;
   return (int)std::max(1l, std::min((long)sm_count(), *whole ? items : (items * blocks + 1) / 2));
 }

@@ -414,6 +414,17 @@ def test_attention_kernel_stray_positions(dk, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("seqs,hkv", [(24, 6), (25, 6), (37, 4), (38, 8)])
+def test_attention_kernel_windows_around_a_round(seqs, hkv):
+    """As many windowed items as there are SMs, some fewer and some more: left whole, or cut."""
+    r = random.Random(seqs)
+    s = attention_inputs([r.randint(1, 9) for _ in range(seqs)], [r.randint(0, 900) for _ in range(seqs)], 2 * hkv, hkv, 64, 64, 16, seed=seqs)
+    s["window"] = 600
+    close(tree.tree_attention(**on_gpu(s)), s)
+    _native.assert_status_ok()
+
+
+@gpu
 def test_attention_kernel_single_rows():
     """The strides of dimensions of size one do not matter."""
     for nodes, hq, hkv in (([1], 4, 2), ([3], 1, 1)):
