@@ -205,7 +205,7 @@ class Engine:
     def _sample(self, logits: torch.Tensor, sp: SamplingParams, step: int, step_ctr: Optional[torch.Tensor] = None,
                 uniform: Optional[torch.Tensor] = None) -> torch.Tensor:
         if sp.temperature > 0 and sp.min_p > 0:
-            if hasattr(self.par, "merge_sampled"):
+            if logits.shape[1] != self.cfg.vocab:
                 raise NotImplementedError("min-p needs an unsharded LM head")
             if uniform is None:
                 uniform = sampling.uniform_numbers(sp.seed, step, logits.shape[0]).to(logits.device)

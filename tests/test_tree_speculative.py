@@ -327,3 +327,20 @@ def test_build_paged_of_more_sequences_than_the_table_kernel_takes():
             a, b = getattr(got, name), getattr(want, name)[:x]
             assert torch.equal(a, b) and a.dtype == b.dtype, name
         assert got.logit_rows.tolist() == [3, 0] and got.logit_rows.is_cuda and got.n_tokens == t
+
+
+def test_engine_min_p_with_ranks_that_hold_the_whole_head():
+    """Tensor-parallel ranks with an unsharded LM head draw alike, each for itself; a share of the vocabulary is refused."""
+    cfg = get_config("tiny-dense")
+    e = Engine(synthetic_weights(cfg, "bf16", device="cpu", seed=3), 2, 64, page_size=16)
+    logits = torch.randn(2, cfg.vocab, generator=torch.Generator().manual_seed(0))
+    sp = SamplingParams(temperature=1.3, min_p=0.01, seed=5)
+    want = e._sample(logits, sp, 3)
+
+    class Ranks:
+        def merge_sampled(self, tok, logits):
+            raise AssertionError("there is nothing to merge")
+    e.par = Ranks()
+    assert torch.equal(e._sample(logits, sp, 3), want)
+    with pytest.raises(NotImplementedError):
+        e._sample(logits[:, :256].contiguous(), sp, 3)
