@@ -295,6 +295,8 @@ class ForwardBatch:
             raise ValueError(f"trees of 1 to {paging.MAX_NODES} nodes with a parent each are needed")
         if any(p[0] != -1 or any(not 0 <= x < i for i, x in enumerate(p) if i) for p in parents):
             raise ValueError("a node's parent comes in front of it, and the first node has none")
+        if ctx.size != ql.size or have.size != ql.size or (ctx < 0).any():
+            raise ValueError("context lengths and page lists name different sequences than the trees")
         if (ctx + ql > have * page_size).any():
             raise IndexError("a sequence has more tokens than its pages hold")
         t = int(ql.sum())

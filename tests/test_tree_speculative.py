@@ -298,6 +298,16 @@ def test_every_forward_refuses_trees_on_other_models(name):
             call(fb)
 
 
+def test_build_tree_refuses_negative_contexts():
+    for ctx in ([-1], [4, -2]):
+        n = len(ctx)
+        with pytest.raises(ValueError):
+            ForwardBatch.build_tree(ctx, [[1, 2]] * n, [[-1, 0]] * n, [[0]] * n, 16, "cpu")
+    for bad in (dict(ctx_lens=[0]), dict(parents=[[-1, 0]]), dict(pages=[[0]]), dict(parents=[[-1, 0]] * 3)):
+        with pytest.raises(ValueError):
+            ForwardBatch.build_tree(**{**dict(ctx_lens=[0, 0], tokens=[[1, 2]] * 2, parents=[[-1, 0]] * 2, pages=[[0], [1]], page_size=16, device="cpu"), **bad})
+
+
 def test_sequential_min_p_above_one():
     """A min-p above 1 counts as 1, as in ``sampling.draw``: the likeliest token alone."""
     from gemm_b200.serve.sequential import SequentialLLM
