@@ -430,7 +430,8 @@ def main(argv=None):
     g.add_argument("--audio", default="", help="16 kHz WAV clip for a gemma4 model; write <audio> in the prompt where it belongs")
     g.add_argument("--audio-model", default="", help="safetensors checkpoint holding the gemma4 audio tower")
     g.add_argument("--speculative", type=int, default=0, metavar="GAMMA",
-                   help="speculative decoding with prompt-lookup drafts of up to GAMMA tokens, verified in one batched step")
+                   help="speculative decoding with prompt-lookup drafts of up to GAMMA tokens, verified in one batched step (greedy: the same text; "
+                        "sampled: drawn with other numbers than without)")
     g.add_argument("--tree", type=int, default=1, metavar="WIDTH", help="with --speculative: trees of drafts, from the last WIDTH places where the context occurred")
     g.set_defaults(fn=cmd_generate)
     s = sub.add_parser("serve", help="HTTP server")

@@ -36,7 +36,9 @@ class SamplingParams:
     top_p: float = 1.0
     seed: int = 0
     stop_token_ids: Sequence[int] = ()
-    min_p: float = 0.0                # tokens less likely than this times the likeliest one are left out (drawn by ops.sampling.draw)
+    # tokens less likely than this times the likeliest one are left out.  Drawn by ops.sampling.draw then: in the order of ids, from all that is kept, where
+    # ops.sampling.sample goes by probability over 1024 candidates at most; so the same seed gives other tokens than without a min-p
+    min_p: float = 0.0
 
 
 class PageAllocator:

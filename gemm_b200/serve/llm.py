@@ -244,9 +244,11 @@ class LLM:
 
     def generate_speculative(self, prompts: Sequence, max_new_tokens: int = 64, gamma: int = 4, drafter=None,
                              stop_token_ids: Sequence[int] = (), sp: Optional[SamplingParams] = None):
-        """Generation with speculative decoding (``serve/speculative.py``): same tokens as without drafts, fewer model steps when they hit.  Greedy, or with the
-        temperature, top-k, top-p, min-p and seed of ``sp``; chains of drafts, or trees (``NgramTreeDrafter``).  Uses the whole cache, so no request may be in
-        flight.  Returns (outputs, statistics)."""
+        """Generation with speculative decoding (``serve/speculative.py``): chains of drafts, or trees (``NgramTreeDrafter``), fewer model steps when they hit.  Greedy:
+        the tokens of greedy ``generate``.  With the temperature, top-k, top-p, min-p and seed of ``sp`` (its length limit and stop tokens are not looked at, those
+        are the arguments'): the tokens that this call draws without drafts.  ``generate`` draws other ones: without a min-p by ``sampling.sample``, which keeps 1024
+        candidates at most, and with a number of its own for each request, not for each place in the call.  Uses the whole cache, so no request may be in flight.
+        Returns (outputs, statistics)."""
         from .speculative import NgramDrafter, SpeculativeDecoder
         if self.has_work():
             raise RuntimeError("speculative generation needs an idle engine")

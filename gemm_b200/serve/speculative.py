@@ -11,7 +11,7 @@ That holds for attention layers only: recurrent (Delta-Net) state cannot be rewo
 Drafts may also form a TREE (several continuations that share their beginnings), and generation may be sampled.  One forward over all nodes (a node sees the
 context and its ancestors), one draw per node, and the path along the drafts that equal the tokens drawn at their parents is kept: its K / V rows move
 behind the context (``ops.tree``).  The numbers that a token is drawn with depend on the seed, the sequence and the place of the token alone, so that the output equals
-sampling without drafts token for token.
+what the decoder samples without drafts, token for token (where the logits' rounding, which may differ between steps of different sizes, does not decide).
 
 Four drafters are provided: ``NgramDrafter`` (prompt lookup: continue the most recent earlier occurrence of the current
 suffix; needs no second model), ``NgramTreeDrafter`` (the continuations of its last few occurrences as a tree), ``ModelDrafter`` (a smaller model of the same vocabulary with its own paged cache, batched
